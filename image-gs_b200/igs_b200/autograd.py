@@ -6,6 +6,9 @@ Differentiable operators of the training step, with the semantics of the referen
   - quantize_ste: the straight-through step quantization of model.py:993-1006
   - rate_loss (compress/rate.py:178-202)
   - l1_loss: ratio * F.l1_loss in one pass that keeps the signs for the backward pass; install_l1() routes model.py's F.l1_loss to it
+and, over the top-K lists pixel_topk [H, W, 10] of nd_rasterize_forward_topk_norm, two regularizers of the routing:
+  - topk_balance: how the pixels spread over the Gaussians (counts, importance) and the balance loss
+  - rasterize_topk_dropout: the render with gates dropped before the normalization, the mask drawn again in the backward pass
 
 The rasterization's autograd path keeps each pixel's top-K lists in the 16-bit tile-list form (positions in the tile's list; a quarter of
 the bytes of the reference's [H, W, 10] int32 ids); the backward pass selects the lists of a tile again when its list reaches 65535
@@ -16,6 +19,7 @@ from typing import Optional
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -150,6 +154,61 @@ def rate_loss(feat, rot, l1_loss, model, inv_rot_step, l1_ratio, factor):
     """factor / max(l1_loss / l1_ratio, 1e-4) times the smooth Laplace bits of the features and rotations (compress/rate.py:197-202);
     `model` carries the fields of compress.rate.RateModel."""
     return _RateLoss.apply(feat, rot, l1_loss.detach(), model, inv_rot_step, l1_ratio, factor)
+
+
+class _TopkBalance(Function):
+    @staticmethod
+    def forward(ctx, xys, conics, pixel_topk, img_height, img_width, pixel_mask):
+        loss, counts, importance, totals = ops.topk_balance_forward(img_height, img_width, xys, conics, pixel_topk, pixel_mask)
+        ctx.img_height, ctx.img_width = img_height, img_width
+        ctx.save_for_backward(xys, conics, pixel_topk, counts, totals, pixel_mask)
+        ctx.mark_non_differentiable(counts, totals)
+        ctx.set_materialize_grads(False)
+        return loss, counts, importance, totals
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_loss, v_counts, v_importance, v_totals):
+        if v_loss is None and v_importance is None:
+            return (None,) * 6
+        xys, conics, pixel_topk, counts, totals, pixel_mask = ctx.saved_tensors
+        v_loss, v_importance = (None if v is None else v.contiguous() for v in (v_loss, v_importance))
+        v_xy, v_conic = ops.topk_balance_backward(ctx.img_height, ctx.img_width, xys, conics, pixel_topk, counts, totals, v_loss,
+                                                  v_importance, pixel_mask)
+        return v_xy, v_conic, None, None, None, None
+
+
+def topk_balance(xys, conics, pixel_topk, img_height, img_width, pixel_mask=None):
+    """(loss, counts, importance, totals) of ops.topk_balance_forward; loss and importance are differentiable in xys and conics (the counts
+    are constants of the gradient, as in any balance loss over a top-K choice)."""
+    return _TopkBalance.apply(xys.contiguous(), conics.contiguous(), pixel_topk.contiguous(), int(img_height), int(img_width),
+                              None if pixel_mask is None else pixel_mask.contiguous())
+
+
+class _RasterizeTopkDropout(Function):
+    @staticmethod
+    def forward(ctx, xys, conics, colors, pixel_topk, img_height, img_width, p, rng_state):
+        out_img, rng_used = ops.topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk, p, rng_state)
+        ctx.img_height, ctx.img_width, ctx.p = img_height, img_width, p
+        ctx.save_for_backward(xys, conics, colors, pixel_topk, rng_used)
+        return out_img.permute(1, 2, 0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_out_img):
+        xys, conics, colors, pixel_topk, rng_used = ctx.saved_tensors
+        v_output = v_out_img.permute(2, 0, 1).contiguous()
+        v_xy, v_conic, v_colors = ops.topk_dropout_backward(ctx.img_height, ctx.img_width, xys, conics, colors, v_output, pixel_topk,
+                                                            ctx.p, rng_used)
+        return v_xy, v_conic, v_colors, None, None, None, None, None
+
+
+def rasterize_topk_dropout(xys, conics, colors, pixel_topk, img_height, img_width, p, rng_state):
+    """The render [H, W, C] (a view of a channel-planar buffer, as rasterize_gaussians_sum's) from the lists pixel_topk with every slot
+    dropped with probability p before the weights are normalized. rng_state: int64 [2] on the device, seed and offset; the backward pass
+    draws the mask that the forward pass drew, whatever rng_state holds by then."""
+    return _RasterizeTopkDropout.apply(xys.contiguous(), conics.contiguous(), colors.contiguous(), pixel_topk.contiguous(),
+                                       int(img_height), int(img_width), float(p), rng_state)
 
 
 class _L1Loss(Function):

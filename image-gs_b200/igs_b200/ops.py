@@ -293,6 +293,137 @@ def topk_feature_weights(img_height, img_width, xys, conics, pixel_topk, eps=EPS
     return topk_feature_weights_fixed(img_height, img_width, xys, conics, pixel_topk, eps).to(torch.float64) / 2.0**40
 
 
+# ---- routing lists: balance and gate dropout ------------------------------------------------------------------------------------------
+
+def _check_lists(img_height, img_width, xys, conics, pixel_topk, **others):
+    """The inputs shared by the operators over pixel_topk: shapes, types, one device. Returns (H, W, N, device)."""
+    h, w = int(img_height), int(img_width)
+    if h < 0 or w < 0:
+        raise ValueError(f"negative image size {w}x{h}")
+    _check_input(xys, "xys", torch.float32)
+    _check_input(conics, "conics", torch.float32)
+    _check_input(pixel_topk, "pixel_topk", torch.int32)
+    if xys.ndim != 2 or xys.size(1) != 2:
+        raise RuntimeError("xys must have dimensions (num_points, 2)")
+    n = xys.size(0)
+    if tuple(conics.shape) != (n, 3):
+        raise RuntimeError("conics must have dimensions (num_points, 3)")
+    if pixel_topk.numel() != h * w * TOP_K:
+        raise RuntimeError("pixel_topk must be [H, W, TOP_K]")
+    for name, t in dict(conics=conics, pixel_topk=pixel_topk, **others).items():
+        if t is not None and t.device != xys.device:
+            raise RuntimeError(f"{name} must be on {xys.device}, as xys")
+    return h, w, n, xys.device
+
+
+def _check_mask(pixel_mask, h, w):
+    if pixel_mask is None:
+        return
+    _check_input(pixel_mask, "pixel_mask")
+    if pixel_mask.dtype not in (torch.bool, torch.uint8):
+        raise RuntimeError(f"pixel_mask must be torch.bool or torch.uint8, got {pixel_mask.dtype}")
+    if pixel_mask.numel() != h * w:
+        raise RuntimeError("pixel_mask must be [H, W]")
+
+
+def topk_balance_forward(img_height, img_width, xys, conics, pixel_topk, pixel_mask=None):
+    """How the pixels spread over the Gaussians: (loss (0-dim), counts [N] int32, importance [N], totals [2] int64). counts are the slots of
+    pixel_topk that hold each Gaussian, importance the sum of their gates exp(-sigma) / (sum + 1e-4), totals the filled slots A and the
+    pixels T with one, loss = N / (A T) * sum(counts * importance): 1 for an even spread, 0 without slots. pixel_mask [H, W] (bool or uint8)
+    leaves pixels out. The results do not depend on the order of the atomics."""
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, pixel_mask=pixel_mask)
+    _check_mask(pixel_mask, h, w)
+    loss = torch.empty((), device=dev, dtype=torch.float32)
+    counts = torch.empty(n, device=dev, dtype=torch.int32)
+    importance = torch.empty(n, device=dev, dtype=torch.float32)
+    totals = torch.empty(2, device=dev, dtype=torch.int64)
+    ws_bytes = _lib.load().igs_topk_balance_workspace(n)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        _lib_call("igs_topk_balance_fwd", h, w, n, ptr(xys), ptr(conics), ptr(pixel_topk), ptr(pixel_mask), ptr(loss), ptr(counts),
+                  ptr(importance), ptr(totals), ptr(ws), ws_bytes, stream_of(dev))
+    return loss, counts, importance, totals
+
+
+def topk_balance_backward(img_height, img_width, xys, conics, pixel_topk, counts, totals, grad_loss=None, grad_importance=None,
+                          pixel_mask=None):
+    """v_xy [N, 2], v_conic [N, 3] of grad_loss * loss + sum(grad_importance * importance), the counts held constant; counts, totals and
+    pixel_mask as topk_balance_forward returned and took them, grad_loss a device scalar, grad_importance [N]."""
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, counts=counts, totals=totals, grad_loss=grad_loss,
+                                grad_importance=grad_importance, pixel_mask=pixel_mask)
+    _check_mask(pixel_mask, h, w)
+    _check_input(counts, "counts", torch.int32)
+    _check_input(totals, "totals", torch.int64)
+    if counts.numel() != n or totals.numel() != 2:
+        raise RuntimeError("counts must be [N] and totals [2]")
+    if grad_loss is not None:
+        _check_input(grad_loss, "grad_loss", torch.float32)
+        if grad_loss.numel() != 1:
+            raise RuntimeError("grad_loss must hold one value")
+    if grad_importance is not None:
+        _check_input(grad_importance, "grad_importance", torch.float32)
+        if grad_importance.numel() != n:
+            raise RuntimeError("grad_importance must be [N]")
+    v_xy = torch.empty(n, 2, device=dev, dtype=torch.float32)
+    v_conic = torch.empty(n, 3, device=dev, dtype=torch.float32)
+    ws_bytes = _lib.load().igs_topk_balance_workspace(n)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        _lib_call("igs_topk_balance_bwd", h, w, n, ptr(xys), ptr(conics), ptr(pixel_topk), ptr(pixel_mask), ptr(counts), ptr(totals),
+                  ptr(grad_loss), ptr(grad_importance), 0, ptr(v_xy), ptr(v_conic), ptr(ws), ws_bytes, stream_of(dev))
+    return v_xy, v_conic
+
+
+def _check_dropout(h, w, n, colors, p, rng_state):
+    _check_input(colors, "colors", torch.float32)
+    if colors.ndim != 2 or colors.size(0) != n:
+        raise RuntimeError("colors must have dimensions (num_points, channels)")
+    channels = colors.size(1)
+    if not 1 <= channels <= MAX_CHANNELS:
+        raise RuntimeError(f"1 to {MAX_CHANNELS} channels, got {channels}")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must lie in [0, 1], got {p}")
+    _check_input(rng_state, "rng_state", torch.int64)
+    if rng_state.numel() != 2:
+        raise RuntimeError("rng_state must hold a seed and an offset")
+    return channels, p
+
+
+def topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk, p, rng_state):
+    """The render out_img [C, H, W] from the lists pixel_topk with every slot dropped with probability p before the weights are normalized
+    (a pixel with nothing left is 0), and rng_used [2], the seed and offset that the pass saw in rng_state (int64 [2] on the device): the
+    backward pass takes rng_used, and draws the same mask from it. Move the offset on between passes (rng_state[1] += 1, in a captured graph
+    too) for a new mask."""
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, colors=colors, rng_state=rng_state)
+    channels, p = _check_dropout(h, w, n, colors, p, rng_state)
+    out_img = torch.empty(channels, h, w, device=dev, dtype=torch.float32)
+    rng_used = torch.empty(2, device=dev, dtype=torch.int64)
+    ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        _lib_call("igs_topk_dropout_fwd", h, w, channels, n, ptr(xys), ptr(conics), ptr(colors), ptr(pixel_topk), p, ptr(rng_state),
+                  ptr(out_img), ptr(rng_used), ptr(ws), ws_bytes, stream_of(dev))
+    return out_img, rng_used
+
+
+def topk_dropout_backward(img_height, img_width, xys, conics, colors, v_output, pixel_topk, p, rng_used):
+    """v_xy [N, 2], v_conic [N, 3], v_colors [N, C] of topk_dropout_forward, for v_output [C, H, W] and the rng_used it returned."""
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, colors=colors, v_output=v_output, rng_used=rng_used)
+    channels, p = _check_dropout(h, w, n, colors, p, rng_used)
+    _check_input(v_output, "v_output", torch.float32)
+    if v_output.numel() != channels * h * w:
+        raise RuntimeError("v_output must be [C, H, W]")
+    grads = torch.empty(n * (5 + channels), device=dev, dtype=torch.float32)
+    v_xy, v_conic, v_colors = grads[:2 * n].view(n, 2), grads[2 * n:5 * n].view(n, 3), grads[5 * n:].view(n, channels)
+    ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        _lib_call("igs_topk_dropout_bwd", h, w, channels, n, ptr(xys), ptr(conics), ptr(colors), ptr(v_output), ptr(pixel_topk), p,
+                  ptr(rng_used), ptr(v_xy), ptr(v_conic), ptr(v_colors), ptr(ws), ws_bytes, stream_of(dev))
+    return v_xy, v_conic, v_colors
+
+
 # ---- losses, quantization, rate term -------------------------------------------------------------------------------------------------
 
 def l1_loss_and_grad(image: torch.Tensor, target: torch.Tensor, ratio: float = 1.0, workspace: Optional[torch.Tensor] = None):

@@ -271,6 +271,41 @@ int igs_loo_loss_increase(int img_height, int img_width, int channels, int num_p
 int igs_feature_weights(int img_height, int img_width, int num_points, const float *xys, const float *conics, const int32_t *pixel_topk,
                         double eps, int64_t *fixed_point, void *stream);
 
+/* How the pixels spread over the Gaussians, as the load of a router whose tokens are the pixels and whose experts are the Gaussians. Over
+ * the filled slots of pixel_topk [H,W,10] (IDs in [0, N), of pixels whose pixel_mask [H,W] byte is not zero; pixel_mask may be NULL):
+ * counts [N] = slots that hold the Gaussian, importance [N] = sum of their gates w_k / (sum_j w_j + 1e-4), w = exp(-sigma) (0 where sigma
+ * is negative, NaN or infinite), totals [2] (int64) = A, the filled slots, and T, the pixels with one, and
+ * loss = N / (A T) sum_g counts_g importance_g (0 when A is 0). All are written whole; none depends on the order of the atomics.
+ * igs_topk_balance_bwd: the gradient of v_loss * loss + sum_g v_importance_g importance_g with the counts held constant (v_loss a device
+ * scalar, v_importance [N]; either may be NULL, for 0), from the forward's counts and totals: v_xy [N,2], v_conic [N,3], written whole, or
+ * added to when accumulate is not zero. workspace: igs_topk_balance_workspace(N) bytes, 16-byte aligned, whose content need not survive
+ * between the two calls. At most 2^31 / 10 pixels. */
+size_t igs_topk_balance_workspace(int num_points);
+int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const float *xys, const float *conics, const int32_t *pixel_topk,
+                         const uint8_t *pixel_mask, float *loss, int32_t *counts, float *importance, int64_t *totals, void *workspace,
+                         size_t workspace_bytes, void *stream);
+int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const float *xys, const float *conics, const int32_t *pixel_topk,
+                         const uint8_t *pixel_mask, const int32_t *counts, const int64_t *totals, const float *v_loss,
+                         const float *v_importance, int accumulate, float *v_xy, float *v_conic, void *workspace, size_t workspace_bytes,
+                         void *stream);
+
+/* The render [C,H,W] from given top-K lists under gate dropout: each slot is dropped with probability p before the pixel's weights are
+ * normalized (out = sum_kept w_k f_k / (sum_kept w_k + 1e-4), 0 where none is kept), as if its Gaussian were not there. Empty slots and
+ * weights as in igs_topk_balance_fwd. The mask is never stored: rng_state [2] (int64, device) holds seed and offset, and slot k of pixel i
+ * (row-major) is dropped when its 24-bit draw is below rint(p 2^24): with the eight words of Philox4x32-10 at key (seed low, seed high) and
+ * counters (i, j, offset low, offset high), j = 0 and 1, slot k < 8 draws the upper 24 bits of word k, slots 8 and 9 the low bytes of words
+ * 0, 1, 2 and 3, 4, 5 (the first most significant). rng_used [2] gets the values that the pass saw; the backward pass takes them, so the
+ * caller may move rng_state on in between, in a captured graph too. igs_topk_dropout_bwd writes v_xy [N,2], v_conic [N,3] and v_colors
+ * [N,C] whole, from v_output [C,H,W]. 1 to 12 channels, at most 2^31 / 10 pixels. workspace: igs_topk_dropout_workspace(N, C) bytes,
+ * 16-byte aligned, whose content need not survive between the two calls. */
+size_t igs_topk_dropout_workspace(int num_points, int channels);
+int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
+                         const float *colors, const int32_t *pixel_topk, double p, const int64_t *rng_state, float *out_img,
+                         int64_t *rng_used, void *workspace, size_t workspace_bytes, void *stream);
+int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
+                         const float *colors, const float *v_output, const int32_t *pixel_topk, double p, const int64_t *rng_used,
+                         float *v_xy, float *v_conic, float *v_colors, void *workspace, size_t workspace_bytes, void *stream);
+
 /* nearest_neighbors / causal_neighbors of the rate model's preparation (compress/csrc/prediction.cpp:69-166, called by
  * compress/rate.py:56-66 bitstream_neighbors): for integer positions [P, 2] (int64, 16-byte aligned), the 8 nearest earlier Gaussians
  * (causal != 0: indices below the Gaussian's own, i.e. earlier in bitstream order) or the 8 nearest other Gaussians, ordered by squared
