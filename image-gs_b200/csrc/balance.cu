@@ -4,31 +4,36 @@
 //   loss = N / (A T) sum_g counts_g importance_g     (0 when A = 0; 1 when every Gaussian has the same share and the gates sum to one)
 // and, the counts held constant, with alpha_g = v_loss N counts_g / (A T) + v_importance_g:
 //   dL/dsigma_k = -n_k (alpha_k - sum_j n_j alpha_j),
-//   v_xy += dL/dsigma (a dx + b dy, b dx + c dy),  v_conic += dL/dsigma (dx^2 / 2, dx dy, dy^2 / 2).
+//   v_xy += dL/dsigma (a dx + b dy, b dx + c dy),  v_conic += dL/dsigma (dx^2 / 2, dx dy, dy^2 / 2)      (topk_sums.cuh).
 //
-// The importance is summed as 64-bit fixed point with as many fractional bits as the image leaves room for (a Gaussian's importance is at
-// most the pixel count), so the sums, and the loss, do not depend on the order of the atomics.
-#include "topk_lists.cuh"
+// The importance is summed over a patch in float, in one order, and from there as 64-bit fixed point with as many fractional bits as the
+// image leaves room for (a Gaussian's importance is at most the pixel count), so no result depends on the order of the atomics.
+#include "topk_sums.cuh"
 
 namespace {
 
+using igs::kRowsPerPass;
+using igs::kTile;
+using igs::kTilePixels;
 using igs::kTopK;
+using igs::kWeightPitch;
 
 constexpr int kThreads = 256;
+using SumsOf = igs::SumLayout<1, false>;
 
 struct BalanceWorkspace {
     unsigned long long filled;  // A
     unsigned long long routed;  // T
     unsigned int ticket;
-    unsigned int pad[11];
-    // then uint64 fixed [n] and double partials [blocks of the finish kernel]
+    float scale;                // backward: v_loss N / (A T)
+    unsigned int pad[10];
+    // forward: then uint64 fixed [n] and double partials [blocks of the finish kernel]; backward: then float sums [n, SumsOf::kValues]
 };
 
 int finish_blocks(int n) { return n > 0 ? igs::ceil_div(n, kThreads) : 1; }
-
-size_t fixed_offset() { return sizeof(BalanceWorkspace); }
-size_t partials_offset(int n) { return fixed_offset() + sizeof(unsigned long long) * (size_t)n; }
-size_t workspace_bytes_of(int n) { return partials_offset(n) + sizeof(double) * (size_t)finish_blocks(n) + sizeof(float) * (size_t)n; }
+size_t forward_bytes(int n) { return sizeof(BalanceWorkspace) + sizeof(unsigned long long) * (size_t)n + sizeof(double) * (size_t)finish_blocks(n); }
+size_t backward_bytes(int n) { return sizeof(BalanceWorkspace) + sizeof(float) * SumsOf::kValues * (size_t)n; }
+size_t workspace_bytes_of(int n) { return forward_bytes(n) > backward_bytes(n) ? forward_bytes(n) : backward_bytes(n); }
 
 // Fractional bits of the importance sums: pixels * 2^bits stays below 2^63
 int fraction_bits(int64_t pixels) {
@@ -37,55 +42,123 @@ int fraction_bits(int64_t pixels) {
     return 62 - log2;
 }
 
-struct Slots {
-    int id[kTopK];  // -1: empty
-    float dx[kTopK], dy[kTopK], gate[kTopK];
-};
-
-__device__ __forceinline__ void read_slots(Slots &s, const int p, const int img_w, const int n, const float2 *xys, const float *conics,
-                                           const int *pixel_topk) {
-    const float px = (float)(p % img_w), py = (float)(p / img_w);
-    const int2 *row = reinterpret_cast<const int2 *>(pixel_topk + (size_t)p * kTopK);
-    float sum = (float)igs::kNormEps;
-#pragma unroll
-    for (int k = 0; k < kTopK; k += 2) {
-        const int2 v = __ldg(&row[k / 2]);
-        s.id[k] = (unsigned)v.x < (unsigned)n ? v.x : -1, s.id[k + 1] = (unsigned)v.y < (unsigned)n ? v.y : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        s.gate[k] = 0.f;
-        if (s.id[k] < 0) continue;
-        const float2 xy = __ldg(&xys[s.id[k]]);
-        const float *c = conics + 3 * (size_t)s.id[k];
-        s.dx[k] = xy.x - px, s.dy[k] = xy.y - py;
-        s.gate[k] = igs::slot_weight(igs::gaussian_sigma(xy.x, xy.y, __ldg(&c[0]), __ldg(&c[1]), __ldg(&c[2]), px, py));
-        sum += s.gate[k];
-    }
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) s.gate[k] *= inv;
+__global__ void __launch_bounds__(kThreads) balance_zero_kernel(const int n, int *__restrict__ counts, unsigned long long *__restrict__ fixed,
+                                                                BalanceWorkspace *__restrict__ ws) {
+    igs::wait_for_predecessor();
+    const int g = blockIdx.x * kThreads + threadIdx.x;
+    if (g == 0) ws->filled = 0, ws->routed = 0, ws->ticket = 0;
+    if (g < n) counts[g] = 0, fixed[g] = 0;
 }
 
-__global__ void __launch_bounds__(kThreads) balance_kernel(const int pixels, const int img_w, const int n, const float2 *__restrict__ xys,
-                                                           const float *__restrict__ conics, const int *__restrict__ pixel_topk,
-                                                           const uint8_t *__restrict__ mask, const float scale, int *__restrict__ counts,
-                                                           unsigned long long *__restrict__ fixed, BalanceWorkspace *__restrict__ ws) {
-    const int p = blockIdx.x * kThreads + threadIdx.x;
-    bool routed = false;
-    if (p < pixels && (mask == nullptr || mask[p] != 0)) {
-        Slots s;
-        read_slots(s, p, img_w, n, xys, conics, pixel_topk);
-#pragma unroll
+struct BalanceSmem {
+    igs::TileTable table;
+    union {
+        alignas(16) int lists[igs::kListWords];
+        struct {
+            alignas(16) float weight[8][kRowsPerPass * kWeightPitch];
+            alignas(16) float inv[8][32];
+        };
+    };
+    float4 rows[igs::kMaxRows];
+    float rows_c[igs::kMaxRows];
+};
+
+// One pixel's slots one by one, from global memory (topk_sums.cuh says when)
+__device__ __noinline__ void count_slots(const int p, const int img_w, const int n, const float *xys, const float *conics,
+                                         const int *pixel_topk, const float scale, int *counts, unsigned long long *fixed) {
+    const float px = (float)(p % img_w), py = (float)(p / img_w);
+    const int *list = pixel_topk + (size_t)p * kTopK;
+    float total = (float)igs::kNormEps;
+    for (int pass = 0; pass < 2; ++pass) {
+        const float inv = 1.f / total;
         for (int k = 0; k < kTopK; ++k) {
-            if (s.id[k] < 0) continue;
-            routed = true;
-            atomicAdd(&counts[s.id[k]], 1);
-            atomicAdd(&fixed[s.id[k]], (unsigned long long)__float2ll_rn(s.gate[k] * scale));
+            const int id = list[k];
+            if ((unsigned)id >= (unsigned)n) continue;
+            const igs::RowGeometry g = igs::stage_geometry(xys, conics, id);
+            const float e = igs::row_exponent(make_float4(g.x, g.y, g.a, g.b), g.c, px, py);
+            const float w = e <= 0.f ? igs::exp2_approx(e) : 0.f;
+            if (pass == 0) {
+                total += w;
+            } else {
+                atomicAdd(&counts[id], 1);
+                atomicAdd(&fixed[id], (unsigned long long)__float2ll_rn(w * inv * scale));
+            }
         }
     }
-    const int in_block = __syncthreads_count(routed);
-    if (threadIdx.x == 0 && in_block) atomicAdd(&ws->routed, (unsigned long long)in_block);
+}
+
+__global__ void __launch_bounds__(kTilePixels, 5) balance_kernel(const int tiles_x, const int img_h, const int img_w, const int n,
+                                                              const float *__restrict__ xys, const float *__restrict__ conics,
+                                                              const int *__restrict__ pixel_topk, const uint8_t *__restrict__ mask,
+                                                              const float scale, int *__restrict__ counts,
+                                                              unsigned long long *__restrict__ fixed, BalanceWorkspace *__restrict__ ws) {
+    __shared__ __align__(16) BalanceSmem sm;
+    igs::wait_for_predecessor();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int i0 = (blockIdx.x / tiles_x) * kTile, j0 = (blockIdx.x % tiles_x) * kTile;
+    const int i = i0 + igs::patch_y(), j = j0 + igs::patch_x();
+    const bool inside = i < img_h && j < img_w;
+    const int p = inside ? i * img_w + j : 0;
+    igs::load_lists(sm.lists, sm.table, pixel_topk, i0, j0, img_h, img_w);
+    const unsigned keep = inside && (mask == nullptr || mask[p] != 0) ? ~0u : 0u;
+    igs::finish_lists();
+    igs::PixelSlots s;
+    igs::place_slots(s, sm.table, sm.lists, n, keep);
+    const int routed = __syncthreads_count(s.filled > 0);
+    if (threadIdx.x == 0 && routed > 0) atomicAdd(&ws->routed, (unsigned long long)routed);
+    const int count = sm.table.count;
+    if (count > igs::kMaxRows) {
+        if (keep) count_slots(p, img_w, n, xys, conics, pixel_topk, scale, counts, fixed);
+        return;
+    }
+    igs::rank_rows(sm.table, count, [&](const int row, const int id) {
+        const igs::RowGeometry g = igs::stage_geometry(xys, conics, id);
+        sm.rows[row] = make_float4(g.x, g.y, g.a, g.b), sm.rows_c[row] = g.c;
+    });
+    __syncthreads();
+    if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count))) {
+        if (keep) count_slots(p, img_w, n, xys, conics, pixel_topk, scale, counts, fixed);
+        return;
+    }
+    // a lane is a pixel: the first rows' weights and the sum over all; a lane is half a row: its gates' sum (topk_sums.cuh)
+    const float px = (float)j, py = (float)i;
+    float *const weight = sm.weight[warp];
+    const int half = lane >> 4, r = lane & (kRowsPerPass - 1);
+    float total = (float)igs::kNormEps;
+    int visited = 0, my_row = 0, my_count = 0;
+    auto visit = [&](const int slot, const int row, const bool held) {
+        const float e = igs::row_exponent(sm.rows[row], sm.rows_c[row], px, py);
+        const float w = held && e <= 0.f ? igs::exp2_approx(e) : 0.f;
+        if (slot >= 0 && slot < kRowsPerPass) {
+            weight[slot * kWeightPitch + lane] = w;
+            const int holders = __popc(__ballot_sync(0xffffffffu, held));
+            if (r == slot) my_row = row, my_count = holders;
+        }
+        return w;
+    };
+    igs::visit_rows(s, count, [&](const int row, const bool held) { total += visit(visited++, row, held); });
+    sm.inv[warp][lane] = 1.f / total;
+    for (int first = 0; first < visited; first += kRowsPerPass) {
+        if (first > 0) {
+            __syncwarp();
+            int at = 0;
+            igs::visit_rows(s, count, [&](const int row, const bool held) { visit(at++ - first, row, held); });
+        }
+        __syncwarp();
+        float sum = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 w = *reinterpret_cast<const float4 *>(&weight[r * kWeightPitch + half * 16 + q * 4]);
+            const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[warp][half * 16 + q * 4]);
+            sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (r < visited - first) {
+            const int id = sm.table.sorted[my_row];
+            if (half == 0) atomicAdd(&counts[id], my_count);
+            else atomicAdd(&fixed[id], (unsigned long long)__float2ll_rn(sum * scale));
+        }
+    }
 }
 
 // importance from the fixed-point sums, and the loss: each block's sums of counts and of counts * importance (in double, in thread order),
@@ -95,6 +168,7 @@ __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const int n, c
                                                                   float *__restrict__ importance, double *__restrict__ partials,
                                                                   BalanceWorkspace *__restrict__ ws, float *__restrict__ loss,
                                                                   long long *__restrict__ totals) {
+    igs::wait_for_predecessor();
     __shared__ double s_sum[kThreads / 32];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -137,48 +211,15 @@ __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const int n, c
     }
 }
 
-// alpha [n], and the gradients zeroed unless they are added to
-__global__ void __launch_bounds__(kThreads) balance_alpha_kernel(const int n, const int *__restrict__ counts,
-                                                                 const long long *__restrict__ totals, const float *__restrict__ v_loss,
-                                                                 const float *__restrict__ v_importance, const bool zero,
-                                                                 float *__restrict__ alpha, float *__restrict__ v_xy,
-                                                                 float *__restrict__ v_conic) {
-    const int g = blockIdx.x * kThreads + threadIdx.x;
-    if (g >= n) return;
-    const double a = (double)totals[0], t = (double)totals[1];
-    const float scale = v_loss != nullptr && totals[0] > 0 ? (float)((double)n / (a * t)) * *v_loss : 0.f;
-    alpha[g] = scale * (float)counts[g] + (v_importance != nullptr ? v_importance[g] : 0.f);
-    if (zero) {
-        v_xy[2 * (size_t)g] = 0.f, v_xy[2 * (size_t)g + 1] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) v_conic[3 * (size_t)g + j] = 0.f;
-    }
-}
-
-__global__ void __launch_bounds__(kThreads) balance_bwd_kernel(const int pixels, const int img_w, const int n, const float2 *__restrict__ xys,
-                                                               const float *__restrict__ conics, const int *__restrict__ pixel_topk,
-                                                               const uint8_t *__restrict__ mask, const float *__restrict__ alpha,
-                                                               float *__restrict__ v_xy, float *__restrict__ v_conic) {
-    const int p = blockIdx.x * kThreads + threadIdx.x;
-    if (p >= pixels || (mask != nullptr && mask[p] == 0)) return;
-    Slots s;
-    read_slots(s, p, img_w, n, xys, conics, pixel_topk);
-    float mean = 0.f;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k)
-        if (s.id[k] >= 0) mean += s.gate[k] * __ldg(&alpha[s.id[k]]);
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        const int g = s.id[k];
-        if (s.gate[k] == 0.f) continue;  // empty, or a Gaussian whose parameters may not even be finite
-        const float t = s.gate[k] * (mean - __ldg(&alpha[g]));
-        const float *c = conics + 3 * (size_t)g;
-        atomicAdd(&v_xy[2 * (size_t)g], t * (c[0] * s.dx[k] + c[1] * s.dy[k]));
-        atomicAdd(&v_xy[2 * (size_t)g + 1], t * (c[1] * s.dx[k] + c[2] * s.dy[k]));
-        atomicAdd(&v_conic[3 * (size_t)g], 0.5f * t * s.dx[k] * s.dx[k]);
-        atomicAdd(&v_conic[3 * (size_t)g + 1], t * s.dx[k] * s.dy[k]);
-        atomicAdd(&v_conic[3 * (size_t)g + 2], 0.5f * t * s.dy[k] * s.dy[k]);
-    }
+// The backward pass's sums zeroed, and the loss's share of alpha: v_loss N / (A T)
+__global__ void __launch_bounds__(kThreads) balance_scale_kernel(const int n, const long long *__restrict__ totals,
+                                                                 const float *__restrict__ v_loss, float4 *__restrict__ sums,
+                                                                 BalanceWorkspace *__restrict__ ws) {
+    igs::wait_for_predecessor();
+    const int e = blockIdx.x * kThreads + threadIdx.x;
+    if (e == 0)
+        ws->scale = v_loss != nullptr && totals[0] > 0 ? (float)((double)n / ((double)totals[0] * (double)totals[1])) * *v_loss : 0.f;
+    if (e < n * (SumsOf::kValues / 4)) sums[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 }  // namespace
@@ -191,27 +232,29 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
                          const uint8_t *pixel_mask, float *loss, int32_t *counts, float *importance, int64_t *totals, void *workspace,
                          size_t workspace_bytes, void *stream) {
     IGS_REQUIRE(img_height >= 0 && img_width >= 0 && num_points >= 0, "igs_topk_balance_fwd: negative size");
-    IGS_REQUIRE(igs::lists_addressable(img_height, img_width), "igs_topk_balance_fwd: at most 2^31 / 10 pixels and 2^24 a side");
+    IGS_REQUIRE(igs::lists_addressable(img_height, img_width, num_points), "igs_topk_balance_fwd: %s", igs::kListsLimit);
     IGS_REQUIRE(loss && totals && (num_points == 0 || (counts && importance)), "igs_topk_balance_fwd: null output");
     IGS_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(num_points), "igs_topk_balance_fwd: workspace too small");
     IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_balance_fwd: workspace must be 16-byte aligned");
     const int pixels = img_height * img_width;
     IGS_REQUIRE(pixels == 0 || num_points == 0 || (xys && conics && pixel_topk), "igs_topk_balance_fwd: null pointer");
-    IGS_REQUIRE(igs::aligned(xys, 8) && igs::aligned(pixel_topk, 8), "igs_topk_balance_fwd: xys and pixel_topk must be 8-byte aligned");
+    IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_balance_fwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
     char *base = static_cast<char *>(workspace);
     BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(base);
-    unsigned long long *fixed = reinterpret_cast<unsigned long long *>(base + fixed_offset());
-    double *partials = reinterpret_cast<double *>(base + partials_offset(num_points));
-    cudaMemsetAsync(workspace, 0, partials_offset(num_points), s);
-    if (num_points > 0) cudaMemsetAsync(counts, 0, sizeof(int32_t) * (size_t)num_points, s);
+    unsigned long long *fixed = reinterpret_cast<unsigned long long *>(base + sizeof(BalanceWorkspace));
+    double *partials = reinterpret_cast<double *>(fixed + num_points);
     const int bits = fraction_bits(pixels);
-    if (pixels > 0 && num_points > 0)
-        balance_kernel<<<igs::ceil_div(pixels, kThreads), kThreads, 0, s>>>(pixels, img_width, num_points,
-                                                                            reinterpret_cast<const float2 *>(xys), conics, pixel_topk,
-                                                                            pixel_mask, (float)((int64_t)1 << bits), counts, fixed, ws);
-    balance_finish_kernel<<<finish_blocks(num_points), kThreads, 0, s>>>(
-        num_points, counts, fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss, reinterpret_cast<long long *>(totals));
+    const int blocks = finish_blocks(num_points);
+    igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, counts, fixed, ws);
+    if (pixels > 0 && num_points > 0) {
+        const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
+        igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, tiles_x, img_height, img_width, num_points, xys, conics,
+                    pixel_topk, pixel_mask, (float)((int64_t)1 << bits), counts, fixed, ws);
+    }
+    igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
+                (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,
+                reinterpret_cast<long long *>(totals));
     return igs::check_launch("igs_topk_balance_fwd");
 }
 
@@ -220,23 +263,29 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
                          const float *v_importance, int accumulate, float *v_xy, float *v_conic, void *workspace, size_t workspace_bytes,
                          void *stream) {
     IGS_REQUIRE(img_height >= 0 && img_width >= 0 && num_points >= 0, "igs_topk_balance_bwd: negative size");
-    IGS_REQUIRE(igs::lists_addressable(img_height, img_width), "igs_topk_balance_bwd: at most 2^31 / 10 pixels and 2^24 a side");
+    IGS_REQUIRE(igs::lists_addressable(img_height, img_width, num_points), "igs_topk_balance_bwd: %s", igs::kListsLimit);
     if (num_points == 0) return IGS_OK;
     IGS_REQUIRE(xys && conics && counts && totals && v_xy && v_conic, "igs_topk_balance_bwd: null pointer");
     IGS_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(num_points), "igs_topk_balance_bwd: workspace too small");
     IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_balance_bwd: workspace must be 16-byte aligned");
     const int pixels = img_height * img_width;
     IGS_REQUIRE(pixels == 0 || pixel_topk, "igs_topk_balance_bwd: null pointer");
-    IGS_REQUIRE(igs::aligned(xys, 8) && igs::aligned(pixel_topk, 8), "igs_topk_balance_bwd: xys and pixel_topk must be 8-byte aligned");
+    IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_balance_bwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
-    float *alpha = reinterpret_cast<float *>(static_cast<char *>(workspace) + partials_offset(num_points) +
-                                             sizeof(double) * (size_t)finish_blocks(num_points));
-    balance_alpha_kernel<<<igs::ceil_div(num_points, kThreads), kThreads, 0, s>>>(
-        num_points, counts, reinterpret_cast<const long long *>(totals), v_loss, v_importance, accumulate == 0, alpha, v_xy, v_conic);
-    if (pixels > 0)
-        balance_bwd_kernel<<<igs::ceil_div(pixels, kThreads), kThreads, 0, s>>>(pixels, img_width, num_points,
-                                                                                reinterpret_cast<const float2 *>(xys), conics, pixel_topk,
-                                                                                pixel_mask, alpha, v_xy, v_conic);
+    BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(workspace);
+    float *sums = reinterpret_cast<float *>(ws + 1);
+    igs::launch(balance_scale_kernel, dim3(igs::ceil_div(num_points * (SumsOf::kValues / 4), kThreads)), dim3(kThreads), 0, s, num_points,
+                reinterpret_cast<const long long *>(totals), v_loss, reinterpret_cast<float4 *>(sums), ws);
+    if (pixels > 0) {
+        igs::SumArgs a = {};
+        a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.n = num_points;
+        a.xys = xys, a.conics = conics, a.pixel_topk = pixel_topk, a.mask = pixel_mask;
+        a.counts = counts, a.scale = &ws->scale, a.v_importance = v_importance, a.sums = sums;
+        igs::launch(igs::sums_kernel<1, false>, dim3(a.tiles_x * igs::ceil_div(img_height, kTile)), dim3(kTilePixels),
+                    sizeof(igs::SumSmem<1, false>), s, a);
+    }
+    igs::launch(igs::finish_sums_kernel<SumsOf::kValues>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, num_points, 0, conics,
+                (const float *)sums, accumulate != 0, v_xy, v_conic, (float *)nullptr);
     return igs::check_launch("igs_topk_balance_bwd");
 }
 

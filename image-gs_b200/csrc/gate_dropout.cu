@@ -2,125 +2,163 @@
 // sums as if its Gaussian were not there, which is what the leave-one-out pruning score evaluates (loo.cu):
 //   out_c = sum_kept w_k f_kc / (sum_kept w_k + eps)          (0 where no slot is kept)
 // and with gates n_k = w_k / (sum_kept w_j + eps), s_k = f_k . v_out:
-//   v_f += n_k v_out,  dL/dsigma_k = -n_k (s_k - sum_j n_j s_j),  and the geometry's gradients from dL/dsigma as in balance.cu.
+//   v_f += n_k v_out,  dL/dsigma_k = -n_k (s_k - sum_j n_j s_j),  and the geometry's gradients from dL/dsigma (topk_sums.cuh).
 // The mask is drawn from the pixel's index and two 64-bit values on the device, seed and offset (keep_bits in topk_lists.cuh), in the
 // forward pass and again in the backward pass, so it is never stored, and a captured graph draws a new one whenever the offset has moved.
-#include "topk_lists.cuh"
+#include "topk_sums.cuh"
 
 namespace {
 
 using igs::kMaxChannels;
+using igs::kTile;
+using igs::kTilePixels;
 using igs::kTopK;
 
-constexpr int kThreads = 256;
-
-size_t workspace_bytes_of(int num_points, int channels) { return 16; }
-
-struct Slots {
-    int id[kTopK];  // -1: empty or dropped
-    float dx[kTopK], dy[kTopK], gate[kTopK];
+template <int C>
+struct DropoutSmem {
+    igs::TileTable table;
+    alignas(16) int lists[igs::kListWords];
+    float4 rows[igs::kMaxRows * igs::SumLayout<C, true>::kRowQuads];
 };
 
-__device__ __forceinline__ void read_slots(Slots &s, const int p, const int img_w, const int n, const float2 *xys, const float *conics,
-                                           const int *pixel_topk, const unsigned keep) {
-    const float px = (float)(p % img_w), py = (float)(p / img_w);
-    const int2 *row = reinterpret_cast<const int2 *>(pixel_topk + (size_t)p * kTopK);
-    float sum = (float)igs::kNormEps;
-#pragma unroll
-    for (int k = 0; k < kTopK; k += 2) {
-        const int2 v = __ldg(&row[k / 2]);
-        s.id[k] = (unsigned)v.x < (unsigned)n && (keep >> k & 1) ? v.x : -1;
-        s.id[k + 1] = (unsigned)v.y < (unsigned)n && (keep >> (k + 1) & 1) ? v.y : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        s.gate[k] = 0.f;
-        if (s.id[k] < 0) continue;
-        const float2 xy = __ldg(&xys[s.id[k]]);
-        const float *c = conics + 3 * (size_t)s.id[k];
-        s.dx[k] = xy.x - px, s.dy[k] = xy.y - py;
-        s.gate[k] = igs::slot_weight(igs::gaussian_sigma(xy.x, xy.y, __ldg(&c[0]), __ldg(&c[1]), __ldg(&c[2]), px, py));
-        sum += s.gate[k];
-    }
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) s.gate[k] *= inv;
-}
+struct DropoutArgs {
+    int tiles_x, img_h, img_w, channels, n;
+    const float *xys, *conics, *colors;
+    const int *pixel_topk;
+    uint32_t threshold;
+    const long long *rng;
+    float *out_img;
+    long long *rng_used;
+};
 
-__global__ void __launch_bounds__(kThreads) dropout_fwd_kernel(const int pixels, const int img_w, const int channels, const int n,
-                                                               const float2 *__restrict__ xys, const float *__restrict__ conics,
-                                                               const float *__restrict__ colors, const int *__restrict__ pixel_topk,
-                                                               const uint32_t threshold, const long long *__restrict__ rng,
-                                                               float *__restrict__ out_img, long long *__restrict__ rng_used) {
-    const int p = blockIdx.x * kThreads + threadIdx.x;
-    const long long seed = rng[0], offset = rng[1];
-    if (p == 0) rng_used[0] = seed, rng_used[1] = offset;
-    if (p >= pixels) return;
-    Slots s;
-    read_slots(s, p, img_w, n, xys, conics, pixel_topk, igs::keep_bits(p, seed, offset, threshold));
-    float pix[kMaxChannels];
-#pragma unroll
-    for (int c = 0; c < kMaxChannels; ++c) pix[c] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        if (s.id[k] < 0) continue;
-#pragma unroll
-        for (int c = 0; c < kMaxChannels; ++c)
-            if (c < channels) pix[c] += s.gate[k] * __ldg(&colors[(size_t)s.id[k] * channels + c]);
-    }
-#pragma unroll
-    for (int c = 0; c < kMaxChannels; ++c)
-        if (c < channels) out_img[(size_t)c * pixels + p] = pix[c];
-}
-
-__global__ void __launch_bounds__(kThreads) dropout_bwd_kernel(const int pixels, const int img_w, const int channels, const int n,
-                                                               const float2 *__restrict__ xys, const float *__restrict__ conics,
-                                                               const float *__restrict__ colors, const float *__restrict__ v_output,
-                                                               const int *__restrict__ pixel_topk, const uint32_t threshold,
-                                                               const long long *__restrict__ rng, float *__restrict__ v_xy,
-                                                               float *__restrict__ v_conic, float *__restrict__ v_colors) {
-    const int p = blockIdx.x * kThreads + threadIdx.x;
-    if (p >= pixels) return;
-    Slots s;
-    read_slots(s, p, img_w, n, xys, conics, pixel_topk, igs::keep_bits(p, rng[0], rng[1], threshold));
-    float score[kTopK], mean = 0.f;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        score[k] = 0.f;
-        if (s.id[k] < 0) continue;
-        for (int c = 0; c < channels; ++c) {
-            const float v = __ldg(&v_output[(size_t)c * pixels + p]);
-            score[k] += __ldg(&colors[(size_t)s.id[k] * channels + c]) * v;
-            atomicAdd(&v_colors[(size_t)s.id[k] * channels + c], s.gate[k] * v);
+// One pixel's slots one by one, from global memory
+__device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p, const unsigned keep) {
+    const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
+    const int *list = a.pixel_topk + (size_t)p * kTopK;
+    float *out = a.out_img + p;
+    const size_t plane = (size_t)a.img_h * a.img_w;
+    for (int c = 0; c < a.channels; ++c) {
+        float total = (float)igs::kNormEps, pix = 0.f;
+        for (int k = 0; k < kTopK; ++k) {
+            const int id = list[k];
+            if ((unsigned)id >= (unsigned)a.n || !(keep >> k & 1)) continue;
+            const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
+            const float e = igs::row_exponent(make_float4(g.x, g.y, g.a, g.b), g.c, px, py);
+            if (!(e <= 0.f)) continue;
+            const float w = igs::exp2_approx(e);
+            total += w;
+            pix = fmaf(w, __ldg(&a.colors[(size_t)id * a.channels + c]), pix);
         }
-        mean += s.gate[k] * score[k];
+        out[c * plane] = pix / total;
     }
+}
+
+template <int C>
+__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 6 : 4)
+    dropout_kernel(const __grid_constant__ DropoutArgs a) {
+    constexpr int kQuads = igs::SumLayout<C, true>::kRowQuads;
+    __shared__ __align__(16) DropoutSmem<C> sm;
+    igs::wait_for_predecessor();
+    const int i0 = (blockIdx.x / a.tiles_x) * kTile, j0 = (blockIdx.x % a.tiles_x) * kTile;
+    const int i = i0 + igs::patch_y(), j = j0 + igs::patch_x();
+    const bool inside = i < a.img_h && j < a.img_w;
+    const int p = inside ? i * a.img_w + j : 0;
+    igs::load_lists(sm.lists, sm.table, a.pixel_topk, i0, j0, a.img_h, a.img_w);
+    const long long seed = a.rng[0], offset = a.rng[1];
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
+    const unsigned keep = inside ? igs::keep_bits((uint32_t)p, (uint64_t)seed, (uint64_t)offset, a.threshold) : 0u;
+    igs::finish_lists();
+    igs::PixelSlots s;
+    igs::place_slots(s, sm.table, sm.lists, a.n, keep);
+    __syncthreads();
+    const int count = sm.table.count;
+    if (count > igs::kMaxRows) {
+        if (inside) blend_slots(a, p, keep);
+        return;
+    }
+    igs::rank_rows(sm.table, count, [&](const int row, const int id) {
+        const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
+        float q[4 * kQuads];
+        q[0] = g.x, q[1] = g.y, q[2] = g.a, q[3] = g.b, q[4] = g.c;
 #pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        const int g = s.id[k];
-        if (s.gate[k] == 0.f) continue;  // empty, or a Gaussian whose parameters may not even be finite
-        const float t = s.gate[k] * (mean - score[k]);
-        const float *c = conics + 3 * (size_t)g;
-        atomicAdd(&v_xy[2 * (size_t)g], t * (c[0] * s.dx[k] + c[1] * s.dy[k]));
-        atomicAdd(&v_xy[2 * (size_t)g + 1], t * (c[1] * s.dx[k] + c[2] * s.dy[k]));
-        atomicAdd(&v_conic[3 * (size_t)g], 0.5f * t * s.dx[k] * s.dx[k]);
-        atomicAdd(&v_conic[3 * (size_t)g + 1], t * s.dx[k] * s.dy[k]);
-        atomicAdd(&v_conic[3 * (size_t)g + 2], 0.5f * t * s.dy[k] * s.dy[k]);
+        for (int c = 0; c < 4 * kQuads - 5; ++c) q[5 + c] = c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
+#pragma unroll
+        for (int e = 0; e < kQuads; ++e) sm.rows[row * kQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
+    });
+    __syncthreads();
+    if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count))) {
+        if (inside) blend_slots(a, p, keep);
+        return;
     }
+    const float px = (float)j, py = (float)i;
+    float total = (float)igs::kNormEps;
+    float pix[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) pix[c] = 0.f;
+    igs::visit_rows(s, count, [&](const int row, const bool held) {
+        float q[4 * kQuads];
+#pragma unroll
+        for (int e = 0; e < kQuads; ++e) {
+            const float4 v = sm.rows[row * kQuads + e];
+            q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
+        }
+        const float e = igs::row_exponent(make_float4(q[0], q[1], q[2], q[3]), q[4], px, py);
+        if (held && e <= 0.f) {
+            const float w = igs::exp2_approx(e);
+            total += w;
+#pragma unroll
+            for (int c = 0; c < C; ++c) pix[c] = fmaf(w, q[5 + c], pix[c]);
+        }
+    });
+    if (!inside) return;
+    const float inv = 1.f / total;
+    const size_t plane = (size_t)a.img_h * a.img_w;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        if (c < a.channels) a.out_img[c * plane + p] = pix[c] * inv;
+}
+
+__global__ void rng_used_kernel(const long long *rng, long long *rng_used) {
+    igs::wait_for_predecessor();
+    rng_used[0] = rng[0], rng_used[1] = rng[1];
+}
+
+__global__ void __launch_bounds__(256) zero_kernel(const int64_t quads, float4 *__restrict__ sums) {
+    igs::wait_for_predecessor();
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e < quads) sums[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// The kernels' widths: channels are padded with zeros to one less than a multiple of four, so that a staged row (geometry 5, colours) and a
+// Gaussian's sums (5, colours) are whole 16-byte words. 12 stands for itself (12 + 5 = 17 of 20).
+template <typename F>
+void with_width(int channels, F f) {
+    if (channels <= 3) f(std::integral_constant<int, 3>());
+    else if (channels <= 7) f(std::integral_constant<int, 7>());
+    else if (channels <= 11) f(std::integral_constant<int, 11>());
+    else f(std::integral_constant<int, 12>());
+}
+
+size_t workspace_bytes_of(int num_points, int channels) {
+    size_t values = 0;
+    with_width(channels, [&](auto width) { values = igs::SumLayout<decltype(width)::value, true>::kValues; });
+    return sizeof(float) * values * (size_t)num_points + 16;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t igs_topk_dropout_workspace(int num_points, int channels) { return num_points < 0 || channels < 0 ? 0 : workspace_bytes_of(num_points, channels); }
+size_t igs_topk_dropout_workspace(int num_points, int channels) {
+    return num_points < 0 || channels < 0 ? 0 : workspace_bytes_of(num_points, channels);
+}
 
 int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
                          const float *colors, const int32_t *pixel_topk, double p, const int64_t *rng_state, float *out_img,
                          int64_t *rng_used, void *workspace, size_t workspace_bytes, void *stream) {
     IGS_REQUIRE(img_height >= 0 && img_width >= 0 && num_points >= 0, "igs_topk_dropout_fwd: negative size");
     IGS_REQUIRE(channels >= 1 && channels <= kMaxChannels, "igs_topk_dropout_fwd: 1 to %d channels", kMaxChannels);
-    IGS_REQUIRE(igs::lists_addressable(img_height, img_width), "igs_topk_dropout_fwd: at most 2^31 / 10 pixels and 2^24 a side");
+    IGS_REQUIRE(igs::lists_addressable(img_height, img_width, num_points), "igs_topk_dropout_fwd: %s", igs::kListsLimit);
     IGS_REQUIRE(p >= 0.0 && p <= 1.0, "igs_topk_dropout_fwd: p must lie in [0, 1]");
     IGS_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(num_points, channels), "igs_topk_dropout_fwd: workspace too small");
     IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_dropout_fwd: workspace must be 16-byte aligned");
@@ -128,11 +166,20 @@ int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_po
     const int pixels = img_height * img_width;
     IGS_REQUIRE(pixels == 0 || (pixel_topk && out_img && (num_points == 0 || (xys && conics && colors))),
                 "igs_topk_dropout_fwd: null pointer");
-    IGS_REQUIRE(igs::aligned(xys, 8) && igs::aligned(pixel_topk, 8), "igs_topk_dropout_fwd: xys and pixel_topk must be 8-byte aligned");
-    const int blocks = pixels > 0 ? igs::ceil_div(pixels, kThreads) : 1;
-    dropout_fwd_kernel<<<blocks, kThreads, 0, igs::as_stream(stream)>>>(
-        pixels, img_width, channels, num_points, reinterpret_cast<const float2 *>(xys), conics, colors, pixel_topk,
-        (uint32_t)rint(p * 16777216.0), reinterpret_cast<const long long *>(rng_state), out_img, reinterpret_cast<long long *>(rng_used));
+    IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_dropout_fwd: pixel_topk must be 8-byte aligned");
+    cudaStream_t s = igs::as_stream(stream);
+    const long long *rng = reinterpret_cast<const long long *>(rng_state);
+    long long *used = reinterpret_cast<long long *>(rng_used);
+    if (pixels == 0) {
+        igs::launch(rng_used_kernel, dim3(1), dim3(1), 0, s, rng, used);
+    } else {
+        const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
+        const DropoutArgs a = {tiles_x, img_height, img_width, channels, num_points, xys, conics, colors, pixel_topk,
+                               (uint32_t)rint(p * 16777216.0), rng, out_img, used};
+        with_width(channels, [&](auto width) {
+            igs::launch(dropout_kernel<decltype(width)::value>, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
+        });
+    }
     return igs::check_launch("igs_topk_dropout_fwd");
 }
 
@@ -141,23 +188,33 @@ int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_po
                          float *v_xy, float *v_conic, float *v_colors, void *workspace, size_t workspace_bytes, void *stream) {
     IGS_REQUIRE(img_height >= 0 && img_width >= 0 && num_points >= 0, "igs_topk_dropout_bwd: negative size");
     IGS_REQUIRE(channels >= 1 && channels <= kMaxChannels, "igs_topk_dropout_bwd: 1 to %d channels", kMaxChannels);
-    IGS_REQUIRE(igs::lists_addressable(img_height, img_width), "igs_topk_dropout_bwd: at most 2^31 / 10 pixels and 2^24 a side");
+    IGS_REQUIRE(igs::lists_addressable(img_height, img_width, num_points), "igs_topk_dropout_bwd: %s", igs::kListsLimit);
     IGS_REQUIRE(p >= 0.0 && p <= 1.0, "igs_topk_dropout_bwd: p must lie in [0, 1]");
     if (num_points == 0) return IGS_OK;
     IGS_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(num_points, channels), "igs_topk_dropout_bwd: workspace too small");
     IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_dropout_bwd: workspace must be 16-byte aligned");
     IGS_REQUIRE(v_xy && v_conic && v_colors, "igs_topk_dropout_bwd: null output");
     const int pixels = img_height * img_width;
-    IGS_REQUIRE(pixels == 0 || (xys && conics && colors && v_output && pixel_topk && rng_used), "igs_topk_dropout_bwd: null pointer");
-    IGS_REQUIRE(igs::aligned(xys, 8) && igs::aligned(pixel_topk, 8), "igs_topk_dropout_bwd: xys and pixel_topk must be 8-byte aligned");
+    IGS_REQUIRE(conics && (pixels == 0 || (xys && colors && v_output && pixel_topk && rng_used)), "igs_topk_dropout_bwd: null pointer");
+    IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_dropout_bwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
-    cudaMemsetAsync(v_xy, 0, sizeof(float) * 2 * (size_t)num_points, s);
-    cudaMemsetAsync(v_conic, 0, sizeof(float) * 3 * (size_t)num_points, s);
-    cudaMemsetAsync(v_colors, 0, sizeof(float) * channels * (size_t)num_points, s);
-    if (pixels > 0)
-        dropout_bwd_kernel<<<igs::ceil_div(pixels, kThreads), kThreads, 0, s>>>(
-            pixels, img_width, channels, num_points, reinterpret_cast<const float2 *>(xys), conics, colors, v_output, pixel_topk,
-            (uint32_t)rint(p * 16777216.0), reinterpret_cast<const long long *>(rng_used), v_xy, v_conic, v_colors);
+    float *sums = static_cast<float *>(workspace);
+    with_width(channels, [&](auto width) {
+        constexpr int kWidth = decltype(width)::value;
+        constexpr int kValues = igs::SumLayout<kWidth, true>::kValues;
+        const int64_t quads = (int64_t)num_points * (kValues / 4);
+        igs::launch(zero_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, quads, reinterpret_cast<float4 *>(sums));
+        if (pixels > 0) {
+            igs::SumArgs a = {};
+            a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
+            a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
+            a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0), a.sums = sums;
+            igs::launch(igs::sums_kernel<kWidth, true>, dim3(a.tiles_x * igs::ceil_div(img_height, kTile)), dim3(kTilePixels),
+                        sizeof(igs::SumSmem<kWidth, true>), s, a);
+        }
+        igs::launch(igs::finish_sums_kernel<kValues>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, num_points, channels, conics,
+                    (const float *)sums, false, v_xy, v_conic, v_colors);
+    });
     return igs::check_launch("igs_topk_dropout_bwd");
 }
 

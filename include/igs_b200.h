@@ -279,7 +279,7 @@ int igs_feature_weights(int img_height, int img_width, int num_points, const flo
  * igs_topk_balance_bwd: the gradient of v_loss * loss + sum_g v_importance_g importance_g with the counts held constant (v_loss a device
  * scalar, v_importance [N]; either may be NULL, for 0), from the forward's counts and totals: v_xy [N,2], v_conic [N,3], written whole, or
  * added to when accumulate is not zero. workspace: igs_topk_balance_workspace(N) bytes, 16-byte aligned, whose content need not survive
- * between the two calls. At most 2^31 / 10 pixels. */
+ * between the two calls. At most 2^31 / 10 pixels, 2^24 a side, and 2^26 Gaussians. */
 size_t igs_topk_balance_workspace(int num_points);
 int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const float *xys, const float *conics, const int32_t *pixel_topk,
                          const uint8_t *pixel_mask, float *loss, int32_t *counts, float *importance, int64_t *totals, void *workspace,
@@ -296,7 +296,7 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
  * counters (i, j, offset low, offset high), j = 0 and 1, slot k < 8 draws the upper 24 bits of word k, slots 8 and 9 the low bytes of words
  * 0, 1, 2 and 3, 4, 5 (the first most significant). rng_used [2] gets the values that the pass saw; the backward pass takes them, so the
  * caller may move rng_state on in between, in a captured graph too. igs_topk_dropout_bwd writes v_xy [N,2], v_conic [N,3] and v_colors
- * [N,C] whole, from v_output [C,H,W]. 1 to 12 channels, at most 2^31 / 10 pixels. workspace: igs_topk_dropout_workspace(N, C) bytes,
+ * [N,C] whole, from v_output [C,H,W]. 1 to 12 channels, sizes as above. workspace: igs_topk_dropout_workspace(N, C) bytes,
  * 16-byte aligned, whose content need not survive between the two calls. */
 size_t igs_topk_dropout_workspace(int num_points, int channels);
 int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,

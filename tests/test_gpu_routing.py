@@ -373,3 +373,50 @@ def test_operators_on_a_side_stream(device):
         got = ops.topk_balance_forward(h, w, x, k, t), ops.topk_dropout_forward(h, w, x, k, f, t, 0.2, rng)
     stream.synchronize()
     assert all(torch.equal(a, b) for s, u in zip(want, got) for a, b in zip(s, u))
+
+
+def test_values_that_are_not_finite_stay_where_they_belong(device):
+    """A NaN or infinite image gradient, colour or importance gradient reaches the Gaussians of the pixels concerned, and no other: not
+    those of neighbouring pixels, and nothing at a pixel without a slot."""
+    h, w, n = 16, 40, 60
+    xys, conics, lists = lists_case(h, w, n, 51, empty=0.5)
+    lists[2, 5] = -1
+    x, k, t = to_gpu(device, xys, conics, lists)
+    rng = torch.tensor([1, 1], device=device)
+    f, v = torch.randn(n, 3, device=device), torch.randn(3, h, w, device=device)
+    used = ops.topk_dropout_forward(h, w, x, k, f, t, 0.0, rng)[1]
+    g = routing.Gates(h, w, np_(x), np_(k), lists)
+    holds = lambda i, j: set(g.ids.reshape(h, w, 10)[i, j][g.weight.reshape(h, w, 10)[i, j] > 1e-37])  # noqa: E731
+    clean = ops.topk_dropout_backward(h, w, x, k, f, v, t, 0.0, used)
+
+    def compare(got, want, touched):
+        others = np.setdiff1d(np.arange(n), list(touched))
+        assert len(others) > 10
+        for a, b in zip(got, want):
+            a, b = np_(a)[others], np_(b)[others]
+            assert np.all(np.isfinite(a)) and np.all(abs(a - b) <= 1e-4 * abs(b) + 1e-5 * abs(b).max())  # paths that sum in other orders
+
+    bad = v.clone()
+    bad[1, 2, 5], bad[0, 9, 33] = float("nan"), float("inf")  # (2, 5) has no slot
+    got = ops.topk_dropout_backward(h, w, x, k, f, bad, t, 0.0, used)
+    compare(got, clean, holds(9, 33))
+    assert all(not torch.isfinite(got[2][i]).all() for i in holds(9, 33))
+
+    alpha = torch.randn(n, device=device)
+    alpha[7] = float("nan")
+    _, counts, _, totals = ops.topk_balance_forward(h, w, x, k, t)
+    want = ops.topk_balance_backward(h, w, x, k, t, counts, totals, None, torch.where(torch.isnan(alpha), 0.0, alpha))
+    got = ops.topk_balance_backward(h, w, x, k, t, counts, totals, None, alpha)
+    together = set().union(*(holds(i, j) for i in range(h) for j in range(w) if 7 in holds(i, j)))
+    apart = np.setdiff1d(np.arange(n), list(together))
+    if len(apart) > 10:
+        compare(got, want, together)
+    one = torch.full((h, w, 10), -1, dtype=torch.int32, device=device)  # each Gaussian alone in its pixel: only the broken one is touched
+    one.view(-1, 10)[:n, 4] = torch.arange(n, device=device, dtype=torch.int32)
+    _, counts, _, totals = ops.topk_balance_forward(h, w, x, k, one)
+    got = ops.topk_balance_backward(h, w, x, k, one, counts, totals, None, alpha)
+    want = ops.topk_balance_backward(h, w, x, k, one, counts, totals, None, torch.where(torch.isnan(alpha), 0.0, alpha))
+    compare(got, want, {7})
+    f2 = f.clone()
+    f2[7] = float("inf")
+    compare(ops.topk_dropout_backward(h, w, x, k, f2, v, one, 0.0, used), ops.topk_dropout_backward(h, w, x, k, f, v, one, 0.0, used), {7})
