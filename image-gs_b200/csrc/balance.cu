@@ -12,7 +12,7 @@
 
 namespace {
 
-using igs::kRowsPerPass;
+using igs::kGroup;
 using igs::kTile;
 using igs::kTilePixels;
 using igs::kTopK;
@@ -55,110 +55,132 @@ struct BalanceSmem {
     union {
         alignas(16) int lists[igs::kListWords];
         struct {
-            alignas(16) float weight[8][kRowsPerPass * kWeightPitch];
-            alignas(16) float inv[8][32];
+            alignas(16) float weight[igs::kWarps][kGroup * kWeightPitch];
+            alignas(16) float inv[igs::kWarps][32];
         };
     };
-    float4 rows[igs::kMaxRows];
-    float rows_c[igs::kMaxRows];
+    float4 rows[igs::kMaxRows * igs::Rows<0>::kRowQuads];
+    float4 group[igs::kWarps][igs::Rows<0>::kGroupQuads];
+};
+
+struct BalanceArgs {
+    int tiles_x, img_h, img_w, n;
+    const float *xys, *conics;
+    const int *pixel_topk;
+    const uint8_t *mask;
+    float scale;  // 2^fraction bits
+    int *counts;
+    unsigned long long *fixed;
+    BalanceWorkspace *ws;
 };
 
 // One pixel's slots one by one, from global memory (topk_sums.cuh says when)
-__device__ __noinline__ void count_slots(const int p, const int img_w, const int n, const float *xys, const float *conics,
-                                         const int *pixel_topk, const float scale, int *counts, unsigned long long *fixed) {
-    const float px = (float)(p % img_w), py = (float)(p / img_w);
-    const int *list = pixel_topk + (size_t)p * kTopK;
+__device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
+    const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
+    const int *list = a.pixel_topk + (size_t)p * kTopK;
     float total = (float)igs::kNormEps;
     for (int pass = 0; pass < 2; ++pass) {
         const float inv = 1.f / total;
         for (int k = 0; k < kTopK; ++k) {
             const int id = list[k];
-            if ((unsigned)id >= (unsigned)n) continue;
-            const igs::RowGeometry g = igs::stage_geometry(xys, conics, id);
-            const float e = igs::row_exponent(make_float4(g.x, g.y, g.a, g.b), g.c, px, py);
-            const float w = e <= 0.f ? igs::exp2_approx(e) : 0.f;
+            if ((unsigned)id >= (unsigned)a.n) continue;
+            const float w = igs::slot_weight(igs::stage_geometry(a.xys, a.conics, id), px, py);
             if (pass == 0) {
                 total += w;
             } else {
-                atomicAdd(&counts[id], 1);
-                atomicAdd(&fixed[id], (unsigned long long)__float2ll_rn(w * inv * scale));
+                atomicAdd(&a.counts[id], 1);
+                atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(w * inv * a.scale));
             }
         }
     }
 }
 
-__global__ void __launch_bounds__(kTilePixels, 5) balance_kernel(const int tiles_x, const int img_h, const int img_w, const int n,
-                                                              const float *__restrict__ xys, const float *__restrict__ conics,
-                                                              const int *__restrict__ pixel_topk, const uint8_t *__restrict__ mask,
-                                                              const float scale, int *__restrict__ counts,
-                                                              unsigned long long *__restrict__ fixed, BalanceWorkspace *__restrict__ ws) {
+__global__ void __launch_bounds__(kTilePixels, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
+    using Rows = igs::Rows<0>;
     __shared__ __align__(16) BalanceSmem sm;
     igs::wait_for_predecessor();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int i0 = (blockIdx.x / tiles_x) * kTile, j0 = (blockIdx.x % tiles_x) * kTile;
+    const int i0 = (blockIdx.x / a.tiles_x) * kTile, j0 = (blockIdx.x % a.tiles_x) * kTile;
     const int i = i0 + igs::patch_y(), j = j0 + igs::patch_x();
-    const bool inside = i < img_h && j < img_w;
-    const int p = inside ? i * img_w + j : 0;
-    igs::load_lists(sm.lists, sm.table, pixel_topk, i0, j0, img_h, img_w);
-    const unsigned keep = inside && (mask == nullptr || mask[p] != 0) ? ~0u : 0u;
-    igs::finish_lists();
+    const bool inside = i < a.img_h && j < a.img_w;
+    const int p = inside ? i * a.img_w + j : 0;
+    igs::load_lists(sm.lists, sm.table, a.pixel_topk, i0, j0, a.img_h, a.img_w);
+    const unsigned keep = inside && (a.mask == nullptr || a.mask[p] != 0) ? ~0u : 0u;
+    igs::seed_table(sm.table, sm.lists, i0, j0, a.img_h, a.img_w, a.n);
     igs::PixelSlots s;
-    igs::place_slots(s, sm.table, sm.lists, n, keep);
+    igs::place_slots(s, sm.table, sm.lists, a.n, keep);
     const int routed = __syncthreads_count(s.filled > 0);
-    if (threadIdx.x == 0 && routed > 0) atomicAdd(&ws->routed, (unsigned long long)routed);
+    if (threadIdx.x == 0 && routed > 0) atomicAdd(&a.ws->routed, (unsigned long long)routed);
     const int count = sm.table.count;
     if (count > igs::kMaxRows) {
-        if (keep) count_slots(p, img_w, n, xys, conics, pixel_topk, scale, counts, fixed);
+        if (keep) count_slots(a, p);
         return;
     }
     igs::rank_rows(sm.table, count, [&](const int row, const int id) {
-        const igs::RowGeometry g = igs::stage_geometry(xys, conics, id);
-        sm.rows[row] = make_float4(g.x, g.y, g.a, g.b), sm.rows_c[row] = g.c;
+        const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
+        sm.rows[2 * row] = make_float4(g.x, g.y, g.a, g.b), sm.rows[2 * row + 1] = make_float4(g.c, 0.f, 0.f, 0.f);
     });
     __syncthreads();
     if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count))) {
-        if (keep) count_slots(p, img_w, n, xys, conics, pixel_topk, scale, counts, fixed);
+        if (keep) count_slots(a, p);
         return;
     }
-    // a lane is a pixel: the first rows' weights and the sum over all; a lane is half a row: its gates' sum (topk_sums.cuh)
-    const float px = (float)j, py = (float)i;
+    // a lane is a pixel: the first group's weights and the sum over all (topk_sums.cuh). The sign of a weight says whether the slot is
+    // there: -0 for an absent one (which adds nothing either), so that counts come from the same words as the sums.
     float *const weight = sm.weight[warp];
-    const int half = lane >> 4, r = lane & (kRowsPerPass - 1);
-    float total = (float)igs::kNormEps;
-    int visited = 0, my_row = 0, my_count = 0;
-    auto visit = [&](const int slot, const int row, const bool held) {
-        const float e = igs::row_exponent(sm.rows[row], sm.rows_c[row], px, py);
-        const float w = held && e <= 0.f ? igs::exp2_approx(e) : 0.f;
-        if (slot >= 0 && slot < kRowsPerPass) {
-            weight[slot * kWeightPitch + lane] = w;
-            const int holders = __popc(__ballot_sync(0xffffffffu, held));
-            if (r == slot) my_row = row, my_count = holders;
-        }
-        return w;
-    };
-    igs::visit_rows(s, count, [&](const int row, const bool held) { total += visit(visited++, row, held); });
-    sm.inv[warp][lane] = 1.f / total;
-    for (int first = 0; first < visited; first += kRowsPerPass) {
-        if (first > 0) {
-            __syncwarp();
-            int at = 0;
-            igs::visit_rows(s, count, [&](const int row, const bool held) { visit(at++ - first, row, held); });
+    float4 *const group = sm.group[warp];
+    const float2 minus_x = make_float2(-(float)j, -(float)j), minus_y = make_float2(-(float)i, -(float)i);
+    const int half = lane >> 4, r = lane & (kGroup - 1);
+    float2 total = make_float2(0.f, 0.f);
+    int my_row = 0, my_rows = 0;
+    auto weigh = [&](const int first, const unsigned bits, const int begin, const int n, const bool keep_weights) {
+        const int row = Rows::gather(sm.rows, sm.table.order[warp], begin, n, first, group).row;
+        if (keep_weights) my_row = row, my_rows = min(n - begin, kGroup);
+        __syncwarp();
+        for (int pair = 0; 2 * pair < min(n - begin, kGroup); ++pair) {
+            const float4 *q = group + pair * Rows::kPairQuads;
+            const float2 w = Rows::weights(q, bits, minus_x, minus_y);
+            total = igs::add2(total, w);
+            if (keep_weights) {
+                weight[2 * pair * kWeightPitch + lane] = (bits & __float_as_uint(q[2].z)) != 0 ? w.x : -0.f;
+                weight[(2 * pair + 1) * kWeightPitch + lane] = (bits & __float_as_uint(q[2].w)) != 0 ? w.y : -0.f;
+            }
         }
         __syncwarp();
+    };
+    // a lane is half a row: its gates' sum and its holders
+    auto sum_rows = [&]() {
         float sum = 0.f;
+        int absent = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float4 w = *reinterpret_cast<const float4 *>(&weight[r * kWeightPitch + half * 16 + q * 4]);
             const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[warp][half * 16 + q * 4]);
             sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
+            absent += (int)((__float_as_uint(w.x) >> 31) + (__float_as_uint(w.y) >> 31) + (__float_as_uint(w.z) >> 31) +
+                            (__float_as_uint(w.w) >> 31));
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (r < visited - first) {
+        absent += __shfl_xor_sync(0xffffffffu, absent, 16);
+        if (r < my_rows) {
             const int id = sm.table.sorted[my_row];
-            if (half == 0) atomicAdd(&counts[id], my_count);
-            else atomicAdd(&fixed[id], (unsigned long long)__float2ll_rn(sum * scale));
+            if (half == 0) atomicAdd(&a.counts[id], 32 - absent);
+            else atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
         }
-    }
+        __syncwarp();
+    };
+    const int groups = igs::visit_groups(
+        s, sm.table, count,
+        [&](const int at, const int first, const unsigned bits, const int begin, const int n) { weigh(first, bits, begin, n, at == 0); });
+    sm.inv[warp][lane] = 1.f / (total.x + total.y + (float)igs::kNormEps);
+    __syncwarp();
+    if (groups > 0) sum_rows();
+    if (groups > 1)
+        igs::visit_groups(s, sm.table, count, [&](const int at, const int first, const unsigned bits, const int begin, const int n) {
+            if (at == 0) return;
+            weigh(first, bits, begin, n, true);
+            sum_rows();
+        });
 }
 
 // importance from the fixed-point sums, and the loss: each block's sums of counts and of counts * importance (in double, in thread order),
@@ -249,8 +271,9 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, counts, fixed, ws);
     if (pixels > 0 && num_points > 0) {
         const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
-        igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, tiles_x, img_height, img_width, num_points, xys, conics,
-                    pixel_topk, pixel_mask, (float)((int64_t)1 << bits), counts, fixed, ws);
+        const BalanceArgs a = {tiles_x, img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
+                               (float)((int64_t)1 << bits), counts, fixed, ws};
+        igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
     }
     igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
                 (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,
@@ -281,8 +304,7 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
         a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.n = num_points;
         a.xys = xys, a.conics = conics, a.pixel_topk = pixel_topk, a.mask = pixel_mask;
         a.counts = counts, a.scale = &ws->scale, a.v_importance = v_importance, a.sums = sums;
-        igs::launch(igs::sums_kernel<1, false>, dim3(a.tiles_x * igs::ceil_div(img_height, kTile)), dim3(kTilePixels),
-                    sizeof(igs::SumSmem<1, false>), s, a);
+        igs::launch_sums<1, false>(a, s);
     }
     igs::launch(igs::finish_sums_kernel<SumsOf::kValues>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, num_points, 0, conics,
                 (const float *)sums, accumulate != 0, v_xy, v_conic, (float *)nullptr);

@@ -18,7 +18,8 @@ template <int C>
 struct DropoutSmem {
     igs::TileTable table;
     alignas(16) int lists[igs::kListWords];
-    float4 rows[igs::kMaxRows * igs::SumLayout<C, true>::kRowQuads];
+    float4 rows[igs::kMaxRows * igs::Rows<C>::kRowQuads];
+    float4 group[igs::kWarps][igs::Rows<C>::kGroupQuads];
 };
 
 struct DropoutArgs {
@@ -42,10 +43,8 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p, cons
         for (int k = 0; k < kTopK; ++k) {
             const int id = list[k];
             if ((unsigned)id >= (unsigned)a.n || !(keep >> k & 1)) continue;
-            const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
-            const float e = igs::row_exponent(make_float4(g.x, g.y, g.a, g.b), g.c, px, py);
-            if (!(e <= 0.f)) continue;
-            const float w = igs::exp2_approx(e);
+            const float w = igs::slot_weight(igs::stage_geometry(a.xys, a.conics, id), px, py);
+            if (w == 0.f) continue;
             total += w;
             pix = fmaf(w, __ldg(&a.colors[(size_t)id * a.channels + c]), pix);
         }
@@ -56,7 +55,8 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p, cons
 template <int C>
 __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 6 : 4)
     dropout_kernel(const __grid_constant__ DropoutArgs a) {
-    constexpr int kQuads = igs::SumLayout<C, true>::kRowQuads;
+    using Rows = igs::Rows<C>;
+    constexpr int kRowQuads = Rows::kRowQuads;
     __shared__ __align__(16) DropoutSmem<C> sm;
     igs::wait_for_predecessor();
     const int i0 = (blockIdx.x / a.tiles_x) * kTile, j0 = (blockIdx.x % a.tiles_x) * kTile;
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 6 : 4)
     const long long seed = a.rng[0], offset = a.rng[1];
     if (blockIdx.x == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
     const unsigned keep = inside ? igs::keep_bits((uint32_t)p, (uint64_t)seed, (uint64_t)offset, a.threshold) : 0u;
-    igs::finish_lists();
+    igs::seed_table(sm.table, sm.lists, i0, j0, a.img_h, a.img_w, a.n);
     igs::PixelSlots s;
     igs::place_slots(s, sm.table, sm.lists, a.n, keep);
     __syncthreads();
@@ -78,44 +78,51 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 6 : 4)
     }
     igs::rank_rows(sm.table, count, [&](const int row, const int id) {
         const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
-        float q[4 * kQuads];
+        float q[4 * kRowQuads];
         q[0] = g.x, q[1] = g.y, q[2] = g.a, q[3] = g.b, q[4] = g.c;
+        bool finite = true;
 #pragma unroll
-        for (int c = 0; c < 4 * kQuads - 5; ++c) q[5 + c] = c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
+        for (int c = 0; c < 4 * kRowQuads - 5; ++c) {
+            q[5 + c] = c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
+            finite = finite && isfinite(q[5 + c]);
+        }
+        if (!finite) sm.table.per_slot = 1;  // zero times it would reach pixels that do not name it
 #pragma unroll
-        for (int e = 0; e < kQuads; ++e) sm.rows[row * kQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
+        for (int e = 0; e < kRowQuads; ++e) sm.rows[row * kRowQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
     });
     __syncthreads();
-    if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count))) {
+    if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count) && sm.table.per_slot == 0)) {
         if (inside) blend_slots(a, p, keep);
         return;
     }
-    const float px = (float)j, py = (float)i;
-    float total = (float)igs::kNormEps;
-    float pix[C];
+    const int warp = threadIdx.x >> 5;
+    float4 *const group = sm.group[warp];
+    const float2 minus_x = make_float2(-(float)j, -(float)j), minus_y = make_float2(-(float)i, -(float)i);
+    float2 total = make_float2(0.f, 0.f), pix[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) pix[c] = 0.f;
-    igs::visit_rows(s, count, [&](const int row, const bool held) {
-        float q[4 * kQuads];
+    for (int c = 0; c < C; ++c) pix[c] = make_float2(0.f, 0.f);
+    igs::visit_groups(s, sm.table, count, [&](const int, const int first, const unsigned bits, const int begin, const int n) {
+        Rows::gather(sm.rows, sm.table.order[warp], begin, n, first, group);
+        __syncwarp();
+        for (int pair = 0; 2 * pair < min(n - begin, igs::kGroup); ++pair) {
+            const float4 *q = group + pair * Rows::kPairQuads;
+            const float2 w = Rows::weights(q, bits, minus_x, minus_y);
+            total = igs::add2(total, w);
 #pragma unroll
-        for (int e = 0; e < kQuads; ++e) {
-            const float4 v = sm.rows[row * kQuads + e];
-            q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
+            for (int c = 0; c < C; c += 2) {
+                const float4 f = q[3 + c / 2];
+                pix[c] = igs::fma2(w, make_float2(f.x, f.y), pix[c]);
+                if (c + 1 < C) pix[c + 1 < C ? c + 1 : c] = igs::fma2(w, make_float2(f.z, f.w), pix[c + 1 < C ? c + 1 : c]);
+            }
         }
-        const float e = igs::row_exponent(make_float4(q[0], q[1], q[2], q[3]), q[4], px, py);
-        if (held && e <= 0.f) {
-            const float w = igs::exp2_approx(e);
-            total += w;
-#pragma unroll
-            for (int c = 0; c < C; ++c) pix[c] = fmaf(w, q[5 + c], pix[c]);
-        }
+        __syncwarp();
     });
     if (!inside) return;
-    const float inv = 1.f / total;
+    const float inv = 1.f / (total.x + total.y + (float)igs::kNormEps);
     const size_t plane = (size_t)a.img_h * a.img_w;
 #pragma unroll
     for (int c = 0; c < C; ++c)
-        if (c < a.channels) a.out_img[c * plane + p] = pix[c] * inv;
+        if (c < a.channels) a.out_img[c * plane + p] = (pix[c].x + pix[c].y) * inv;
 }
 
 __global__ void rng_used_kernel(const long long *rng, long long *rng_used) {
@@ -209,8 +216,7 @@ int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_po
             a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
             a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
             a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0), a.sums = sums;
-            igs::launch(igs::sums_kernel<kWidth, true>, dim3(a.tiles_x * igs::ceil_div(img_height, kTile)), dim3(kTilePixels),
-                        sizeof(igs::SumSmem<kWidth, true>), s, a);
+            igs::launch_sums<kWidth, true>(a, s);
         }
         igs::launch(igs::finish_sums_kernel<kValues>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, num_points, channels, conics,
                     (const float *)sums, false, v_xy, v_conic, v_colors);

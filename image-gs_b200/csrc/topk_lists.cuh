@@ -43,28 +43,32 @@ __device__ __forceinline__ unsigned keep_bits(uint32_t pixel, uint64_t seed, uin
 // ---- a tile's Gaussians as rows --------------------------------------------------------------------------------------------------------
 //
 // One CTA of 256 threads takes a 16x16 tile, a warp an 8x4 patch of it, a lane one pixel. Neighbouring pixels name nearly the same
-// Gaussians (at a trained image's 100 pixels per Gaussian the 2560 slots of a tile name about 25, a patch about 14), so the tile's distinct
+// Gaussians (at a trained image's 100 pixels per Gaussian the 2560 slots of a tile name 18 to 23, a patch 13 to 14), so the tile's distinct
 // IDs become rows: a hash table in shared memory collects them, they are ranked by ID (so that every sum over rows has one order, whatever
-// thread came first), and each row's parameters are staged once. A pixel's slots are then bits of a row mask, and a warp visits the rows
-// that any of its pixels holds, reading the parameters as broadcasts: no gather per slot, and sums per Gaussian become sums along a row.
-constexpr int kTableBits = 9;
+// thread came first), and each row's parameters are staged once. A pixel's slots are then bits of a row mask. A warp takes the rows that
+// any of its pixels holds in groups of 16, copied side by side in pairs: it reads them as broadcasts, two rows per packed (f32x2)
+// instruction, with no gather per slot, and sums per Gaussian become sums along a row.
+constexpr int kTableBits = 10;
 constexpr int kTableSize = 1 << kTableBits;
-constexpr int kMaxRows = 128;       // more distinct IDs in a tile than this (or an ID twice in a pixel) take the per-slot path
+constexpr int kMaxRows = 128;   // more distinct IDs in a tile than this (or an ID twice in a pixel) take the per-slot path
+constexpr int kGroup = 16;      // rows of a warp's group
 constexpr int kNoRow = 0xFF;
-constexpr int kListPitch = 176;     // words per row of 16 pixels: 160, padded so that the 8x4 patches' 8-byte reads do not conflict
+constexpr int kListPitch = 176;  // words per row of 16 pixels: 160, padded so that the 8x4 patches' 8-byte reads do not conflict
 constexpr int kListWords = kTile * kListPitch;
+constexpr int kWarps = kTilePixels / 32;
 
 struct alignas(16) TileTable {
-    int ids[kTableSize];            // -1: free
+    int ids[kTableSize];        // -1: free
     uint8_t row[kTableSize];
-    int found[kMaxRows];            // distinct IDs in the order found, and their places in the table
+    int found[kMaxRows];        // distinct IDs in the order found, and their places in the table
     uint16_t place[kMaxRows];
-    int sorted[kMaxRows];           // the same by rank
+    int sorted[kMaxRows];       // the same by rank
+    uint8_t order[kWarps][32];  // a warp's rows of the current 32, closed up
     int count;
-    int per_slot;                   // set when a row's values ask for the per-slot path
+    int per_slot;               // set when a row's values ask for the per-slot path
 };
 
-// Copies the tile's lists into shared memory (asynchronously; wait with finish_lists) and clears the table
+// Copies the tile's lists into shared memory (asynchronously; finish_lists waits) and clears the table
 __device__ __forceinline__ void load_lists(int *s_lists, TileTable &t, const int *pixel_topk, const int i0, const int j0, const int img_h,
                                            const int img_w) {
     const int pairs = min(kTile, img_w - j0) * (kTopK / 2);  // 8-byte words of a row that lie in the image
@@ -79,19 +83,18 @@ __device__ __forceinline__ void load_lists(int *s_lists, TileTable &t, const int
             asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
         }
     }
-    for (int e = threadIdx.x; e < kTableSize; e += kTilePixels) t.ids[e] = -1;
+#pragma unroll
+    for (int e = 0; e < kTableSize / 4 / kTilePixels; ++e)
+        reinterpret_cast<int4 *>(t.ids)[e * kTilePixels + threadIdx.x] = make_int4(-1, -1, -1, -1);
     if (threadIdx.x == 0) t.count = 0, t.per_slot = 0;
 }
 
-__device__ __forceinline__ void finish_lists() {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-}
+__device__ __forceinline__ int hash_of(const int id) { return (int)((unsigned)id * 2654435761u >> (32 - kTableBits)); }
 
 // The place of id in the table, found or made. A new ID takes the next entry of found[]; count past kMaxRows means that the tile does not
 // fit (the place returned is then meaningless, and so it is when the table is full).
-__device__ __forceinline__ int table_place(TileTable &t, const int id) {
-    int h = (int)((unsigned)id * 2654435761u >> (32 - kTableBits));
+static __device__ __noinline__ int table_place(TileTable &t, const int id) {
+    int h = hash_of(id);
     for (int probe = 0; probe < kTableSize; ++probe, h = (h + 1) & (kTableSize - 1)) {
         int v = *(volatile int *)&t.ids[h];
         if (v == id) break;
@@ -107,6 +110,58 @@ __device__ __forceinline__ int table_place(TileTable &t, const int id) {
         }
     }
     return h;
+}
+
+// Waits for the lists, then enters the IDs of 25 pixels spread over the tile, a thread each: nearly all of the tile's, so that afterwards
+// most pixels only look theirs up. (Slots that the caller leaves out may enter too: a row that nobody holds is never visited.)
+__device__ __forceinline__ void seed_table(TileTable &t, const int *s_lists, const int i0, const int j0, const int img_h, const int img_w,
+                                           const int n) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    const int pixel = threadIdx.x / kTopK, slot = threadIdx.x % kTopK;
+    const int y = (pixel / 5) * 15 / 4, x = (pixel % 5) * 15 / 4;  // 0, 3, 7, 11, 15
+    if (pixel < 25 && i0 + y < img_h && j0 + x < img_w) {
+        const int id = s_lists[y * kListPitch + x * kTopK + slot];
+        if ((unsigned)id < (unsigned)n) table_place(t, id);
+    }
+    __syncthreads();
+}
+
+// The pixel of a thread: warp w covers the 8x4 patch (w % 2, w / 2) of the tile, lane l its pixel (l % 8, l / 8)
+__device__ __forceinline__ int patch_x() { return (threadIdx.x >> 5 & 1) * 8 + (threadIdx.x & 7); }
+__device__ __forceinline__ int patch_y() { return (threadIdx.x >> 6) * 4 + (threadIdx.x >> 3 & 3); }
+
+// A pixel's slots: first their places in the table (-1: empty), then their rows
+struct PixelSlots {
+    int place[kTopK];
+    unsigned rows[3];  // a byte per slot, kNoRow for an empty one
+    unsigned bits;     // rows 0-31 as a mask
+    int filled;
+};
+
+// From the pixel's list in shared memory; keep holds a bit per slot that may be filled
+__device__ __forceinline__ void place_slots(PixelSlots &s, TileTable &t, const int *s_lists, const int n, const unsigned keep) {
+    const int *list = s_lists + patch_y() * kListPitch + patch_x() * kTopK;
+    s.filled = 0;
+    unsigned missing = 0;
+#pragma unroll
+    for (int k = 0; k < kTopK; k += 2) {
+        const int2 v = *reinterpret_cast<const int2 *>(list + k);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int id = b ? v.y : v.x;
+            const bool filled = (unsigned)id < (unsigned)n && (keep >> (k + b) & 1) != 0;
+            const int h = hash_of(id);
+            s.place[k + b] = filled ? h : -1;
+            s.filled += filled;
+            if (filled && t.ids[h] != id) missing |= 1u << (k + b);
+        }
+    }
+    if (__any_sync(0xffffffffu, missing != 0)) {
+#pragma unroll
+        for (int k = 0; k < kTopK; ++k)
+            if (missing >> k & 1) s.place[k] = table_place(t, list[k]);
+    }
 }
 
 // Ranks the IDs found (count <= kMaxRows), writes each place's row and calls stage(row, id); the caller synchronizes before and after
@@ -127,38 +182,6 @@ __device__ __forceinline__ unsigned bit_or_nothing(const unsigned shift) {
     unsigned r;
     asm("shl.b32 %0, 1, %1;" : "=r"(r) : "r"(shift));
     return r;
-}
-
-// exp2(x) (ex2.approx: 2 ulp, 0 for -inf)
-__device__ __forceinline__ float exp2_approx(const float x) {
-    float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// The pixel of a thread: warp w covers the 8x4 patch (w % 2, w / 2) of the tile, lane l its pixel (l % 8, l / 8)
-__device__ __forceinline__ int patch_x() { return (threadIdx.x >> 5 & 1) * 8 + (threadIdx.x & 7); }
-__device__ __forceinline__ int patch_y() { return (threadIdx.x >> 6) * 4 + (threadIdx.x >> 3 & 3); }
-
-// A pixel's slots: first their places in the table (-1: empty), then their rows
-struct PixelSlots {
-    int place[kTopK];
-    unsigned rows[3];  // a byte per slot, kNoRow for an empty one
-    unsigned bits;     // rows 0-31 as a mask
-    int filled;
-};
-
-// From the pixel's list in shared memory; keep holds a bit per slot that may be filled
-__device__ __forceinline__ void place_slots(PixelSlots &s, TileTable &t, const int *s_lists, const int n, const unsigned keep) {
-    const int2 *list = reinterpret_cast<const int2 *>(s_lists + patch_y() * kListPitch + patch_x() * kTopK);
-    s.filled = 0;
-#pragma unroll
-    for (int k = 0; k < kTopK; k += 2) {
-        const int2 v = list[k / 2];
-        s.place[k] = (unsigned)v.x < (unsigned)n && (keep >> k & 1) ? table_place(t, v.x) : -1;
-        s.place[k + 1] = (unsigned)v.y < (unsigned)n && (keep >> (k + 1) & 1) ? table_place(t, v.y) : -1;
-        s.filled += (s.place[k] >= 0) + (s.place[k + 1] >= 0);
-    }
 }
 
 // The rows of the slots with first <= row < first + 32 as a mask
@@ -184,19 +207,11 @@ __device__ __forceinline__ bool find_rows(PixelSlots &s, const TileTable &t, con
     return distinct == s.filled;
 }
 
-// Calls visit(row, held) for each row that a pixel of the warp holds, in order, held being whether this lane's pixel does; all lanes of the
-// warp together
-template <typename Visit>
-__device__ __forceinline__ void visit_rows(const PixelSlots &s, const int count, Visit visit) {
-    for (int first = 0; first < count; first += 32) {
-        const unsigned bits = first == 0 ? s.bits : row_bits(s, first);
-        unsigned any = __reduce_or_sync(0xffffffffu, bits);
-        while (any) {
-            const int b = __ffs(any) - 1;
-            any &= any - 1;
-            visit(first + b, (bits >> b & 1) != 0);
-        }
-    }
+// exp2(x) (ex2.approx: 2 ulp; results below 2^-126 are 0, far below what eps leaves of a gate)
+__device__ __forceinline__ float exp2_approx(const float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // The staged geometry of a row: centre, and the conic times -log2(e) (its outer terms halved too), so that the weight is exp2 of
@@ -216,9 +231,102 @@ __device__ __forceinline__ RowGeometry stage_geometry(const float *xys, const fl
     return {0.f, 0.f, __int_as_float(0x7fc00000), 0.f, 0.f};
 }
 
-__device__ __forceinline__ float row_exponent(const float4 g, const float c, const float px, const float py) {
+// The weight of one slot, from global memory: the per-slot path
+__device__ __forceinline__ float slot_weight(const RowGeometry &g, const float px, const float py) {
     const float dx = g.x - px, dy = g.y - py;
-    return fmaf(fmaf(c, dy, g.w * dx), dy, (g.z * dx) * dx);
+    const float e = fmaf(fmaf(g.c, dy, g.b * dx), dy, (g.a * dx) * dx);
+    return e <= 0.f ? exp2_approx(e) : 0.f;
+}
+
+// Two float operations in one instruction
+__device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(r))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)), "l"(reinterpret_cast<const uint64_t &>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(const float2 a, const float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(r))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(r))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+    return r;
+}
+
+// A staged row in the CTA's table: x, y, a', b', c', f[C], padded to whole float4s. A warp's group of 16 rows, in 8 pairs of
+// (x x y y) (a' a' b' b') (c' c' m m) (f0 f0 f1 f1) ..., m the row's bit in the mask (0 for a row that pads the last pair).
+template <int C>
+struct Rows {
+    static constexpr int kRowQuads = (5 + C + 3) / 4;
+    static constexpr int kPairQuads = 3 + (C + 1) / 2;
+    static constexpr int kGroupQuads = kGroup / 2 * kPairQuads;
+
+    // This lane's row (lane % 16) of the group from the table, into registers and, by the first 16 lanes, into the warp's group
+    struct Mine {
+        int row;
+        float x, y, f[C > 0 ? C : 1];
+    };
+    static __device__ __forceinline__ Mine gather(const float4 *table, const uint8_t *order, const int begin, const int n, const int first,
+                                                  float4 *group) {
+        const int lane = threadIdx.x & 31, r = lane & (kGroup - 1);
+        const int bit = begin + r < n ? order[begin + r] : 0;
+        Mine mine;
+        mine.row = first + bit;
+        float q[4 * kRowQuads];
+#pragma unroll
+        for (int e = 0; e < kRowQuads; ++e) {
+            const float4 v = table[mine.row * kRowQuads + e];
+            q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
+        }
+        mine.x = q[0], mine.y = q[1];
+#pragma unroll
+        for (int c = 0; c < C; ++c) mine.f[c] = q[5 + c];
+        if (lane < kGroup) {
+            float *pair = reinterpret_cast<float *>(group + (r >> 1) * kPairQuads) + (r & 1);
+#pragma unroll
+            for (int e = 0; e < 5; ++e) pair[2 * e] = q[e];
+            reinterpret_cast<unsigned *>(pair)[10] = begin + r < n ? 1u << bit : 0u;
+#pragma unroll
+            for (int c = 0; c < C; ++c) pair[12 + 2 * c] = q[5 + c];
+        }
+        return mine;
+    }
+
+    // The weights of a pair's two rows at a pixel; minus holds (-px, -px), (-py, -py)
+    static __device__ __forceinline__ float2 weights(const float4 *pair, const unsigned bits, const float2 minus_x, const float2 minus_y) {
+        const float4 xy = pair[0], ab = pair[1], cm = pair[2];
+        const float2 dx = add2(make_float2(xy.x, xy.y), minus_x), dy = add2(make_float2(xy.z, xy.w), minus_y);
+        const float2 slope = fma2(make_float2(cm.x, cm.y), dy, mul2(make_float2(ab.z, ab.w), dx));
+        const float2 e = fma2(slope, dy, mul2(mul2(make_float2(ab.x, ab.y), dx), dx));
+        const bool held0 = (bits & __float_as_uint(cm.z)) != 0, held1 = (bits & __float_as_uint(cm.w)) != 0;
+        return make_float2(held0 && e.x <= 0.f ? exp2_approx(e.x) : 0.f, held1 && e.y <= 0.f ? exp2_approx(e.y) : 0.f);
+    }
+};
+
+// Calls visit(first row of the 32, this lane's mask of them, begin, rows of the 32 that the warp holds) for each group of 16 rows that the
+// warp's pixels hold, in order, with t.order closed up for it; all lanes of the warp together. Returns the number of groups.
+template <typename Visit>
+__device__ __forceinline__ int visit_groups(const PixelSlots &s, TileTable &t, const int count, Visit visit) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int groups = 0;
+    for (int first = 0; first < count; first += 32) {
+        const unsigned bits = first == 0 ? s.bits : row_bits(s, first);
+        const unsigned any = __reduce_or_sync(0xffffffffu, bits);
+        const int n = __popc(any);
+        __syncwarp();
+        if (any >> lane & 1) t.order[warp][__popc(any & ((1u << lane) - 1))] = (uint8_t)lane;
+        __syncwarp();
+        for (int begin = 0; begin < n; begin += kGroup, ++groups) visit(groups, first, bits, begin, n);
+    }
+    return groups;
 }
 
 // Host checks of the sizes, shared by the entry points: slots and Gaussians' sums indexed with 32 bits, coordinates exact in float

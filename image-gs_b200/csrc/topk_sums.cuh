@@ -5,19 +5,19 @@
 // a Gaussian's sums are sum t dx, t dy, t dx^2, t dx dy, t dy^2 and (dropout) w v'_c, from which finish_kernel forms
 //   v_xy = (a Sx + b Sy, b Sx + c Sy),  v_conic = (Sxx / 2, Sxy, Syy / 2),  v_f = S_c.
 //
-// A warp (an 8x4 patch, topk_lists.cuh) visits its rows twice. First a lane is a pixel: weights into shared memory (16 rows of 32), D and
-// the scores' sum in registers. Then a lane is half a row: lane l sums row l % 16 over 16 pixels (two patch rows of 8), reading the
-// weights four at a time and the pixels' v' and m' as broadcasts, two pixels per packed (f32x2) instruction; dy is one value per patch row,
-// so t and t dx are summed along it first. One shuffle joins the halves, and the sums go to global memory with one 16-byte vector atomic
-// per four values. A tile with an ID twice in a list, too many IDs or values that are not finite takes the per-slot path instead: zero
-// times a value that is not finite would reach Gaussians that the pixel does not name.
+// A warp (an 8x4 patch, topk_lists.cuh) goes over its rows twice. First a lane is a pixel: weights into shared memory (16 rows of 32), D
+// and the scores' sum in registers. Then a lane is half a row: lane l sums row l % 16 over 16 pixels (two patch rows of 8), reading the
+// weights four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per patch row, so t
+// and t dx are summed along it first. One shuffle joins the halves, and the sums go to global memory with one 16-byte vector atomic per
+// four values. A patch of more than 16 rows computes the later groups' weights again. A tile with an ID twice in a list, too many IDs or
+// values that are not finite takes the per-slot path instead: zero times a value that is not finite would reach Gaussians that the pixel
+// does not name.
 #pragma once
 
 #include "topk_lists.cuh"
 
 namespace igs {
 
-constexpr int kRowsPerPass = 16;
 constexpr int kWeightPitch = 36;  // words: the reads of four pixels by eight lanes (rows) fall on distinct banks
 
 struct SumArgs {
@@ -36,8 +36,7 @@ struct SumArgs {
 // C: the values per row and pixel (1 for balance; 3, 7, 11 or 12 channels, the unused ones zero)
 template <int C, bool kDropout>
 struct SumLayout {
-    static constexpr int kRowQuads = (5 + C + 3) / 4;                         // staged row: x, y, a', b', c', f
-    static constexpr int kValues = ((5 + (kDropout ? C : 0)) + 3) / 4 * 4;    // Sx, Sy, Sxx, Sxy, Syy, S_c
+    static constexpr int kValues = ((5 + (kDropout ? C : 0)) + 3) / 4 * 4;  // Sx, Sy, Sxx, Sxy, Syy, S_c
 };
 
 template <int C, bool kDropout>
@@ -46,34 +45,13 @@ struct SumSmem {
     union {
         alignas(16) int lists[kListWords];
         struct {
-            alignas(16) float weight[8][kRowsPerPass * kWeightPitch];
-            alignas(16) float pixel[8][C + 1][32];  // v'_c, m'
+            alignas(16) float weight[kWarps][kGroup * kWeightPitch];
+            alignas(16) float pixel[kWarps][C + 1][32];  // v'_c, m'
         };
     };
-    float4 rows[kMaxRows * SumLayout<C, kDropout>::kRowQuads];
+    float4 rows[kMaxRows * Rows<C>::kRowQuads];
+    float4 group[kWarps][Rows<C>::kGroupQuads];
 };
-
-__device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t &>(r))
-        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)), "l"(reinterpret_cast<const uint64_t &>(c)));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(const float2 a, const float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t &>(r))
-        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t &>(r))
-        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
-    return r;
-}
 
 // Value c of a Gaussian's score
 template <bool kDropout>
@@ -100,8 +78,7 @@ __device__ __noinline__ void add_slots(const SumArgs &a, const int p, const unsi
             const int id = list[k];
             if ((unsigned)id >= (unsigned)a.n || !(keep >> k & 1)) continue;
             const RowGeometry g = stage_geometry(a.xys, a.conics, id);
-            const float e = row_exponent(make_float4(g.x, g.y, g.a, g.b), g.c, px, py);
-            const float w = e <= 0.f ? exp2_approx(e) : 0.f;
+            const float w = slot_weight(g, px, py);
             if (w == 0.f) continue;
             float score = 0.f;
             for (int c = 0; c < (kDropout ? a.channels : 1); ++c) score += row_value<kDropout>(a, id, c) * pixel_value<kDropout>(a, p, c);
@@ -120,9 +97,9 @@ __device__ __noinline__ void add_slots(const SumArgs &a, const int p, const unsi
 }
 
 template <int C, bool kDropout>
-__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
-    using Layout = SumLayout<C, kDropout>;
-    constexpr int kQuads = Layout::kRowQuads;
+__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
+    constexpr int kValues = SumLayout<C, kDropout>::kValues;
+    constexpr int kRowQuads = Rows<C>::kRowQuads, kPairQuads = Rows<C>::kPairQuads;
     extern __shared__ __align__(16) char smem_bytes[];
     SumSmem<C, kDropout> &sm = *reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes);
     wait_for_predecessor();
@@ -140,7 +117,7 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 3) sums_kernel(const
     float v[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) v[c] = inside ? pixel_value<kDropout>(a, p, c) : 0.f;
-    finish_lists();
+    seed_table(sm.table, sm.lists, i0, j0, a.img_h, a.img_w, a.n);
     PixelSlots s;
     place_slots(s, sm.table, sm.lists, a.n, keep);
     __syncthreads();
@@ -151,53 +128,50 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 3) sums_kernel(const
     }
     rank_rows(sm.table, count, [&](const int row, const int id) {
         const RowGeometry g = stage_geometry(a.xys, a.conics, id);
-        float q[4 * kQuads];
+        float q[4 * kRowQuads];
         q[0] = g.x, q[1] = g.y, q[2] = g.a, q[3] = g.b, q[4] = g.c;
         bool finite = true;
 #pragma unroll
-        for (int c = 0; c < 4 * kQuads - 5; ++c) {
+        for (int c = 0; c < 4 * kRowQuads - 5; ++c) {
             q[5 + c] = c < C ? row_value<kDropout>(a, id, c) : 0.f;
             finite = finite && isfinite(q[5 + c]);
         }
         if (!finite) sm.table.per_slot = 1;
 #pragma unroll
-        for (int e = 0; e < kQuads; ++e) sm.rows[row * kQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
+        for (int e = 0; e < kRowQuads; ++e) sm.rows[row * kRowQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
     });
     __syncthreads();
     bool regular = find_rows(s, sm.table, count) && sm.table.per_slot == 0;
-    const float px = (float)j, py = (float)i;
-    auto load_row = [&](const int row, float (&q)[4 * kQuads]) {
-#pragma unroll
-        for (int e = 0; e < kQuads; ++e) {
-            const float4 r = sm.rows[row * kQuads + e];
-            q[4 * e] = r.x, q[4 * e + 1] = r.y, q[4 * e + 2] = r.z, q[4 * e + 3] = r.w;
-        }
-    };
-    // a lane is a pixel: the first kRowsPerPass rows' weights, the sums over all rows
     float *const weight = sm.weight[warp];
-    float total = (float)kNormEps, scores = 0.f;
-    int visited = 0, my_row = 0;
-    visit_rows(s, count, [&](const int row, const bool held) {
-        float q[4 * kQuads];
-        load_row(row, q);
-        const float e = row_exponent(make_float4(q[0], q[1], q[2], q[3]), q[4], px, py);
-        float w = 0.f;
-        if (held && e <= 0.f) {
-            w = exp2_approx(e);
-            float score = 0.f;
+    float4 *const group = sm.group[warp];
+    const float2 minus_x = make_float2(-(float)j, -(float)j), minus_y = make_float2(-(float)i, -(float)i);
+    // a lane is a pixel: the first group's weights, the sums over all groups
+    typename Rows<C>::Mine mine;
+    float2 total2 = make_float2(0.f, 0.f), scores2 = make_float2(0.f, 0.f);
+    int first_rows = 0;
+    const int groups = visit_groups(s, sm.table, count, [&](const int at, const int first, const unsigned bits, const int begin, const int n) {
+        const typename Rows<C>::Mine got = Rows<C>::gather(sm.rows, sm.table.order[warp], begin, n, first, group);
+        if (at == 0) mine = got, first_rows = min(n - begin, kGroup);
+        __syncwarp();
+        for (int pair = 0; 2 * pair < min(n - begin, kGroup); ++pair) {
+            const float4 *q = group + pair * kPairQuads;
+            const float2 w = Rows<C>::weights(q, bits, minus_x, minus_y);
+            float2 score = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < C; ++c) score = fmaf(q[5 + c], v[c], score);
-            total += w;
-            scores = fmaf(w, score, scores);
+            for (int c = 0; c < C; c += 2) {
+                const float4 f = q[3 + c / 2];
+                score = fma2(make_float2(f.x, f.y), make_float2(v[c], v[c]), score);
+                if (c + 1 < C) score = fma2(make_float2(f.z, f.w), make_float2(v[c + 1 < C ? c + 1 : c], v[c + 1 < C ? c + 1 : c]), score);
+            }
+            total2 = add2(total2, w);
+            scores2 = fma2(w, score, scores2);
+            if (at == 0) weight[2 * pair * kWeightPitch + lane] = w.x, weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
         }
-        if (visited < kRowsPerPass) {
-            weight[visited * kWeightPitch + lane] = w;
-            if ((lane & (kRowsPerPass - 1)) == visited) my_row = row;
-        }
-        ++visited;
+        __syncwarp();
     });
-    const bool some = total > (float)kNormEps;  // a pixel without a weight adds nothing, whatever its values
-    const float inv = 1.f / total, m = some ? scores * inv * inv : 0.f;
+    const float total = total2.x + total2.y, scores = scores2.x + scores2.y;
+    const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
+    const float inv = 1.f / (total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
     float size = fabsf(m);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -212,29 +186,14 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 3) sums_kernel(const
         return;
     }
     // a lane is half a row
-    const int half = lane >> 4, r = lane & (kRowsPerPass - 1);
+    const int half = lane >> 4, r = lane & (kGroup - 1);
     const float x0 = (float)(j0 + (warp & 1) * 8), y0 = (float)(i0 + (warp >> 1) * 4 + half * 2);
-    for (int first = 0; first < visited; first += kRowsPerPass) {
-        if (first > 0) {  // a patch of more than 16 rows: the next ones' weights again
-            __syncwarp();
-            int at = 0;
-            visit_rows(s, count, [&](const int row, const bool held) {
-                const int slot = at++ - first;
-                if (slot < 0 || slot >= kRowsPerPass) return;
-                const float4 g = sm.rows[row * kQuads];
-                const float e = row_exponent(g, sm.rows[row * kQuads + 1].x, px, py);
-                weight[slot * kWeightPitch + lane] = held && e <= 0.f ? exp2_approx(e) : 0.f;
-                if (r == slot) my_row = row;
-            });
-        }
-        __syncwarp();
-        float q[4 * kQuads];
-        load_row(my_row, q);
+    auto sum_rows = [&](const int rows) {
         float2 dx[4], f[C], color[C];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dx[e] = make_float2(q[0] - (x0 + (float)(2 * e)), q[0] - (x0 + (float)(2 * e + 1)));
+        for (int e = 0; e < 4; ++e) dx[e] = make_float2(mine.x - (x0 + (float)(2 * e)), mine.x - (x0 + (float)(2 * e + 1)));
 #pragma unroll
-        for (int c = 0; c < C; ++c) f[c] = make_float2(-q[5 + c], -q[5 + c]), color[c] = make_float2(0.f, 0.f);
+        for (int c = 0; c < C; ++c) f[c] = make_float2(-mine.f[c], -mine.f[c]), color[c] = make_float2(0.f, 0.f);
         float2 xx = make_float2(0.f, 0.f);
         float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
 #pragma unroll
@@ -259,28 +218,51 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 3) sums_kernel(const
                 ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
                 xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
             }
-            const float dy = q[1] - (y0 + (float)y);
+            const float dy = mine.y - (y0 + (float)y);
             const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
             sx += ur, sy += ty;
             sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
         }
-        float sum[Layout::kValues];
+        float sum[kValues];
 #pragma unroll
-        for (int e = 0; e < Layout::kValues; ++e) sum[e] = 0.f;
+        for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
         sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
         if constexpr (kDropout) {
 #pragma unroll
             for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
         }
 #pragma unroll
-        for (int e = 0; e < Layout::kValues; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
-        if (r < visited - first) {
-            float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)sm.table.sorted[my_row] * Layout::kValues);
+        for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
+        if (r < rows) {
+            float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)sm.table.sorted[mine.row] * kValues);
 #pragma unroll
-            for (int e = 0; e < Layout::kValues / 4; ++e)
+            for (int e = 0; e < kValues / 4; ++e)
                 if ((e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
         }
-    }
+    };
+    __syncwarp();
+    if (groups > 0) sum_rows(first_rows);
+    if (groups > 1)
+        visit_groups(s, sm.table, count, [&](const int at, const int first, const unsigned bits, const int begin, const int n) {
+            if (at == 0) return;
+            mine = Rows<C>::gather(sm.rows, sm.table.order[warp], begin, n, first, group);
+            __syncwarp();
+            for (int pair = 0; 2 * pair < min(n - begin, kGroup); ++pair) {
+                const float2 w = Rows<C>::weights(group + pair * kPairQuads, bits, minus_x, minus_y);
+                weight[2 * pair * kWeightPitch + lane] = w.x, weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
+            }
+            __syncwarp();
+            sum_rows(min(n - begin, kGroup));
+            __syncwarp();
+        });
+}
+
+template <int C, bool kDropout>
+void launch_sums(const SumArgs &a, cudaStream_t s) {
+    constexpr int kBytes = (int)sizeof(SumSmem<C, kDropout>);
+    // past 48 KB (11 and 12 channels) the kernel has to be told; the setting is the device's, so every call makes it
+    if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    launch(sums_kernel<C, kDropout>, dim3(a.tiles_x * ceil_div(a.img_h, kTile)), dim3(kTilePixels), kBytes, s, a);
 }
 
 // Zero times a conic that is not finite is nothing here: a Gaussian without a weight has no gradient
