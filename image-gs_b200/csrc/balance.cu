@@ -8,32 +8,34 @@
 //
 // The importance is summed over a patch in float, in one order, and from there as 64-bit fixed point with as many fractional bits as the
 // image leaves room for (a Gaussian's importance is at most the pixel count), so no result depends on the order of the atomics.
+#include <algorithm>
+
 #include "topk_sums.cuh"
 
 namespace {
 
-using igs::kGroup;
 using igs::kTile;
 using igs::kTilePixels;
 using igs::kTopK;
 using igs::kWeightPitch;
 
 constexpr int kThreads = 256;
-using SumsOf = igs::SumLayout<1, false>;
+constexpr int kRoutedSlots = 32;
 
 struct BalanceWorkspace {
-    unsigned long long filled;  // A
-    unsigned long long routed;  // T
+    unsigned long long filled;                // A
     unsigned int ticket;
-    float scale;                // backward: v_loss N / (A T)
-    unsigned int pad[10];
-    // forward: then uint64 fixed [n] and double partials [blocks of the finish kernel]; backward: then float sums [n, SumsOf::kValues]
+    unsigned int pad;
+    unsigned long long routed[kRoutedSlots];  // T, over this many words, so that no one word takes every patch's atomic
+    // then uint64 fixed [n], float4 rows [n, 2], double partials [blocks of the finish kernel]
 };
 
 int finish_blocks(int n) { return n > 0 ? igs::ceil_div(n, kThreads) : 1; }
-size_t forward_bytes(int n) { return sizeof(BalanceWorkspace) + sizeof(unsigned long long) * (size_t)n + sizeof(double) * (size_t)finish_blocks(n); }
-size_t backward_bytes(int n) { return sizeof(BalanceWorkspace) + sizeof(float) * SumsOf::kValues * (size_t)n; }
-size_t workspace_bytes_of(int n) { return forward_bytes(n) > backward_bytes(n) ? forward_bytes(n) : backward_bytes(n); }
+size_t forward_bytes(int n) {
+    return sizeof(BalanceWorkspace) + (sizeof(unsigned long long) + sizeof(float4) * igs::Rows<0>::kQuads) * (size_t)n + 8 +
+           sizeof(double) * (size_t)finish_blocks(n);
+}
+size_t workspace_bytes_of(int n) { return std::max(forward_bytes(n), igs::sum_bytes<1, false>(n)); }
 
 // Fractional bits of the importance sums: pixels * 2^bits stays below 2^63
 int fraction_bits(int64_t pixels) {
@@ -41,27 +43,6 @@ int fraction_bits(int64_t pixels) {
     while (((int64_t)1 << log2) < pixels) ++log2;
     return 62 - log2;
 }
-
-__global__ void __launch_bounds__(kThreads) balance_zero_kernel(const int n, int *__restrict__ counts, unsigned long long *__restrict__ fixed,
-                                                                BalanceWorkspace *__restrict__ ws) {
-    igs::wait_for_predecessor();
-    const int g = blockIdx.x * kThreads + threadIdx.x;
-    if (g == 0) ws->filled = 0, ws->routed = 0, ws->ticket = 0;
-    if (g < n) counts[g] = 0, fixed[g] = 0;
-}
-
-struct BalanceSmem {
-    igs::TileTable table;
-    union {
-        alignas(16) int lists[igs::kListWords];
-        struct {
-            alignas(16) float weight[igs::kWarps][kGroup * kWeightPitch];
-            alignas(16) float inv[igs::kWarps][32];
-        };
-    };
-    float4 rows[igs::kMaxRows * igs::Rows<0>::kRowQuads];
-    float4 group[igs::kWarps][igs::Rows<0>::kGroupQuads];
-};
 
 struct BalanceArgs {
     int tiles_x, img_h, img_w, n;
@@ -71,116 +52,84 @@ struct BalanceArgs {
     float scale;  // 2^fraction bits
     int *counts;
     unsigned long long *fixed;
+    float4 *rows;
     BalanceWorkspace *ws;
 };
 
-// One pixel's slots one by one, from global memory (topk_sums.cuh says when)
-__device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
-    const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
-    const int *list = a.pixel_topk + (size_t)p * kTopK;
-    float total = (float)igs::kNormEps;
-    for (int pass = 0; pass < 2; ++pass) {
-        const float inv = 1.f / total;
-        for (int k = 0; k < kTopK; ++k) {
-            const int id = list[k];
-            if ((unsigned)id >= (unsigned)a.n) continue;
-            const float w = igs::slot_weight(igs::stage_geometry(a.xys, a.conics, id), px, py);
-            if (pass == 0) {
-                total += w;
-            } else {
-                atomicAdd(&a.counts[id], 1);
-                atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(w * inv * a.scale));
-            }
-        }
-    }
+// The rows of all Gaussians (topk_lists.cuh), and what the patches add to zeroed
+__global__ void __launch_bounds__(kThreads) balance_rows_kernel(const __grid_constant__ BalanceArgs a) {
+    igs::wait_for_predecessor();
+    const int id = blockIdx.x * kThreads + threadIdx.x;
+    if (id == 0) a.ws->filled = 0, a.ws->ticket = 0;
+    if (id < kRoutedSlots) a.ws->routed[id] = 0;
+    if (id >= a.n) return;
+    a.counts[id] = 0, a.fixed[id] = 0;
+    igs::Rows<0>::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), {0.f});
 }
 
-__global__ void __launch_bounds__(kTilePixels, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
+// A warp is a patch, a lane first a pixel and then half a row, as in topk_sums.cuh
+__global__ void __launch_bounds__(kTilePixels, 4) balance_kernel(const __grid_constant__ BalanceArgs a) {
     using Rows = igs::Rows<0>;
-    __shared__ __align__(16) BalanceSmem sm;
+    __shared__ struct {
+        union {
+            int keys[(kTopK + 1) * 32];
+            alignas(16) float weight[igs::kRows * kWeightPitch];
+        };
+        float4 pairs[Rows::kGroupQuads];
+        alignas(16) float inv[32];
+    } smem[igs::kWarps];
+    auto &sm = smem[threadIdx.x >> 5];
+    const int lane = threadIdx.x & 31;
     igs::wait_for_predecessor();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int i0 = (blockIdx.x / a.tiles_x) * kTile, j0 = (blockIdx.x % a.tiles_x) * kTile;
-    const int i = i0 + igs::patch_y(), j = j0 + igs::patch_x();
-    const bool inside = i < a.img_h && j < a.img_w;
-    const int p = inside ? i * a.img_w + j : 0;
-    igs::load_lists(sm.lists, sm.table, a.pixel_topk, i0, j0, a.img_h, a.img_w);
-    const unsigned keep = inside && (a.mask == nullptr || a.mask[p] != 0) ? ~0u : 0u;
-    igs::seed_table(sm.table, sm.lists, i0, j0, a.img_h, a.img_w, a.n);
-    igs::PixelSlots s;
-    igs::place_slots(s, sm.table, sm.lists, a.n, keep);
-    const int routed = __syncthreads_count(s.filled > 0);
-    if (threadIdx.x == 0 && routed > 0) atomicAdd(&a.ws->routed, (unsigned long long)routed);
-    const int count = sm.table.count;
-    if (count > igs::kMaxRows) {
-        if (keep) count_slots(a, p);
-        return;
-    }
-    igs::rank_rows(sm.table, count, [&](const int row, const int id) {
-        const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
-        sm.rows[2 * row] = make_float4(g.x, g.y, g.a, g.b), sm.rows[2 * row + 1] = make_float4(g.c, 0.f, 0.f, 0.f);
-    });
-    __syncthreads();
-    if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count))) {
-        if (keep) count_slots(a, p);
-        return;
-    }
-    // a lane is a pixel: the first group's weights and the sum over all (topk_sums.cuh). The sign of a weight says whether the slot is
-    // there: -0 for an absent one (which adds nothing either), so that counts come from the same words as the sums.
-    float *const weight = sm.weight[warp];
-    float4 *const group = sm.group[warp];
-    const float2 minus_x = make_float2(-(float)j, -(float)j), minus_y = make_float2(-(float)i, -(float)i);
-    const int half = lane >> 4, r = lane & (kGroup - 1);
+    const igs::Patch patch = igs::patch_of(a.tiles_x, a.img_h, a.img_w);
+    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
+    const unsigned keep = patch.inside && (a.mask == nullptr || a.mask[patch.p] != 0) ? ~0u : 0u;
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j), minus_y = make_float2(-(float)patch.i, -(float)patch.i);
+    const int half = lane >> 4;
     float2 total = make_float2(0.f, 0.f);
-    int my_row = 0, my_rows = 0;
-    auto weigh = [&](const int first, const unsigned bits, const int begin, const int n, const bool keep_weights) {
-        const int row = Rows::gather(sm.rows, sm.table.order[warp], begin, n, first, group).row;
-        if (keep_weights) my_row = row, my_rows = min(n - begin, kGroup);
+    bool have_total = false;
+    for (int g = 0;;) {
+        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        Rows::gather(a.rows, rows, sm.pairs);
         __syncwarp();
-        for (int pair = 0; 2 * pair < min(n - begin, kGroup); ++pair) {
-            const float4 *q = group + pair * Rows::kPairQuads;
-            const float2 w = Rows::weights(q, bits, minus_x, minus_y);
-            total = igs::add2(total, w);
-            if (keep_weights) {
-                weight[2 * pair * kWeightPitch + lane] = (bits & __float_as_uint(q[2].z)) != 0 ? w.x : -0.f;
-                weight[(2 * pair + 1) * kWeightPitch + lane] = (bits & __float_as_uint(q[2].w)) != 0 ? w.y : -0.f;
+        unsigned held = rows.bits;
+        for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
+            const float2 w = Rows::weights(sm.pairs + pair * Rows::kPairQuads, held, minus_x, minus_y);
+            sm.weight[2 * pair * kWeightPitch + lane] = w.x, sm.weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
+            if (!have_total) total = igs::add2(total, w);
+        }
+        if (!have_total) {
+            if (rows.more) {
+                ++g;
+                continue;
+            }
+            have_total = true;
+            sm.inv[lane] = 1.f / (total.x + total.y + (float)igs::kNormEps);
+            const unsigned routed = __popc(__ballot_sync(0xffffffffu, rows.filled));
+            if (lane == 0 && routed > 0) atomicAdd(&a.ws->routed[blockIdx.x % kRoutedSlots], (unsigned long long)routed);
+            if (g > 0) {
+                g = 0;
+                continue;
             }
         }
         __syncwarp();
-    };
-    // a lane is half a row: its gates' sum and its holders
-    auto sum_rows = [&]() {
-        float sum = 0.f;
-        int absent = 0;
+        for (int first = 0; first < rows.n; first += 16) {
+            const int r = first + (lane & 15);
+            float sum = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float4 w = *reinterpret_cast<const float4 *>(&weight[r * kWeightPitch + half * 16 + q * 4]);
-            const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[warp][half * 16 + q * 4]);
-            sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
-            absent += (int)((__float_as_uint(w.x) >> 31) + (__float_as_uint(w.y) >> 31) + (__float_as_uint(w.z) >> 31) +
-                            (__float_as_uint(w.w) >> 31));
+            for (int q = 0; q < 4; ++q) {
+                const float4 w = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + half * 16 + q * 4]);
+                const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[half * 16 + q * 4]);
+                sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int id = __shfl_sync(0xffffffffu, rows.id, r);
+            if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        absent += __shfl_xor_sync(0xffffffffu, absent, 16);
-        if (r < my_rows) {
-            const int id = sm.table.sorted[my_row];
-            if (half == 0) atomicAdd(&a.counts[id], 32 - absent);
-            else atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
-        }
-        __syncwarp();
-    };
-    const int groups = igs::visit_groups(
-        s, sm.table, count,
-        [&](const int at, const int first, const unsigned bits, const int begin, const int n) { weigh(first, bits, begin, n, at == 0); });
-    sm.inv[warp][lane] = 1.f / (total.x + total.y + (float)igs::kNormEps);
-    __syncwarp();
-    if (groups > 0) sum_rows();
-    if (groups > 1)
-        igs::visit_groups(s, sm.table, count, [&](const int at, const int first, const unsigned bits, const int begin, const int n) {
-            if (at == 0) return;
-            weigh(first, bits, begin, n, true);
-            sum_rows();
-        });
+        if (lane < rows.n) atomicAdd(&a.counts[rows.id], __popc(rows.holders));
+        if (!rows.more) return;
+        ++g;
+    }
 }
 
 // importance from the fixed-point sums, and the loss: each block's sums of counts and of counts * importance (in double, in thread order),
@@ -227,21 +176,12 @@ __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const int n, c
     for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) sum += __ldcg(&partials[b]);
     const double all = block_sum(sum);
     if (threadIdx.x == 0) {
-        const unsigned long long a = __ldcg(&ws->filled), t = __ldcg(&ws->routed);
+        const unsigned long long a = __ldcg(&ws->filled);
+        unsigned long long t = 0;
+        for (int q = 0; q < kRoutedSlots; ++q) t += __ldcg(&ws->routed[q]);
         *loss = a ? (float)((double)n / ((double)a * (double)t) * all) : 0.f;
         totals[0] = (long long)a, totals[1] = (long long)t;
     }
-}
-
-// The backward pass's sums zeroed, and the loss's share of alpha: v_loss N / (A T)
-__global__ void __launch_bounds__(kThreads) balance_scale_kernel(const int n, const long long *__restrict__ totals,
-                                                                 const float *__restrict__ v_loss, float4 *__restrict__ sums,
-                                                                 BalanceWorkspace *__restrict__ ws) {
-    igs::wait_for_predecessor();
-    const int e = blockIdx.x * kThreads + threadIdx.x;
-    if (e == 0)
-        ws->scale = v_loss != nullptr && totals[0] > 0 ? (float)((double)n / ((double)totals[0] * (double)totals[1])) * *v_loss : 0.f;
-    if (e < n * (SumsOf::kValues / 4)) sums[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 }  // namespace
@@ -265,16 +205,15 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     char *base = static_cast<char *>(workspace);
     BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(base);
     unsigned long long *fixed = reinterpret_cast<unsigned long long *>(base + sizeof(BalanceWorkspace));
-    double *partials = reinterpret_cast<double *>(fixed + num_points);
+    float4 *rows = reinterpret_cast<float4 *>(fixed + (num_points + 1) / 2 * 2);
+    double *partials = reinterpret_cast<double *>(rows + (size_t)igs::Rows<0>::kQuads * num_points);
     const int bits = fraction_bits(pixels);
     const int blocks = finish_blocks(num_points);
-    igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, counts, fixed, ws);
-    if (pixels > 0 && num_points > 0) {
-        const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
-        const BalanceArgs a = {tiles_x, img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
-                               (float)((int64_t)1 << bits), counts, fixed, ws};
-        igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
-    }
+    const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
+    const BalanceArgs a = {tiles_x, img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
+                           (float)((int64_t)1 << bits), counts, fixed, rows, ws};
+    igs::launch(balance_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
+    if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
     igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
                 (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,
                 reinterpret_cast<long long *>(totals));
@@ -295,19 +234,11 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
     IGS_REQUIRE(pixels == 0 || pixel_topk, "igs_topk_balance_bwd: null pointer");
     IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_balance_bwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
-    BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(workspace);
-    float *sums = reinterpret_cast<float *>(ws + 1);
-    igs::launch(balance_scale_kernel, dim3(igs::ceil_div(num_points * (SumsOf::kValues / 4), kThreads)), dim3(kThreads), 0, s, num_points,
-                reinterpret_cast<const long long *>(totals), v_loss, reinterpret_cast<float4 *>(sums), ws);
-    if (pixels > 0) {
-        igs::SumArgs a = {};
-        a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.n = num_points;
-        a.xys = xys, a.conics = conics, a.pixel_topk = pixel_topk, a.mask = pixel_mask;
-        a.counts = counts, a.scale = &ws->scale, a.v_importance = v_importance, a.sums = sums;
-        igs::launch_sums<1, false>(a, s);
-    }
-    igs::launch(igs::finish_sums_kernel<SumsOf::kValues>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, num_points, 0, conics,
-                (const float *)sums, accumulate != 0, v_xy, v_conic, (float *)nullptr);
+    igs::SumArgs a = {};
+    a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.n = num_points;
+    a.xys = xys, a.conics = conics, a.pixel_topk = pixel_topk, a.mask = pixel_mask;
+    a.counts = counts, a.totals = reinterpret_cast<const long long *>(totals), a.v_loss = v_loss, a.v_importance = v_importance;
+    igs::launch_sums<1, false>(a, workspace, accumulate != 0, v_xy, v_conic, nullptr, s);
     return igs::check_launch("igs_topk_balance_bwd");
 }
 

@@ -14,14 +14,6 @@ using igs::kTile;
 using igs::kTilePixels;
 using igs::kTopK;
 
-template <int C>
-struct DropoutSmem {
-    igs::TileTable table;
-    alignas(16) int lists[igs::kListWords];
-    float4 rows[igs::kMaxRows * igs::Rows<C>::kRowQuads];
-    float4 group[igs::kWarps][igs::Rows<C>::kGroupQuads];
-};
-
 struct DropoutArgs {
     int tiles_x, img_h, img_w, channels, n;
     const float *xys, *conics, *colors;
@@ -30,6 +22,7 @@ struct DropoutArgs {
     const long long *rng;
     float *out_img;
     long long *rng_used;
+    float4 *rows;
 };
 
 // One pixel's slots one by one, from global memory
@@ -43,7 +36,7 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p, cons
         for (int k = 0; k < kTopK; ++k) {
             const int id = list[k];
             if ((unsigned)id >= (unsigned)a.n || !(keep >> k & 1)) continue;
-            const float w = igs::slot_weight(igs::stage_geometry(a.xys, a.conics, id), px, py);
+            const float w = igs::slot_weight(igs::row_geometry(a.xys, a.conics, id), px, py);
             if (w == 0.f) continue;
             total += w;
             pix = fmaf(w, __ldg(&a.colors[(size_t)id * a.channels + c]), pix);
@@ -52,88 +45,65 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p, cons
     }
 }
 
+// The rows of all Gaussians (topk_lists.cuh)
 template <int C>
-__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 6 : 4)
-    dropout_kernel(const __grid_constant__ DropoutArgs a) {
-    using Rows = igs::Rows<C>;
-    constexpr int kRowQuads = Rows::kRowQuads;
-    __shared__ __align__(16) DropoutSmem<C> sm;
+__global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant__ DropoutArgs a) {
     igs::wait_for_predecessor();
-    const int i0 = (blockIdx.x / a.tiles_x) * kTile, j0 = (blockIdx.x % a.tiles_x) * kTile;
-    const int i = i0 + igs::patch_y(), j = j0 + igs::patch_x();
-    const bool inside = i < a.img_h && j < a.img_w;
-    const int p = inside ? i * a.img_w + j : 0;
-    igs::load_lists(sm.lists, sm.table, a.pixel_topk, i0, j0, a.img_h, a.img_w);
+    const int id = blockIdx.x * 256 + threadIdx.x;
+    if (id >= a.n) return;
+    float f[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) f[c] = c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
+    igs::Rows<C>::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), f);
+}
+
+// A warp is a patch, a lane a pixel
+template <int C>
+__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 4) dropout_kernel(const __grid_constant__ DropoutArgs a) {
+    using Rows = igs::Rows<C>;
+    __shared__ struct {
+        int keys[(kTopK + 1) * 32];
+        float4 pairs[Rows::kGroupQuads];
+    } smem[igs::kWarps];
+    auto &sm = smem[threadIdx.x >> 5];
+    igs::wait_for_predecessor();
     const long long seed = a.rng[0], offset = a.rng[1];
     if (blockIdx.x == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
-    const unsigned keep = inside ? igs::keep_bits((uint32_t)p, (uint64_t)seed, (uint64_t)offset, a.threshold) : 0u;
-    igs::seed_table(sm.table, sm.lists, i0, j0, a.img_h, a.img_w, a.n);
-    igs::PixelSlots s;
-    igs::place_slots(s, sm.table, sm.lists, a.n, keep);
-    __syncthreads();
-    const int count = sm.table.count;
-    if (count > igs::kMaxRows) {
-        if (inside) blend_slots(a, p, keep);
-        return;
-    }
-    igs::rank_rows(sm.table, count, [&](const int row, const int id) {
-        const igs::RowGeometry g = igs::stage_geometry(a.xys, a.conics, id);
-        float q[4 * kRowQuads];
-        q[0] = g.x, q[1] = g.y, q[2] = g.a, q[3] = g.b, q[4] = g.c;
-        bool finite = true;
-#pragma unroll
-        for (int c = 0; c < 4 * kRowQuads - 5; ++c) {
-            q[5 + c] = c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
-            finite = finite && isfinite(q[5 + c]);
-        }
-        if (!finite) sm.table.per_slot = 1;  // zero times it would reach pixels that do not name it
-#pragma unroll
-        for (int e = 0; e < kRowQuads; ++e) sm.rows[row * kRowQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
-    });
-    __syncthreads();
-    if (!__all_sync(0xffffffffu, igs::find_rows(s, sm.table, count) && sm.table.per_slot == 0)) {
-        if (inside) blend_slots(a, p, keep);
-        return;
-    }
-    const int warp = threadIdx.x >> 5;
-    float4 *const group = sm.group[warp];
-    const float2 minus_x = make_float2(-(float)j, -(float)j), minus_y = make_float2(-(float)i, -(float)i);
+    const igs::Patch patch = igs::patch_of(a.tiles_x, a.img_h, a.img_w);
+    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
+    const unsigned keep = patch.inside ? igs::keep_bits((uint32_t)patch.p, (uint64_t)seed, (uint64_t)offset, a.threshold) : 0u;
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j), minus_y = make_float2(-(float)patch.i, -(float)patch.i);
     float2 total = make_float2(0.f, 0.f), pix[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) pix[c] = make_float2(0.f, 0.f);
-    igs::visit_groups(s, sm.table, count, [&](const int, const int first, const unsigned bits, const int begin, const int n) {
-        Rows::gather(sm.rows, sm.table.order[warp], begin, n, first, group);
-        __syncwarp();
-        for (int pair = 0; 2 * pair < min(n - begin, igs::kGroup); ++pair) {
-            const float4 *q = group + pair * Rows::kPairQuads;
-            const float2 w = Rows::weights(q, bits, minus_x, minus_y);
-            total = igs::add2(total, w);
-#pragma unroll
-            for (int c = 0; c < C; c += 2) {
-                const float4 f = q[3 + c / 2];
-                pix[c] = igs::fma2(w, make_float2(f.x, f.y), pix[c]);
-                if (c + 1 < C) pix[c + 1 < C ? c + 1 : c] = igs::fma2(w, make_float2(f.z, f.w), pix[c + 1 < C ? c + 1 : c]);
-            }
+    for (int g = 0;; ++g) {
+        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        if (!Rows::gather(a.rows, rows, sm.pairs)) {  // zero times a colour that is not finite would reach pixels that do not name it
+            if (patch.inside) blend_slots(a, patch.p, keep);
+            return;
         }
         __syncwarp();
-    });
-    if (!inside) return;
+        unsigned held = rows.bits;
+        for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
+            const float4 *q = sm.pairs + pair * Rows::kPairQuads;
+            const float2 w = Rows::weights(q, held, minus_x, minus_y);
+            total = igs::add2(total, w);
+#pragma unroll
+            for (int c = 0; c < C; ++c) pix[c] = igs::fma2(w, Rows::value(q, c), pix[c]);
+        }
+        if (!rows.more) break;
+    }
+    if (!patch.inside) return;
     const float inv = 1.f / (total.x + total.y + (float)igs::kNormEps);
     const size_t plane = (size_t)a.img_h * a.img_w;
 #pragma unroll
     for (int c = 0; c < C; ++c)
-        if (c < a.channels) a.out_img[c * plane + p] = (pix[c].x + pix[c].y) * inv;
+        if (c < a.channels) a.out_img[c * plane + patch.p] = (pix[c].x + pix[c].y) * inv;
 }
 
 __global__ void rng_used_kernel(const long long *rng, long long *rng_used) {
     igs::wait_for_predecessor();
     rng_used[0] = rng[0], rng_used[1] = rng[1];
-}
-
-__global__ void __launch_bounds__(256) zero_kernel(const int64_t quads, float4 *__restrict__ sums) {
-    igs::wait_for_predecessor();
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e < quads) sums[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 // The kernels' widths: channels are padded with zeros to one less than a multiple of four, so that a staged row (geometry 5, colours) and a
@@ -147,9 +117,9 @@ void with_width(int channels, F f) {
 }
 
 size_t workspace_bytes_of(int num_points, int channels) {
-    size_t values = 0;
-    with_width(channels, [&](auto width) { values = igs::SumLayout<decltype(width)::value, true>::kValues; });
-    return sizeof(float) * values * (size_t)num_points + 16;
+    size_t bytes = 0;
+    with_width(channels, [&](auto width) { bytes = igs::sum_bytes<decltype(width)::value, true>(num_points); });
+    return bytes + 16;  // never nothing
 }
 
 }  // namespace
@@ -182,9 +152,11 @@ int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_po
     } else {
         const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
         const DropoutArgs a = {tiles_x, img_height, img_width, channels, num_points, xys, conics, colors, pixel_topk,
-                               (uint32_t)rint(p * 16777216.0), rng, out_img, used};
+                               (uint32_t)rint(p * 16777216.0), rng, out_img, used, static_cast<float4 *>(workspace)};
         with_width(channels, [&](auto width) {
-            igs::launch(dropout_kernel<decltype(width)::value>, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
+            constexpr int kWidth = decltype(width)::value;
+            if (num_points > 0) igs::launch(dropout_rows_kernel<kWidth>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, a);
+            igs::launch(dropout_kernel<kWidth>, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
         });
     }
     return igs::check_launch("igs_topk_dropout_fwd");
@@ -202,24 +174,15 @@ int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_po
     IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_dropout_bwd: workspace must be 16-byte aligned");
     IGS_REQUIRE(v_xy && v_conic && v_colors, "igs_topk_dropout_bwd: null output");
     const int pixels = img_height * img_width;
-    IGS_REQUIRE(conics && (pixels == 0 || (xys && colors && v_output && pixel_topk && rng_used)), "igs_topk_dropout_bwd: null pointer");
+    IGS_REQUIRE(xys && conics && colors && (pixels == 0 || (v_output && pixel_topk && rng_used)), "igs_topk_dropout_bwd: null pointer");
     IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_dropout_bwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
-    float *sums = static_cast<float *>(workspace);
+    igs::SumArgs a = {};
+    a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
+    a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
+    a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0);
     with_width(channels, [&](auto width) {
-        constexpr int kWidth = decltype(width)::value;
-        constexpr int kValues = igs::SumLayout<kWidth, true>::kValues;
-        const int64_t quads = (int64_t)num_points * (kValues / 4);
-        igs::launch(zero_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, quads, reinterpret_cast<float4 *>(sums));
-        if (pixels > 0) {
-            igs::SumArgs a = {};
-            a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
-            a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
-            a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0), a.sums = sums;
-            igs::launch_sums<kWidth, true>(a, s);
-        }
-        igs::launch(igs::finish_sums_kernel<kValues>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, num_points, channels, conics,
-                    (const float *)sums, false, v_xy, v_conic, v_colors);
+        igs::launch_sums<decltype(width)::value, true>(a, workspace, false, v_xy, v_conic, v_colors, s);
     });
     return igs::check_launch("igs_topk_dropout_bwd");
 }

@@ -40,171 +40,103 @@ __device__ __forceinline__ unsigned keep_bits(uint32_t pixel, uint64_t seed, uin
     return keep;
 }
 
-// ---- a tile's Gaussians as rows --------------------------------------------------------------------------------------------------------
+// ---- a patch's Gaussians as rows -------------------------------------------------------------------------------------------------------
 //
-// One CTA of 256 threads takes a 16x16 tile, a warp an 8x4 patch of it, a lane one pixel. Neighbouring pixels name nearly the same
-// Gaussians (at a trained image's 100 pixels per Gaussian the 2560 slots of a tile name 18 to 23, a patch 13 to 14), so the tile's distinct
-// IDs become rows: a hash table in shared memory collects them, they are ranked by ID (so that every sum over rows has one order, whatever
-// thread came first), and each row's parameters are staged once. A pixel's slots are then bits of a row mask. A warp takes the rows that
-// any of its pixels holds in groups of 16, copied side by side in pairs: it reads them as broadcasts, two rows per packed (f32x2)
-// instruction, with no gather per slot, and sums per Gaussian become sums along a row.
-constexpr int kTableBits = 10;
-constexpr int kTableSize = 1 << kTableBits;
-constexpr int kMaxRows = 128;   // more distinct IDs in a tile than this (or an ID twice in a pixel) take the per-slot path
-constexpr int kGroup = 16;      // rows of a warp's group
-constexpr int kNoRow = 0xFF;
-constexpr int kListPitch = 176;  // words per row of 16 pixels: 160, padded so that the 8x4 patches' 8-byte reads do not conflict
-constexpr int kListWords = kTile * kListPitch;
-constexpr int kWarps = kTilePixels / 32;
+// A warp takes an 8x4 patch of pixels, a lane one pixel. Neighbouring pixels name nearly the same Gaussians (at a trained image's 100 pixels
+// per Gaussian the 320 slots of a patch name 13 to 14), so the patch's distinct IDs become rows, in the order of their IDs: every lane
+// sorts its ten slots (a 29-comparator network) into shared memory, and the warp then takes the smallest unconsumed ID of all its pixels
+// again and again. An ID twice in one list becomes two rows. What a row means to a pixel is a bit of the lane's mask; the rows' parameters
+// are read once, by a lane each, and laid side by side in pairs, so that the warp reads them as broadcasts, two rows per packed (f32x2)
+// instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need no other warp, so nothing waits at a
+// barrier. (The tile's IDs collected by its eight warps in one hash table took twice the instructions, and half the time at barriers.)
+constexpr int kRows = 32;      // rows of a group: a patch with more goes over them group by group
+constexpr int kWarps = 8;      // patches of a CTA: a 16x16 tile
+constexpr int kNoId = 0x7fffffff;
 
-struct alignas(16) TileTable {
-    int ids[kTableSize];        // -1: free
-    uint8_t row[kTableSize];
-    int found[kMaxRows];        // distinct IDs in the order found, and their places in the table
-    uint16_t place[kMaxRows];
-    int sorted[kMaxRows];       // the same by rank
-    uint8_t order[kWarps][32];  // a warp's rows of the current 32, closed up
-    int count;
-    int per_slot;               // set when a row's values ask for the per-slot path
+// The patch of a warp and the pixel of a lane
+struct Patch {
+    int x0, y0, i, j, p;
+    bool inside;
+};
+__device__ __forceinline__ Patch patch_of(const int tiles_x, const int img_h, const int img_w) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Patch a;
+    a.x0 = (blockIdx.x % tiles_x) * kTile + (warp & 1) * 8, a.y0 = (blockIdx.x / tiles_x) * kTile + (warp >> 1) * 4;
+    a.i = a.y0 + (lane >> 3), a.j = a.x0 + (lane & 7);
+    a.inside = a.i < img_h && a.j < img_w;
+    a.p = a.inside ? a.i * img_w + a.j : 0;
+    return a;
+}
+
+// A sorting network for ten keys (29 comparators, depth 8)
+__device__ __forceinline__ void sort_slots(int (&key)[kTopK]) {
+    constexpr int kPairs[29][2] = {{4, 9}, {3, 8}, {2, 7}, {1, 6}, {0, 5}, {1, 4}, {6, 9}, {0, 3}, {5, 8}, {0, 2}, {3, 6}, {7, 9},
+                                   {0, 1}, {2, 4}, {5, 7}, {8, 9}, {1, 2}, {4, 6}, {7, 8}, {3, 5}, {2, 5}, {6, 8}, {1, 3}, {4, 7},
+                                   {2, 3}, {6, 7}, {3, 4}, {5, 6}, {4, 5}};
+#pragma unroll
+    for (int c = 0; c < 29; ++c) {
+        const int i = kPairs[c][0], j = kPairs[c][1];
+        const int lo = min(key[i], key[j]), hi = max(key[i], key[j]);
+        key[i] = lo, key[j] = hi;
+    }
+}
+
+// Rows [32 g, 32 g + 32) of the patch
+struct PatchRows {
+    int n;             // how many there are, at most 32
+    bool more;         // whether others follow
+    unsigned bits;     // the rows that this lane's pixel holds
+    int id;            // lane l < n: the ID of row l,
+    unsigned holders;  // and the pixels that hold it
+    bool filled;       // whether this lane's pixel has a slot at all
 };
 
-// Copies the tile's lists into shared memory (asynchronously; finish_lists waits) and clears the table
-__device__ __forceinline__ void load_lists(int *s_lists, TileTable &t, const int *pixel_topk, const int i0, const int j0, const int img_h,
-                                           const int img_w) {
-    const int pairs = min(kTile, img_w - j0) * (kTopK / 2);  // 8-byte words of a row that lie in the image
-    const int rows = min(kTile, img_h - i0);
+// keys: shared memory of this warp, [kTopK + 1][32]; keep: a bit for each slot that may be filled. All lanes together.
+__device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const int p, const int n_points, const unsigned keep, const int g,
+                                               int *keys) {
+    const int lane = threadIdx.x & 31;
+    int key[kTopK];
 #pragma unroll
-    for (int m = 0; m < kTopK / 2; ++m) {
-        const int idx = m * kTilePixels + threadIdx.x;
-        const int r = idx / (kTile * kTopK / 2), q = idx % (kTile * kTopK / 2);
-        if (r < rows && q < pairs) {
-            const int *src = pixel_topk + ((size_t)(i0 + r) * img_w + j0) * kTopK + 2 * q;
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_lists + r * kListPitch + 2 * q);
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    for (int k = 0; k < kTopK; ++k) key[k] = kNoId;
+    if (keep != 0) {
+        const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)p * kTopK);
+#pragma unroll
+        for (int k = 0; k < kTopK; k += 2) {
+            const int2 v = __ldg(&list[k / 2]);
+            if ((unsigned)v.x < (unsigned)n_points && (keep >> k & 1)) key[k] = v.x;
+            if ((unsigned)v.y < (unsigned)n_points && (keep >> (k + 1) & 1)) key[k + 1] = v.y;
         }
     }
+    sort_slots(key);
+    __syncwarp();
 #pragma unroll
-    for (int e = 0; e < kTableSize / 4 / kTilePixels; ++e)
-        reinterpret_cast<int4 *>(t.ids)[e * kTilePixels + threadIdx.x] = make_int4(-1, -1, -1, -1);
-    if (threadIdx.x == 0) t.count = 0, t.per_slot = 0;
-}
-
-__device__ __forceinline__ int hash_of(const int id) { return (int)((unsigned)id * 2654435761u >> (32 - kTableBits)); }
-
-// The place of id in the table, found or made. A new ID takes the next entry of found[]; count past kMaxRows means that the tile does not
-// fit (the place returned is then meaningless, and so it is when the table is full).
-static __device__ __noinline__ int table_place(TileTable &t, const int id) {
-    int h = hash_of(id);
-    for (int probe = 0; probe < kTableSize; ++probe, h = (h + 1) & (kTableSize - 1)) {
-        int v = *(volatile int *)&t.ids[h];
-        if (v == id) break;
-        if (v == -1) {
-            if (*(volatile int *)&t.count > kMaxRows) break;
-            v = atomicCAS(&t.ids[h], -1, id);
-            if (v == id) break;
-            if (v == -1) {
-                const int r = atomicAdd(&t.count, 1);
-                if (r < kMaxRows) t.found[r] = id, t.place[r] = (uint16_t)h;
-                break;
-            }
+    for (int k = 1; k < kTopK; ++k) keys[k * 32 + lane] = key[k];
+    keys[kTopK * 32 + lane] = kNoId;
+    __syncwarp();
+    PatchRows rows = {0, false, 0, 0, 0, key[0] != kNoId};
+    int head = key[0];
+    const int *next = keys + 32 + lane;
+    int row = -kRows * g;
+    while (true) {
+        const int id = __reduce_min_sync(0xffffffffu, head);
+        if (id == kNoId) break;
+        if (row == kRows) {
+            rows.more = true;
+            break;
         }
-    }
-    return h;
-}
-
-// Waits for the lists, then enters the IDs of 25 pixels spread over the tile, a thread each: nearly all of the tile's, so that afterwards
-// most pixels only look theirs up. (Slots that the caller leaves out may enter too: a row that nobody holds is never visited.)
-__device__ __forceinline__ void seed_table(TileTable &t, const int *s_lists, const int i0, const int j0, const int img_h, const int img_w,
-                                           const int n) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    const int pixel = threadIdx.x / kTopK, slot = threadIdx.x % kTopK;
-    const int y = (pixel / 5) * 15 / 4, x = (pixel % 5) * 15 / 4;  // 0, 3, 7, 11, 15
-    if (pixel < 25 && i0 + y < img_h && j0 + x < img_w) {
-        const int id = s_lists[y * kListPitch + x * kTopK + slot];
-        if ((unsigned)id < (unsigned)n) table_place(t, id);
-    }
-    __syncthreads();
-}
-
-// The pixel of a thread: warp w covers the 8x4 patch (w % 2, w / 2) of the tile, lane l its pixel (l % 8, l / 8)
-__device__ __forceinline__ int patch_x() { return (threadIdx.x >> 5 & 1) * 8 + (threadIdx.x & 7); }
-__device__ __forceinline__ int patch_y() { return (threadIdx.x >> 6) * 4 + (threadIdx.x >> 3 & 3); }
-
-// A pixel's slots: first their places in the table (-1: empty), then their rows
-struct PixelSlots {
-    int place[kTopK];
-    unsigned rows[3];  // a byte per slot, kNoRow for an empty one
-    unsigned bits;     // rows 0-31 as a mask
-    int filled;
-};
-
-// From the pixel's list in shared memory; keep holds a bit per slot that may be filled
-__device__ __forceinline__ void place_slots(PixelSlots &s, TileTable &t, const int *s_lists, const int n, const unsigned keep) {
-    const int *list = s_lists + patch_y() * kListPitch + patch_x() * kTopK;
-    s.filled = 0;
-    unsigned missing = 0;
-#pragma unroll
-    for (int k = 0; k < kTopK; k += 2) {
-        const int2 v = *reinterpret_cast<const int2 *>(list + k);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int id = b ? v.y : v.x;
-            const bool filled = (unsigned)id < (unsigned)n && (keep >> (k + b) & 1) != 0;
-            const int h = hash_of(id);
-            s.place[k + b] = filled ? h : -1;
-            s.filled += filled;
-            if (filled && t.ids[h] != id) missing |= 1u << (k + b);
+        const bool held = head == id;
+        const unsigned holders = __ballot_sync(0xffffffffu, held);
+        if (held) {
+            head = *next;
+            next += 32;
+            if (row >= 0) rows.bits |= 1u << row;
         }
+        if (row == lane) rows.id = id, rows.holders = holders;
+        ++row;
     }
-    if (__any_sync(0xffffffffu, missing != 0)) {
-#pragma unroll
-        for (int k = 0; k < kTopK; ++k)
-            if (missing >> k & 1) s.place[k] = table_place(t, list[k]);
-    }
-}
-
-// Ranks the IDs found (count <= kMaxRows), writes each place's row and calls stage(row, id); the caller synchronizes before and after
-template <typename Stage>
-__device__ __forceinline__ void rank_rows(TileTable &t, const int count, Stage stage) {
-    for (int r = threadIdx.x; r < count; r += kTilePixels) {
-        const int id = t.found[r];
-        int rank = 0;
-        for (int o = 0; o < count; ++o) rank += t.found[o] < id ? 1 : 0;
-        t.row[t.place[r]] = (uint8_t)rank;
-        t.sorted[rank] = id;
-        stage(rank, id);
-    }
-}
-
-// 1 << shift, 0 for a shift of 32 or more (the clamp of PTX's shl; in C++ it would be undefined)
-__device__ __forceinline__ unsigned bit_or_nothing(const unsigned shift) {
-    unsigned r;
-    asm("shl.b32 %0, 1, %1;" : "=r"(r) : "r"(shift));
-    return r;
-}
-
-// The rows of the slots with first <= row < first + 32 as a mask
-__device__ __forceinline__ unsigned row_bits(const PixelSlots &s, const int first) {
-    unsigned bits = 0;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) bits |= bit_or_nothing((s.rows[k / 4] >> 8 * (k % 4) & 255) - first);
-    return bits;
-}
-
-// After rank_rows: the slots' rows. False where an ID stands twice in the list, which the mask cannot say.
-__device__ __forceinline__ bool find_rows(PixelSlots &s, const TileTable &t, const int count) {
-    s.rows[0] = s.rows[1] = s.rows[2] = 0;
-    s.bits = 0;
-#pragma unroll
-    for (int k = 0; k < kTopK; ++k) {
-        const unsigned row = s.place[k] >= 0 ? t.row[s.place[k]] : kNoRow;
-        s.rows[k / 4] |= row << 8 * (k % 4);
-        s.bits |= bit_or_nothing(row);
-    }
-    int distinct = __popc(s.bits);
-    for (int first = 32; first < count; first += 32) distinct += __popc(row_bits(s, first));
-    return distinct == s.filled;
+    rows.n = max(row, 0);
+    __syncwarp();
+    return rows;
 }
 
 // exp2(x) (ex2.approx: 2 ulp; results below 2^-126 are 0, far below what eps leaves of a gate)
@@ -214,21 +146,23 @@ __device__ __forceinline__ float exp2_approx(const float x) {
     return r;
 }
 
-// The staged geometry of a row: centre, and the conic times -log2(e) (its outer terms halved too), so that the weight is exp2 of
+// A Gaussian's geometry as the kernels use it: centre, and the conic times -log2(e) (its outer terms halved too), so that the weight is
+// exp2 of
 //   (a' dx) dx + (c' dy + b' dx) dy
 // where that is not positive, and 0 where it is positive or NaN. A Gaussian whose parameters are not all finite has no finite sigma
-// anywhere; it is staged at the origin with a NaN conic, so that its weights are 0 and its offsets finite.
+// anywhere; it stands at the origin with a NaN conic, so that its weights are 0 and its offsets finite.
 struct RowGeometry {
     float x, y, a, b, c;
+    bool finite;
 };
 
-__device__ __forceinline__ RowGeometry stage_geometry(const float *xys, const float *conics, const int id) {
+__device__ __forceinline__ RowGeometry row_geometry(const float *xys, const float *conics, const int id) {
     constexpr float kLog2e = 1.4426950408889634f;
-    RowGeometry g = {__ldg(&xys[2 * (size_t)id]), __ldg(&xys[2 * (size_t)id + 1]), __ldg(&conics[3 * (size_t)id]),
-                     __ldg(&conics[3 * (size_t)id + 1]), __ldg(&conics[3 * (size_t)id + 2])};
-    if (isfinite(g.x) && isfinite(g.y) && isfinite(g.a) && isfinite(g.b) && isfinite(g.c))
-        return {g.x, g.y, -0.5f * kLog2e * g.a, -kLog2e * g.b, -0.5f * kLog2e * g.c};
-    return {0.f, 0.f, __int_as_float(0x7fc00000), 0.f, 0.f};
+    const float x = __ldg(&xys[2 * (size_t)id]), y = __ldg(&xys[2 * (size_t)id + 1]);
+    const float a = __ldg(&conics[3 * (size_t)id]), b = __ldg(&conics[3 * (size_t)id + 1]), c = __ldg(&conics[3 * (size_t)id + 2]);
+    if (isfinite(x) && isfinite(y) && isfinite(a) && isfinite(b) && isfinite(c))
+        return {x, y, -0.5f * kLog2e * a, -kLog2e * b, -0.5f * kLog2e * c, true};
+    return {0.f, 0.f, __int_as_float(0x7fc00000), 0.f, 0.f, false};
 }
 
 // The weight of one slot, from global memory: the per-slot path
@@ -261,73 +195,60 @@ __device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
     return r;
 }
 
-// A staged row in the CTA's table: x, y, a', b', c', f[C], padded to whole float4s. A warp's group of 16 rows, in 8 pairs of
-// (x x y y) (a' a' b' b') (c' c' m m) (f0 f0 f1 f1) ..., m the row's bit in the mask (0 for a row that pads the last pair).
+// A Gaussian's row with C values f: x, y, a', b', c', f, padded to whole 16-byte words. The rows of all Gaussians are laid out so once per
+// call: a lane then reads its row with a few wide loads (each of which costs a pass of the L1 per lane) instead of 5 + C narrow ones. In
+// shared memory, in pairs: (x x y y) (a' a' b' b') (c' c' f0 f0) (f1 f1 f2 f2) ...
 template <int C>
 struct Rows {
-    static constexpr int kRowQuads = (5 + C + 3) / 4;
-    static constexpr int kPairQuads = 3 + (C + 1) / 2;
-    static constexpr int kGroupQuads = kGroup / 2 * kPairQuads;
+    static constexpr int kQuads = (5 + C + 3) / 4;
+    static constexpr int kPairQuads = (5 + C + 1) / 2;
+    static constexpr int kGroupQuads = kRows / 2 * kPairQuads;
 
-    // This lane's row (lane % 16) of the group from the table, into registers and, by the first 16 lanes, into the warp's group
-    struct Mine {
-        int row;
-        float x, y, f[C > 0 ? C : 1];
-    };
-    static __device__ __forceinline__ Mine gather(const float4 *table, const uint8_t *order, const int begin, const int n, const int first,
-                                                  float4 *group) {
-        const int lane = threadIdx.x & 31, r = lane & (kGroup - 1);
-        const int bit = begin + r < n ? order[begin + r] : 0;
-        Mine mine;
-        mine.row = first + bit;
-        float q[4 * kRowQuads];
+    static __device__ __forceinline__ void store(float4 *all, const int id, const RowGeometry &g, const float (&f)[C > 0 ? C : 1]) {
+        float q[4 * kQuads] = {g.x, g.y, g.a, g.b, g.c};
 #pragma unroll
-        for (int e = 0; e < kRowQuads; ++e) {
-            const float4 v = table[mine.row * kRowQuads + e];
-            q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
-        }
-        mine.x = q[0], mine.y = q[1];
+        for (int c = 0; c < C; ++c) q[5 + c] = g.finite ? f[c] : 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) mine.f[c] = q[5 + c];
-        if (lane < kGroup) {
-            float *pair = reinterpret_cast<float *>(group + (r >> 1) * kPairQuads) + (r & 1);
-#pragma unroll
-            for (int e = 0; e < 5; ++e) pair[2 * e] = q[e];
-            reinterpret_cast<unsigned *>(pair)[10] = begin + r < n ? 1u << bit : 0u;
-#pragma unroll
-            for (int c = 0; c < C; ++c) pair[12 + 2 * c] = q[5 + c];
-        }
-        return mine;
+        for (int e = 0; e < kQuads; ++e) all[(size_t)id * kQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
     }
 
-    // The weights of a pair's two rows at a pixel; minus holds (-px, -px), (-py, -py)
-    static __device__ __forceinline__ float2 weights(const float4 *pair, const unsigned bits, const float2 minus_x, const float2 minus_y) {
-        const float4 xy = pair[0], ab = pair[1], cm = pair[2];
+    // The group's rows into the warp's pairs. False, on all lanes, where a value f is not finite.
+    static __device__ __forceinline__ bool gather(const float4 *all, const PatchRows &rows, float4 *pairs) {
+        const int lane = threadIdx.x & 31;
+        float q[4 * kQuads];
+#pragma unroll
+        for (int e = 0; e < 4 * kQuads; ++e) q[e] = 0.f;
+        if (lane < rows.n) {
+#pragma unroll
+            for (int e = 0; e < kQuads; ++e) {
+                const float4 v = __ldg(&all[(size_t)rows.id * kQuads + e]);
+                q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
+            }
+        }
+        float size = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) size += fabsf(q[5 + c]);
+        if (lane <= rows.n) {  // one more, of zeros, to pad the last pair
+            float *pair = reinterpret_cast<float *>(pairs + (lane >> 1) * kPairQuads) + (lane & 1);
+#pragma unroll
+            for (int e = 0; e < 5 + C; ++e) pair[2 * e] = q[e];
+        }
+        return C == 0 || __all_sync(0xffffffffu, isfinite(size));
+    }
+
+    // The weights of a pair's two rows at a pixel, bits 0 and 1 of held saying whether the pixel holds them
+    static __device__ __forceinline__ float2 weights(const float4 *pair, const unsigned held, const float2 minus_x, const float2 minus_y) {
+        const float4 xy = pair[0], ab = pair[1];
+        const float2 c = *reinterpret_cast<const float2 *>(&pair[2]);
         const float2 dx = add2(make_float2(xy.x, xy.y), minus_x), dy = add2(make_float2(xy.z, xy.w), minus_y);
-        const float2 slope = fma2(make_float2(cm.x, cm.y), dy, mul2(make_float2(ab.z, ab.w), dx));
+        const float2 slope = fma2(c, dy, mul2(make_float2(ab.z, ab.w), dx));
         const float2 e = fma2(slope, dy, mul2(mul2(make_float2(ab.x, ab.y), dx), dx));
-        const bool held0 = (bits & __float_as_uint(cm.z)) != 0, held1 = (bits & __float_as_uint(cm.w)) != 0;
-        return make_float2(held0 && e.x <= 0.f ? exp2_approx(e.x) : 0.f, held1 && e.y <= 0.f ? exp2_approx(e.y) : 0.f);
+        return make_float2((held & 1) && e.x <= 0.f ? exp2_approx(e.x) : 0.f, (held & 2) && e.y <= 0.f ? exp2_approx(e.y) : 0.f);
+    }
+    static __device__ __forceinline__ float2 value(const float4 *pair, const int c) {
+        return reinterpret_cast<const float2 *>(pair)[5 + c];
     }
 };
-
-// Calls visit(first row of the 32, this lane's mask of them, begin, rows of the 32 that the warp holds) for each group of 16 rows that the
-// warp's pixels hold, in order, with t.order closed up for it; all lanes of the warp together. Returns the number of groups.
-template <typename Visit>
-__device__ __forceinline__ int visit_groups(const PixelSlots &s, TileTable &t, const int count, Visit visit) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int groups = 0;
-    for (int first = 0; first < count; first += 32) {
-        const unsigned bits = first == 0 ? s.bits : row_bits(s, first);
-        const unsigned any = __reduce_or_sync(0xffffffffu, bits);
-        const int n = __popc(any);
-        __syncwarp();
-        if (any >> lane & 1) t.order[warp][__popc(any & ((1u << lane) - 1))] = (uint8_t)lane;
-        __syncwarp();
-        for (int begin = 0; begin < n; begin += kGroup, ++groups) visit(groups, first, bits, begin, n);
-    }
-    return groups;
-}
 
 // Host checks of the sizes, shared by the entry points: slots and Gaussians' sums indexed with 32 bits, coordinates exact in float
 constexpr const char *kListsLimit = "at most 2^31 / 10 pixels, 2^24 pixels a side and 2^26 Gaussians";

@@ -5,13 +5,12 @@
 // a Gaussian's sums are sum t dx, t dy, t dx^2, t dx dy, t dy^2 and (dropout) w v'_c, from which finish_kernel forms
 //   v_xy = (a Sx + b Sy, b Sx + c Sy),  v_conic = (Sxx / 2, Sxy, Syy / 2),  v_f = S_c.
 //
-// A warp (an 8x4 patch, topk_lists.cuh) goes over its rows twice. First a lane is a pixel: weights into shared memory (16 rows of 32), D
+// A warp (an 8x4 patch, topk_lists.cuh) goes over its rows twice. First a lane is a pixel: weights into shared memory (32 rows of 32), D
 // and the scores' sum in registers. Then a lane is half a row: lane l sums row l % 16 over 16 pixels (two patch rows of 8), reading the
 // weights four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per patch row, so t
 // and t dx are summed along it first. One shuffle joins the halves, and the sums go to global memory with one 16-byte vector atomic per
-// four values. A patch of more than 16 rows computes the later groups' weights again. A tile with an ID twice in a list, too many IDs or
-// values that are not finite takes the per-slot path instead: zero times a value that is not finite would reach Gaussians that the pixel
-// does not name.
+// four values. A patch of more than 32 rows goes over its groups once for D and the scores and once more for the sums. Where a value is not
+// finite, the patch takes the per-slot path instead: zero times it would reach Gaussians that the pixel does not name.
 #pragma once
 
 #include "topk_lists.cuh"
@@ -25,12 +24,14 @@ struct SumArgs {
     const float *xys, *conics;
     const int *pixel_topk;
     const uint8_t *mask;         // balance: pixels that count (NULL: all)
-    const int *counts;           // balance: alpha = *scale * counts + v_importance
-    const float *scale, *v_importance;
+    const int *counts;           // balance: alpha = v_loss N / (A T) counts + v_importance
+    const long long *totals;
+    const float *v_loss, *v_importance;
     const float *colors, *v_output;  // dropout
     const long long *rng;
     uint32_t threshold;
-    float *sums;                 // [N, SumLayout::kValues], zero before
+    float4 *rows;                // all Gaussians' rows
+    float *sums;                 // [N, SumLayout::kValues]
 };
 
 // C: the values per row and pixel (1 for balance; 3, 7, 11 or 12 channels, the unused ones zero)
@@ -41,23 +42,23 @@ struct SumLayout {
 
 template <int C, bool kDropout>
 struct SumSmem {
-    TileTable table;
-    union {
-        alignas(16) int lists[kListWords];
-        struct {
-            alignas(16) float weight[kWarps][kGroup * kWeightPitch];
-            alignas(16) float pixel[kWarps][C + 1][32];  // v'_c, m'
+    struct Warp {
+        union {
+            int keys[(kTopK + 1) * 32];
+            alignas(16) float weight[kRows * kWeightPitch];
         };
-    };
-    float4 rows[kMaxRows * Rows<C>::kRowQuads];
-    float4 group[kWarps][Rows<C>::kGroupQuads];
+        float4 pairs[Rows<C>::kGroupQuads];
+        alignas(16) float pixel[C + 1][32];  // v'_c, m'
+    } warp[kWarps];
 };
 
 // Value c of a Gaussian's score
 template <bool kDropout>
 __device__ __forceinline__ float row_value(const SumArgs &a, const int id, const int c) {
     if constexpr (kDropout) return c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
-    return *a.scale * (float)__ldg(&a.counts[id]) + (a.v_importance != nullptr ? __ldg(&a.v_importance[id]) : 0.f);
+    const double slots = (double)a.totals[0], pixels = (double)a.totals[1];
+    const float scale = a.v_loss != nullptr && slots > 0.0 ? (float)((double)a.n / (slots * pixels)) * *a.v_loss : 0.f;
+    return scale * (float)a.counts[id] + (a.v_importance != nullptr ? a.v_importance[id] : 0.f);
 }
 template <bool kDropout>
 __device__ __forceinline__ float pixel_value(const SumArgs &a, const int p, const int c) {
@@ -77,7 +78,7 @@ __device__ __noinline__ void add_slots(const SumArgs &a, const int p, const unsi
         for (int k = 0; k < kTopK; ++k) {
             const int id = list[k];
             if ((unsigned)id >= (unsigned)a.n || !(keep >> k & 1)) continue;
-            const RowGeometry g = stage_geometry(a.xys, a.conics, id);
+            const RowGeometry g = row_geometry(a.xys, a.conics, id);
             const float w = slot_weight(g, px, py);
             if (w == 0.f) continue;
             float score = 0.f;
@@ -96,173 +97,151 @@ __device__ __noinline__ void add_slots(const SumArgs &a, const int p, const unsi
     }
 }
 
+// The rows of all Gaussians, and their sums zeroed
 template <int C, bool kDropout>
-__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
-    constexpr int kValues = SumLayout<C, kDropout>::kValues;
-    constexpr int kRowQuads = Rows<C>::kRowQuads, kPairQuads = Rows<C>::kPairQuads;
-    extern __shared__ __align__(16) char smem_bytes[];
-    SumSmem<C, kDropout> &sm = *reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes);
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int i0 = (blockIdx.x / a.tiles_x) * kTile, j0 = (blockIdx.x % a.tiles_x) * kTile;
-    const int i = i0 + patch_y(), j = j0 + patch_x();
-    const bool inside = i < a.img_h && j < a.img_w;
-    const int p = inside ? i * a.img_w + j : 0;
-    load_lists(sm.lists, sm.table, a.pixel_topk, i0, j0, a.img_h, a.img_w);
-    unsigned keep = 0;
-    if (inside) {
-        if constexpr (kDropout) keep = keep_bits((uint32_t)p, (uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold);
-        else keep = a.mask == nullptr || a.mask[p] != 0 ? ~0u : 0u;
-    }
-    float v[C];
+    const int id = blockIdx.x * 256 + threadIdx.x;
+    if (id >= a.n) return;
+    float f[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = inside ? pixel_value<kDropout>(a, p, c) : 0.f;
-    seed_table(sm.table, sm.lists, i0, j0, a.img_h, a.img_w, a.n);
-    PixelSlots s;
-    place_slots(s, sm.table, sm.lists, a.n, keep);
-    __syncthreads();
-    const int count = sm.table.count;
-    if (count > kMaxRows) {
-        add_slots<C, kDropout>(a, p, keep);
-        return;
-    }
-    rank_rows(sm.table, count, [&](const int row, const int id) {
-        const RowGeometry g = stage_geometry(a.xys, a.conics, id);
-        float q[4 * kRowQuads];
-        q[0] = g.x, q[1] = g.y, q[2] = g.a, q[3] = g.b, q[4] = g.c;
-        bool finite = true;
+    for (int c = 0; c < C; ++c) f[c] = row_value<kDropout>(a, id, c);
+    Rows<C>::store(a.rows, id, row_geometry(a.xys, a.conics, id), f);
+    constexpr int kValues = SumLayout<C, kDropout>::kValues;
 #pragma unroll
-        for (int c = 0; c < 4 * kRowQuads - 5; ++c) {
-            q[5 + c] = c < C ? row_value<kDropout>(a, id, c) : 0.f;
-            finite = finite && isfinite(q[5 + c]);
-        }
-        if (!finite) sm.table.per_slot = 1;
-#pragma unroll
-        for (int e = 0; e < kRowQuads; ++e) sm.rows[row * kRowQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
-    });
-    __syncthreads();
-    bool regular = find_rows(s, sm.table, count) && sm.table.per_slot == 0;
-    float *const weight = sm.weight[warp];
-    float4 *const group = sm.group[warp];
-    const float2 minus_x = make_float2(-(float)j, -(float)j), minus_y = make_float2(-(float)i, -(float)i);
-    // a lane is a pixel: the first group's weights, the sums over all groups
-    typename Rows<C>::Mine mine;
-    float2 total2 = make_float2(0.f, 0.f), scores2 = make_float2(0.f, 0.f);
-    int first_rows = 0;
-    const int groups = visit_groups(s, sm.table, count, [&](const int at, const int first, const unsigned bits, const int begin, const int n) {
-        const typename Rows<C>::Mine got = Rows<C>::gather(sm.rows, sm.table.order[warp], begin, n, first, group);
-        if (at == 0) mine = got, first_rows = min(n - begin, kGroup);
-        __syncwarp();
-        for (int pair = 0; 2 * pair < min(n - begin, kGroup); ++pair) {
-            const float4 *q = group + pair * kPairQuads;
-            const float2 w = Rows<C>::weights(q, bits, minus_x, minus_y);
-            float2 score = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < C; c += 2) {
-                const float4 f = q[3 + c / 2];
-                score = fma2(make_float2(f.x, f.y), make_float2(v[c], v[c]), score);
-                if (c + 1 < C) score = fma2(make_float2(f.z, f.w), make_float2(v[c + 1 < C ? c + 1 : c], v[c + 1 < C ? c + 1 : c]), score);
-            }
-            total2 = add2(total2, w);
-            scores2 = fma2(w, score, scores2);
-            if (at == 0) weight[2 * pair * kWeightPitch + lane] = w.x, weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
-        }
-        __syncwarp();
-    });
-    const float total = total2.x + total2.y, scores = scores2.x + scores2.y;
-    const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
-    const float inv = 1.f / (total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
-    float size = fabsf(m);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        v[c] = some ? v[c] * inv : 0.f;
-        size += fabsf(v[c]);
-        sm.pixel[warp][c][lane] = v[c];
-    }
-    sm.pixel[warp][C][lane] = m;
-    regular = regular && isfinite(size);
-    if (!__all_sync(0xffffffffu, regular)) {
-        if (inside) add_slots<C, kDropout>(a, p, keep);
-        return;
-    }
-    // a lane is half a row
-    const int half = lane >> 4, r = lane & (kGroup - 1);
-    const float x0 = (float)(j0 + (warp & 1) * 8), y0 = (float)(i0 + (warp >> 1) * 4 + half * 2);
-    auto sum_rows = [&](const int rows) {
-        float2 dx[4], f[C], color[C];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dx[e] = make_float2(mine.x - (x0 + (float)(2 * e)), mine.x - (x0 + (float)(2 * e + 1)));
-#pragma unroll
-        for (int c = 0; c < C; ++c) f[c] = make_float2(-mine.f[c], -mine.f[c]), color[c] = make_float2(0.f, 0.f);
-        float2 xx = make_float2(0.f, 0.f);
-        float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int quad = 0; quad < 2; ++quad) {
-                const int at = half * 16 + y * 8 + quad * 4;
-                const float4 w4 = *reinterpret_cast<const float4 *>(&weight[r * kWeightPitch + at]);
-                const float4 m4 = *reinterpret_cast<const float4 *>(&sm.pixel[warp][C][at]);
-                float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
-                const float2 w0 = make_float2(w4.x, w4.y), w1 = make_float2(w4.z, w4.w);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float4 v4 = *reinterpret_cast<const float4 *>(&sm.pixel[warp][c][at]);
-                    const float2 v0 = make_float2(v4.x, v4.y), v1 = make_float2(v4.z, v4.w);
-                    d0 = fma2(f[c], v0, d0), d1 = fma2(f[c], v1, d1);
-                    if constexpr (kDropout) color[c] = fma2(w1, v1, fma2(w0, v0, color[c]));
-                }
-                const float2 t0 = mul2(w0, d0), t1 = mul2(w1, d1);
-                const float2 u0 = mul2(t0, dx[2 * quad]), u1 = mul2(t1, dx[2 * quad + 1]);
-                ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
-                xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
-            }
-            const float dy = mine.y - (y0 + (float)y);
-            const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
-            sx += ur, sy += ty;
-            sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
-        }
-        float sum[kValues];
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
-        sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
-        if constexpr (kDropout) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
-        }
-#pragma unroll
-        for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
-        if (r < rows) {
-            float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)sm.table.sorted[mine.row] * kValues);
-#pragma unroll
-            for (int e = 0; e < kValues / 4; ++e)
-                if ((e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
-        }
-    };
-    __syncwarp();
-    if (groups > 0) sum_rows(first_rows);
-    if (groups > 1)
-        visit_groups(s, sm.table, count, [&](const int at, const int first, const unsigned bits, const int begin, const int n) {
-            if (at == 0) return;
-            mine = Rows<C>::gather(sm.rows, sm.table.order[warp], begin, n, first, group);
-            __syncwarp();
-            for (int pair = 0; 2 * pair < min(n - begin, kGroup); ++pair) {
-                const float2 w = Rows<C>::weights(group + pair * kPairQuads, bits, minus_x, minus_y);
-                weight[2 * pair * kWeightPitch + lane] = w.x, weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
-            }
-            __syncwarp();
-            sum_rows(min(n - begin, kGroup));
-            __syncwarp();
-        });
+    for (int e = 0; e < kValues / 4; ++e) reinterpret_cast<float4 *>(a.sums)[(size_t)id * (kValues / 4) + e] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 template <int C, bool kDropout>
-void launch_sums(const SumArgs &a, cudaStream_t s) {
-    constexpr int kBytes = (int)sizeof(SumSmem<C, kDropout>);
-    // past 48 KB (11 and 12 channels) the kernel has to be told; the setting is the device's, so every call makes it
-    if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-    launch(sums_kernel<C, kDropout>, dim3(a.tiles_x * ceil_div(a.img_h, kTile)), dim3(kTilePixels), kBytes, s, a);
+__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
+    constexpr int kValues = SumLayout<C, kDropout>::kValues;
+    constexpr int kPairQuads = Rows<C>::kPairQuads;
+    extern __shared__ __align__(16) char smem_bytes[];
+    const int lane = threadIdx.x & 31;
+    typename SumSmem<C, kDropout>::Warp &sm = reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes)->warp[threadIdx.x >> 5];
+    wait_for_predecessor();
+    const Patch patch = patch_of(a.tiles_x, a.img_h, a.img_w);
+    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
+    unsigned keep = 0;
+    if (patch.inside) {
+        if constexpr (kDropout) keep = keep_bits((uint32_t)patch.p, (uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold);
+        else keep = a.mask == nullptr || a.mask[patch.p] != 0 ? ~0u : 0u;
+    }
+    float v[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c] = patch.inside ? pixel_value<kDropout>(a, patch.p, c) : 0.f;
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j), minus_y = make_float2(-(float)patch.i, -(float)patch.i);
+    const int half = lane >> 4;
+    const float x0 = (float)patch.x0, y0 = (float)(patch.y0 + half * 2);
+    float2 total2 = make_float2(0.f, 0.f), scores2 = make_float2(0.f, 0.f);
+    bool regular = true, have_totals = false;
+    for (int g = 0;;) {
+        const PatchRows rows = find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        regular = Rows<C>::gather(a.rows, rows, sm.pairs) && regular;
+        __syncwarp();
+        // a lane is a pixel: the group's weights, and the sums over all groups
+        unsigned held = rows.bits;
+        for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
+            const float4 *q = sm.pairs + pair * kPairQuads;
+            const float2 w = Rows<C>::weights(q, held, minus_x, minus_y);
+            sm.weight[2 * pair * kWeightPitch + lane] = w.x, sm.weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
+            if (!have_totals) {
+                float2 score = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(q, c), make_float2(v[c], v[c]), score);
+                total2 = add2(total2, w);
+                scores2 = fma2(w, score, scores2);
+            }
+        }
+        if (!have_totals) {
+            if (rows.more) {
+                ++g;
+                continue;
+            }
+            const float total = total2.x + total2.y, scores = scores2.x + scores2.y;
+            const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
+            const float inv = 1.f / (total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
+            float size = fabsf(m);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float vc = some ? v[c] * inv : 0.f;
+                size += fabsf(vc);
+                sm.pixel[c][lane] = vc;
+            }
+            sm.pixel[C][lane] = m;
+            if (!__all_sync(0xffffffffu, regular && isfinite(size))) {
+                if (patch.inside) add_slots<C, kDropout>(a, patch.p, keep);
+                return;
+            }
+            have_totals = true;
+            if (g > 0) {
+                g = 0;
+                continue;
+            }
+        }
+        __syncwarp();
+        // a lane is half a row
+        for (int first = 0; first < rows.n; first += 16) {
+            const int r = first + (lane & 15);
+            const float2 *mine = reinterpret_cast<const float2 *>(sm.pairs + (r >> 1) * kPairQuads);
+            const bool odd = (r & 1) != 0;
+            auto field = [&](const int e) { return odd ? mine[e].y : mine[e].x; };
+            const float x = field(0), y = field(1);
+            float2 dx[4], f[C], color[C];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dx[e] = make_float2(x - (x0 + (float)(2 * e)), x - (x0 + (float)(2 * e + 1)));
+#pragma unroll
+            for (int c = 0; c < C; ++c) f[c].x = -field(5 + c), f[c].y = f[c].x, color[c] = make_float2(0.f, 0.f);
+            float2 xx = make_float2(0.f, 0.f);
+            float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
+#pragma unroll
+            for (int line = 0; line < 2; ++line) {
+                float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int quad = 0; quad < 2; ++quad) {
+                    const int at = half * 16 + line * 8 + quad * 4;
+                    const float4 w4 = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + at]);
+                    const float4 m4 = *reinterpret_cast<const float4 *>(&sm.pixel[C][at]);
+                    float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
+                    const float2 w0 = make_float2(w4.x, w4.y), w1 = make_float2(w4.z, w4.w);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const float4 v4 = *reinterpret_cast<const float4 *>(&sm.pixel[c][at]);
+                        const float2 v0 = make_float2(v4.x, v4.y), v1 = make_float2(v4.z, v4.w);
+                        d0 = fma2(f[c], v0, d0), d1 = fma2(f[c], v1, d1);
+                        if constexpr (kDropout) color[c] = fma2(w1, v1, fma2(w0, v0, color[c]));
+                    }
+                    const float2 t0 = mul2(w0, d0), t1 = mul2(w1, d1);
+                    const float2 u0 = mul2(t0, dx[2 * quad]), u1 = mul2(t1, dx[2 * quad + 1]);
+                    ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
+                    xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
+                }
+                const float dy = y - (y0 + (float)line);
+                const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
+                sx += ur, sy += ty;
+                sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
+            }
+            float sum[kValues];
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
+            sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
+            if constexpr (kDropout) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
+            }
+#pragma unroll
+            for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
+            const int id = __shfl_sync(0xffffffffu, rows.id, r);
+            if (r < rows.n) {
+                float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)id * kValues);
+#pragma unroll
+                for (int e = 0; e < kValues / 4; ++e)
+                    if ((e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
+            }
+        }
+        if (!rows.more) return;
+        ++g;
+    }
 }
 
 // Zero times a conic that is not finite is nothing here: a Gaussian without a weight has no gradient
@@ -291,6 +270,28 @@ __global__ void __launch_bounds__(256) finish_sums_kernel(const int n, const int
 #pragma unroll
     for (int e = 5; e < kValues; ++e)
         if (e - 5 < channels) v_colors[(size_t)g * channels + e - 5] = s[e];
+}
+
+// The backward pass: rows, sums, gradients. a.rows and a.sums are in the workspace, of sum_bytes.
+template <int C, bool kDropout>
+constexpr size_t sum_bytes(const int n) {
+    return (sizeof(float4) * Rows<C>::kQuads + sizeof(float) * SumLayout<C, kDropout>::kValues) * (size_t)n;
+}
+
+template <int C, bool kDropout>
+void launch_sums(SumArgs a, void *workspace, const bool accumulate, float *v_xy, float *v_conic, float *v_colors, cudaStream_t s) {
+    constexpr int kValues = SumLayout<C, kDropout>::kValues;
+    constexpr int kBytes = (int)sizeof(SumSmem<C, kDropout>);
+    a.rows = static_cast<float4 *>(workspace);
+    a.sums = reinterpret_cast<float *>(a.rows + (size_t)Rows<C>::kQuads * a.n);
+    launch(rows_kernel<C, kDropout>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a);
+    if (a.img_h > 0 && a.img_w > 0) {
+        // past 48 KB the kernel has to be told; the setting belongs to the device, so every call makes it
+        if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        launch(sums_kernel<C, kDropout>, dim3(a.tiles_x * ceil_div(a.img_h, kTile)), dim3(kTilePixels), kBytes, s, a);
+    }
+    launch(finish_sums_kernel<kValues>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a.n, a.channels, a.conics, (const float *)a.sums,
+           accumulate, v_xy, v_conic, v_colors);
 }
 
 }  // namespace igs
