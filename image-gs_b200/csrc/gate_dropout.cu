@@ -14,6 +14,8 @@ using igs::kTile;
 using igs::kTilePixels;
 using igs::kTopK;
 
+constexpr int kLayOutTiles = 1024;
+
 struct DropoutArgs {
     int tiles_x, img_h, img_w, channels, n;
     const float *xys, *conics, *colors;
@@ -22,7 +24,7 @@ struct DropoutArgs {
     const long long *rng;
     float *out_img;
     long long *rng_used;
-    float4 *rows;
+    float4 *rows;  // of all Gaussians, or NULL
 };
 
 // One pixel's slots one by one, from global memory
@@ -78,7 +80,14 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 4) dropout_kernel(co
     for (int c = 0; c < C; ++c) pix[c] = make_float2(0.f, 0.f);
     for (int g = 0;; ++g) {
         const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
-        if (!Rows::gather(a.rows, rows, sm.pairs)) {  // zero times a colour that is not finite would reach pixels that do not name it
+        const bool finite = Rows::gather(a.rows, rows, sm.pairs, [&](const int id, float(&q)[4 * Rows::kQuads]) {
+            const igs::RowGeometry r = igs::row_geometry(a.xys, a.conics, id);
+            q[0] = r.x, q[1] = r.y, q[2] = r.a, q[3] = r.b, q[4] = r.c;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (c < a.channels && r.finite) q[5 + c] = __ldg(&a.colors[(size_t)id * a.channels + c]);
+        });
+        if (!finite) {  // zero times a colour that is not finite would reach pixels that do not name it
             if (patch.inside) blend_slots(a, patch.p, keep);
             return;
         }
@@ -151,11 +160,13 @@ int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_po
         igs::launch(rng_used_kernel, dim3(1), dim3(1), 0, s, rng, used);
     } else {
         const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
+        // laying the rows out is a launch of its own, which a small image does not repay
+        const bool lay_out = num_points > 0 && tiles_x * tiles_y > kLayOutTiles;
         const DropoutArgs a = {tiles_x, img_height, img_width, channels, num_points, xys, conics, colors, pixel_topk,
-                               (uint32_t)rint(p * 16777216.0), rng, out_img, used, static_cast<float4 *>(workspace)};
+                               (uint32_t)rint(p * 16777216.0), rng, out_img, used, lay_out ? static_cast<float4 *>(workspace) : nullptr};
         with_width(channels, [&](auto width) {
             constexpr int kWidth = decltype(width)::value;
-            if (num_points > 0) igs::launch(dropout_rows_kernel<kWidth>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, a);
+            if (lay_out) igs::launch(dropout_rows_kernel<kWidth>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, a);
             igs::launch(dropout_kernel<kWidth>, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
         });
     }

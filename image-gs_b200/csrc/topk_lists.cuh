@@ -212,17 +212,23 @@ struct Rows {
         for (int e = 0; e < kQuads; ++e) all[(size_t)id * kQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
     }
 
-    // The group's rows into the warp's pairs. False, on all lanes, where a value f is not finite.
-    static __device__ __forceinline__ bool gather(const float4 *all, const PatchRows &rows, float4 *pairs) {
+    // The group's rows into the warp's pairs: from the rows of all Gaussians or, where all is NULL, from read(id, q). False, on all lanes,
+    // where a value f is not finite.
+    template <typename Read>
+    static __device__ __forceinline__ bool gather(const float4 *all, const PatchRows &rows, float4 *pairs, Read read) {
         const int lane = threadIdx.x & 31;
         float q[4 * kQuads];
 #pragma unroll
         for (int e = 0; e < 4 * kQuads; ++e) q[e] = 0.f;
         if (lane < rows.n) {
+            if (all != nullptr) {
 #pragma unroll
-            for (int e = 0; e < kQuads; ++e) {
-                const float4 v = __ldg(&all[(size_t)rows.id * kQuads + e]);
-                q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
+                for (int e = 0; e < kQuads; ++e) {
+                    const float4 v = __ldg(&all[(size_t)rows.id * kQuads + e]);
+                    q[4 * e] = v.x, q[4 * e + 1] = v.y, q[4 * e + 2] = v.z, q[4 * e + 3] = v.w;
+                }
+            } else {
+                read(rows.id, q);
             }
         }
         float size = 0.f;
@@ -234,6 +240,10 @@ struct Rows {
             for (int e = 0; e < 5 + C; ++e) pair[2 * e] = q[e];
         }
         return C == 0 || __all_sync(0xffffffffu, isfinite(size));
+    }
+
+    static __device__ __forceinline__ bool gather(const float4 *all, const PatchRows &rows, float4 *pairs) {
+        return gather(all, rows, pairs, [](int, float (&)[4 * kQuads]) {});
     }
 
     // The weights of a pair's two rows at a pixel, bits 0 and 1 of held saying whether the pixel holds them

@@ -295,6 +295,17 @@ def topk_feature_weights(img_height, img_width, xys, conics, pixel_topk, eps=EPS
 
 # ---- routing lists: balance and gate dropout ------------------------------------------------------------------------------------------
 
+def _run(dev, name, *args):
+    """One entry point on dev's current stream, the arguments (tensors as pointers) before the stream. These operators are used on small
+    images too, where the host's time is the time: the device is only changed where it is not the current one."""
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    if torch.cuda.current_device() == dev.index:
+        _lib_call(name, *args, stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib_call(name, *args, stream_of(dev))
+
+
 def _check_lists(img_height, img_width, xys, conics, pixel_topk, **others):
     """The inputs shared by the operators over pixel_topk: shapes, types, one device. Returns (H, W, N, device)."""
     h, w = int(img_height), int(img_width)
@@ -339,9 +350,8 @@ def topk_balance_forward(img_height, img_width, xys, conics, pixel_topk, pixel_m
     totals = torch.empty(2, device=dev, dtype=torch.int64)
     ws_bytes = _lib.load().igs_topk_balance_workspace(n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        _lib_call("igs_topk_balance_fwd", h, w, n, ptr(xys), ptr(conics), ptr(pixel_topk), ptr(pixel_mask), ptr(loss), ptr(counts),
-                  ptr(importance), ptr(totals), ptr(ws), ws_bytes, stream_of(dev))
+    _run(dev, "igs_topk_balance_fwd", h, w, n, xys, conics, pixel_topk, pixel_mask, loss, counts,
+         importance, totals, ws, ws_bytes)
     return loss, counts, importance, totals
 
 
@@ -368,9 +378,8 @@ def topk_balance_backward(img_height, img_width, xys, conics, pixel_topk, counts
     v_conic = torch.empty(n, 3, device=dev, dtype=torch.float32)
     ws_bytes = _lib.load().igs_topk_balance_workspace(n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        _lib_call("igs_topk_balance_bwd", h, w, n, ptr(xys), ptr(conics), ptr(pixel_topk), ptr(pixel_mask), ptr(counts), ptr(totals),
-                  ptr(grad_loss), ptr(grad_importance), 0, ptr(v_xy), ptr(v_conic), ptr(ws), ws_bytes, stream_of(dev))
+    _run(dev, "igs_topk_balance_bwd", h, w, n, xys, conics, pixel_topk, pixel_mask, counts, totals,
+         grad_loss, grad_importance, 0, v_xy, v_conic, ws, ws_bytes)
     return v_xy, v_conic
 
 
@@ -401,9 +410,8 @@ def topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk,
     rng_used = torch.empty(2, device=dev, dtype=torch.int64)
     ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        _lib_call("igs_topk_dropout_fwd", h, w, channels, n, ptr(xys), ptr(conics), ptr(colors), ptr(pixel_topk), p, ptr(rng_state),
-                  ptr(out_img), ptr(rng_used), ptr(ws), ws_bytes, stream_of(dev))
+    _run(dev, "igs_topk_dropout_fwd", h, w, channels, n, xys, conics, colors, pixel_topk, p, rng_state,
+         out_img, rng_used, ws, ws_bytes)
     return out_img, rng_used
 
 
@@ -414,13 +422,11 @@ def topk_dropout_backward(img_height, img_width, xys, conics, colors, v_output, 
     _check_input(v_output, "v_output", torch.float32)
     if v_output.numel() != channels * h * w:
         raise RuntimeError("v_output must be [C, H, W]")
-    grads = torch.empty(n * (5 + channels), device=dev, dtype=torch.float32)
-    v_xy, v_conic, v_colors = grads[:2 * n].view(n, 2), grads[2 * n:5 * n].view(n, 3), grads[5 * n:].view(n, channels)
+    v_xy, v_conic, v_colors = (torch.empty(n, c, device=dev, dtype=torch.float32) for c in (2, 3, channels))
     ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        _lib_call("igs_topk_dropout_bwd", h, w, channels, n, ptr(xys), ptr(conics), ptr(colors), ptr(v_output), ptr(pixel_topk), p,
-                  ptr(rng_used), ptr(v_xy), ptr(v_conic), ptr(v_colors), ptr(ws), ws_bytes, stream_of(dev))
+    _run(dev, "igs_topk_dropout_bwd", h, w, channels, n, xys, conics, colors, v_output, pixel_topk, p,
+         rng_used, v_xy, v_conic, v_colors, ws, ws_bytes)
     return v_xy, v_conic, v_colors
 
 
