@@ -89,14 +89,14 @@ __global__ void __launch_bounds__(kTilePixels, 4) balance_kernel(const __grid_co
     float2 total = make_float2(0.f, 0.f);
     bool have_total = false;
     for (int g = 0;;) {
-        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        const igs::PatchRows rows = igs::find_rows<false>(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
         Rows::gather(a.rows, rows, sm.pairs);
         __syncwarp();
         unsigned held = rows.bits;
         for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
             const float2 w = Rows::weights(sm.pairs + pair * Rows::kPairQuads, held, minus_x, minus_y);
             sm.weight[2 * pair * kWeightPitch + lane] = w.x, sm.weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
-            if (!have_total) total = igs::add2(total, w);
+            total = igs::add2(total, w);  // (unused the second time)
         }
         if (!have_total) {
             if (rows.more) {

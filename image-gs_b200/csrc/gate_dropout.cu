@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 4) dropout_kernel(co
 #pragma unroll
     for (int c = 0; c < C; ++c) pix[c] = make_float2(0.f, 0.f);
     for (int g = 0;; ++g) {
-        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        const igs::PatchRows rows = igs::find_rows<true>(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
         const bool finite = Rows::gather(a.rows, rows, sm.pairs, [&](const int id, float(&q)[4 * Rows::kQuads]) {
             const igs::RowGeometry r = igs::row_geometry(a.xys, a.conics, id);
             q[0] = r.x, q[1] = r.y, q[2] = r.a, q[3] = r.b, q[4] = r.c;

@@ -51,7 +51,6 @@ __device__ __forceinline__ unsigned keep_bits(uint32_t pixel, uint64_t seed, uin
 // barrier. (The tile's IDs collected by its eight warps in one hash table took twice the instructions, and half the time at barriers.)
 constexpr int kRows = 32;      // rows of a group: a patch with more goes over them group by group
 constexpr int kWarps = 8;      // patches of a CTA: a 16x16 tile
-constexpr int kNoId = 0x7fffffff;
 
 // The patch of a warp and the pixel of a lane
 struct Patch {
@@ -91,50 +90,50 @@ struct PatchRows {
     bool filled;       // whether this lane's pixel has a slot at all
 };
 
-// keys: shared memory of this warp, [kTopK + 1][32]; keep: a bit for each slot that may be filled. All lanes together.
+// keys: shared memory of this warp, [kTopK + 1][32]; keep: a bit for each slot that may be filled (kBits false: all or none of them). All
+// lanes together.
+template <bool kBits>
 __device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const int p, const int n_points, const unsigned keep, const int g,
                                                int *keys) {
     const int lane = threadIdx.x & 31;
+    const int none = n_points;  // the key of an empty slot: behind every ID
     int key[kTopK];
 #pragma unroll
-    for (int k = 0; k < kTopK; ++k) key[k] = kNoId;
+    for (int k = 0; k < kTopK; ++k) key[k] = none;
     if (keep != 0) {
         const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)p * kTopK);
 #pragma unroll
         for (int k = 0; k < kTopK; k += 2) {
             const int2 v = __ldg(&list[k / 2]);
-            if ((unsigned)v.x < (unsigned)n_points && (keep >> k & 1)) key[k] = v.x;
-            if ((unsigned)v.y < (unsigned)n_points && (keep >> (k + 1) & 1)) key[k + 1] = v.y;
+            key[k] = !kBits || (keep >> k & 1) ? (int)min((unsigned)v.x, (unsigned)none) : none;
+            key[k + 1] = !kBits || (keep >> (k + 1) & 1) ? (int)min((unsigned)v.y, (unsigned)none) : none;
         }
     }
     sort_slots(key);
     __syncwarp();
 #pragma unroll
     for (int k = 1; k < kTopK; ++k) keys[k * 32 + lane] = key[k];
-    keys[kTopK * 32 + lane] = kNoId;
+    keys[kTopK * 32 + lane] = none;
     __syncwarp();
-    PatchRows rows = {0, false, 0, 0, 0, key[0] != kNoId};
+    PatchRows rows = {0, false, 0, 0, 0, key[0] != none};
     int head = key[0];
     const int *next = keys + 32 + lane;
-    int row = -kRows * g;
-    while (true) {
+    for (int skip = kRows * g; skip > 0; --skip) {
+        if (head == __reduce_min_sync(0xffffffffu, head) && head != none) head = *next, next += 32;
+    }
+    const unsigned mine = 1u << lane;
+    unsigned bit = 1;
+    do {
         const int id = __reduce_min_sync(0xffffffffu, head);
-        if (id == kNoId) break;
-        if (row == kRows) {
-            rows.more = true;
-            break;
-        }
+        if (id == none) break;
         const bool held = head == id;
         const unsigned holders = __ballot_sync(0xffffffffu, held);
-        if (held) {
-            head = *next;
-            next += 32;
-            if (row >= 0) rows.bits |= 1u << row;
-        }
-        if (row == lane) rows.id = id, rows.holders = holders;
-        ++row;
-    }
-    rows.n = max(row, 0);
+        if (held) head = *next, next += 32, rows.bits |= bit;
+        if (bit == mine) rows.id = id, rows.holders = holders;
+        bit <<= 1;
+    } while (bit != 0);
+    rows.n = bit != 0 ? __ffs(bit) - 1 : kRows;
+    rows.more = bit == 0 && __reduce_min_sync(0xffffffffu, head) != none;
     __syncwarp();
     return rows;
 }

@@ -136,22 +136,21 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const
     float2 total2 = make_float2(0.f, 0.f), scores2 = make_float2(0.f, 0.f);
     bool regular = true, have_totals = false;
     for (int g = 0;;) {
-        const PatchRows rows = find_rows(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        const PatchRows rows = find_rows<kDropout>(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
         regular = Rows<C>::gather(a.rows, rows, sm.pairs) && regular;
         __syncwarp();
         // a lane is a pixel: the group's weights, and the sums over all groups
         unsigned held = rows.bits;
+#pragma unroll 1
         for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
             const float4 *q = sm.pairs + pair * kPairQuads;
             const float2 w = Rows<C>::weights(q, held, minus_x, minus_y);
             sm.weight[2 * pair * kWeightPitch + lane] = w.x, sm.weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
-            if (!have_totals) {
-                float2 score = make_float2(0.f, 0.f);
+            float2 score = make_float2(0.f, 0.f);  // (unused the second time)
 #pragma unroll
-                for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(q, c), make_float2(v[c], v[c]), score);
-                total2 = add2(total2, w);
-                scores2 = fma2(w, score, scores2);
-            }
+            for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(q, c), make_float2(v[c], v[c]), score);
+            total2 = add2(total2, w);
+            scores2 = fma2(w, score, scores2);
         }
         if (!have_totals) {
             if (rows.more) {
@@ -181,11 +180,12 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const
         }
         __syncwarp();
         // a lane is half a row
+#pragma unroll 1
         for (int first = 0; first < rows.n; first += 16) {
+            asm volatile("" ::: "memory");  // the pixels' values stay in shared memory: carried over this loop, they would spill
             const int r = first + (lane & 15);
-            const float2 *mine = reinterpret_cast<const float2 *>(sm.pairs + (r >> 1) * kPairQuads);
-            const bool odd = (r & 1) != 0;
-            auto field = [&](const int e) { return odd ? mine[e].y : mine[e].x; };
+            const float *mine = reinterpret_cast<const float *>(sm.pairs + (r >> 1) * kPairQuads) + (r & 1);
+            auto field = [&](const int e) { return mine[2 * e]; };
             const float x = field(0), y = field(1);
             float2 dx[4], f[C], color[C];
 #pragma unroll
