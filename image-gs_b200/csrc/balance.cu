@@ -15,8 +15,6 @@
 namespace {
 
 using igs::kTile;
-using igs::kTilePixels;
-using igs::kTopK;
 using igs::kWeightPitch;
 
 constexpr int kThreads = 256;
@@ -67,36 +65,48 @@ __global__ void __launch_bounds__(kThreads) balance_rows_kernel(const __grid_con
     igs::Rows<0>::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), {0.f});
 }
 
-// A warp is a patch, a lane first a pixel and then half a row, as in topk_sums.cuh
-__global__ void __launch_bounds__(kTilePixels, 4) balance_kernel(const __grid_constant__ BalanceArgs a) {
+// A warp is a patch, a lane first its pixels and then half a row, as in topk_sums.cuh
+__global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
     using Rows = igs::Rows<0>;
+    constexpr int kPix = igs::kPix;
     __shared__ struct {
         union {
-            int keys[(kTopK + 1) * 32];
+            int keys[igs::kKeyWords];
             alignas(16) float weight[igs::kRows * kWeightPitch];
         };
         float4 pairs[Rows::kGroupQuads];
-        alignas(16) float inv[32];
+        alignas(16) float inv[igs::kPatchPixels];
     } smem[igs::kWarps];
     auto &sm = smem[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31;
     igs::wait_for_predecessor();
     const igs::Patch patch = igs::patch_of(a.tiles_x, a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
-    const unsigned keep = patch.inside && (a.mask == nullptr || a.mask[patch.p] != 0) ? ~0u : 0u;
-    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j), minus_y = make_float2(-(float)patch.i, -(float)patch.i);
+    const auto slots = [&](const int p, const bool inside) { return igs::AllSlots{inside && (a.mask == nullptr || a.mask[p] != 0)}; };
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
+    float2 minus_y[kPix], total[kPix];
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), total[b] = make_float2(0.f, 0.f);
     const int half = lane >> 4;
-    float2 total = make_float2(0.f, 0.f);
     bool have_total = false;
     for (int g = 0;;) {
-        const igs::PatchRows rows = igs::find_rows<false>(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
         Rows::gather(a.rows, rows, sm.pairs);
         __syncwarp();
-        unsigned held = rows.bits;
-        for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
-            const float2 w = Rows::weights(sm.pairs + pair * Rows::kPairQuads, held, minus_x, minus_y);
-            sm.weight[2 * pair * kWeightPitch + lane] = w.x, sm.weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
-            total = igs::add2(total, w);  // (unused the second time)
+        unsigned held[kPix];
+#pragma unroll
+        for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
+#pragma unroll 1
+        for (int pair = 0; 2 * pair < rows.n; ++pair) {
+            float *weight = sm.weight + 2 * pair * kWeightPitch + lane;
+            float2 w[kPix];
+            Rows::weights(sm.pairs + pair * Rows::kPairQuads, held, minus_x, minus_y, w);
+#pragma unroll
+            for (int b = 0; b < kPix; ++b) {
+                held[b] >>= 2;
+                weight[32 * b] = w[b].x, weight[kWeightPitch + 32 * b] = w[b].y;
+                total[b] = igs::add2(total[b], w[b]);  // (unused the second time)
+            }
         }
         if (!have_total) {
             if (rows.more) {
@@ -104,8 +114,9 @@ __global__ void __launch_bounds__(kTilePixels, 4) balance_kernel(const __grid_co
                 continue;
             }
             have_total = true;
-            sm.inv[lane] = 1.f / (total.x + total.y + (float)igs::kNormEps);
-            const unsigned routed = __popc(__ballot_sync(0xffffffffu, rows.filled));
+#pragma unroll
+            for (int b = 0; b < kPix; ++b) sm.inv[32 * b + lane] = 1.f / (total[b].x + total[b].y + (float)igs::kNormEps);
+            const unsigned routed = __reduce_add_sync(0xffffffffu, (unsigned)rows.filled);
             if (lane == 0 && routed > 0) atomicAdd(&a.ws->routed[blockIdx.x % kRoutedSlots], (unsigned long long)routed);
             if (g > 0) {
                 g = 0;
@@ -113,20 +124,22 @@ __global__ void __launch_bounds__(kTilePixels, 4) balance_kernel(const __grid_co
             }
         }
         __syncwarp();
+#pragma unroll 1
         for (int first = 0; first < rows.n; first += 16) {
             const int r = first + (lane & 15);
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 w = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + half * 16 + q * 4]);
-                const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[half * 16 + q * 4]);
+            for (int q = 0; q < igs::kPatchPixels / 8; ++q) {
+                const int at = half * (igs::kPatchPixels / 2) + q * 4;
+                const float4 w = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + at]);
+                const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[at]);
                 sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 16);
             const int id = __shfl_sync(0xffffffffu, rows.id, r);
             if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
         }
-        if (lane < rows.n) atomicAdd(&a.counts[rows.id], __popc(rows.holders));
+        if (lane < rows.n) atomicAdd(&a.counts[rows.id], rows.holders);
         if (!rows.more) return;
         ++g;
     }
@@ -213,7 +226,7 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     const BalanceArgs a = {tiles_x, img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
                            (float)((int64_t)1 << bits), counts, fixed, rows, ws};
     igs::launch(balance_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
-    if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
+    if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(igs::kPatchThreads), 0, s, a);
     igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
                 (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,
                 reinterpret_cast<long long *>(totals));

@@ -11,7 +11,6 @@ namespace {
 
 using igs::kMaxChannels;
 using igs::kTile;
-using igs::kTilePixels;
 using igs::kTopK;
 
 constexpr int kLayOutTiles = 1024;
@@ -28,7 +27,11 @@ struct DropoutArgs {
 };
 
 // One pixel's slots one by one, from global memory
-__device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p, const unsigned keep) {
+__device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p) {
+    const igs::KeptSlots kept({(uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold}, (uint32_t)p, true);
+    unsigned keep = 0;
+#pragma unroll
+    for (int k = 0; k < kTopK; ++k) keep |= kept(k) ? 1u << k : 0u;
     const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
     const int *list = a.pixel_topk + (size_t)p * kTopK;
     float *out = a.out_img + p;
@@ -59,12 +62,13 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
     igs::Rows<C>::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), f);
 }
 
-// A warp is a patch, a lane a pixel
+// A warp is a patch, a lane its pixels
 template <int C>
-__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 4) dropout_kernel(const __grid_constant__ DropoutArgs a) {
+__global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 5) dropout_kernel(const __grid_constant__ DropoutArgs a) {
     using Rows = igs::Rows<C>;
+    constexpr int kPix = igs::kPix;
     __shared__ struct {
-        int keys[(kTopK + 1) * 32];
+        int keys[igs::kKeyWords];
         float4 pairs[Rows::kGroupQuads];
     } smem[igs::kWarps];
     auto &sm = smem[threadIdx.x >> 5];
@@ -73,13 +77,19 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 4) dropout_kernel(co
     if (blockIdx.x == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
     const igs::Patch patch = igs::patch_of(a.tiles_x, a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
-    const unsigned keep = patch.inside ? igs::keep_bits((uint32_t)patch.p, (uint64_t)seed, (uint64_t)offset, a.threshold) : 0u;
-    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j), minus_y = make_float2(-(float)patch.i, -(float)patch.i);
-    float2 total = make_float2(0.f, 0.f), pix[C];
+    const auto slots = [&](const int p, const bool inside) {
+        return igs::KeptSlots({(uint64_t)seed, (uint64_t)offset, a.threshold}, (uint32_t)p, inside);
+    };
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
+    float2 minus_y[kPix], total[kPix], pix[kPix][C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) pix[c] = make_float2(0.f, 0.f);
+    for (int b = 0; b < kPix; ++b) {
+        minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), total[b] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < C; ++c) pix[b][c] = make_float2(0.f, 0.f);
+    }
     for (int g = 0;; ++g) {
-        const igs::PatchRows rows = igs::find_rows<true>(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
         const bool finite = Rows::gather(a.rows, rows, sm.pairs, [&](const int id, float(&q)[4 * Rows::kQuads]) {
             const igs::RowGeometry r = igs::row_geometry(a.xys, a.conics, id);
             q[0] = r.x, q[1] = r.y, q[2] = r.a, q[3] = r.b, q[4] = r.c;
@@ -88,26 +98,39 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 5 : 4) dropout_kernel(co
                 if (c < a.channels && r.finite) q[5 + c] = __ldg(&a.colors[(size_t)id * a.channels + c]);
         });
         if (!finite) {  // zero times a colour that is not finite would reach pixels that do not name it
-            if (patch.inside) blend_slots(a, patch.p, keep);
+#pragma unroll 1
+            for (int b = 0; b < kPix; ++b)
+                if (patch.inside[b]) blend_slots(a, patch.p[b]);
             return;
         }
         __syncwarp();
-        unsigned held = rows.bits;
-        for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
-            const float4 *q = sm.pairs + pair * Rows::kPairQuads;
-            const float2 w = Rows::weights(q, held, minus_x, minus_y);
-            total = igs::add2(total, w);
+        unsigned held[kPix];
 #pragma unroll
-            for (int c = 0; c < C; ++c) pix[c] = igs::fma2(w, Rows::value(q, c), pix[c]);
+        for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
+#pragma unroll 1
+        for (int pair = 0; 2 * pair < rows.n; ++pair) {
+            const float4 *q = sm.pairs + pair * Rows::kPairQuads;
+            float2 w[kPix];
+            Rows::weights(q, held, minus_x, minus_y, w);
+#pragma unroll
+            for (int b = 0; b < kPix; ++b) {
+                held[b] >>= 2;
+                total[b] = igs::add2(total[b], w[b]);
+#pragma unroll
+                for (int c = 0; c < C; ++c) pix[b][c] = igs::fma2(w[b], Rows::value(q, c), pix[b][c]);
+            }
         }
         if (!rows.more) break;
     }
-    if (!patch.inside) return;
-    const float inv = 1.f / (total.x + total.y + (float)igs::kNormEps);
     const size_t plane = (size_t)a.img_h * a.img_w;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-        if (c < a.channels) a.out_img[c * plane + patch.p] = (pix[c].x + pix[c].y) * inv;
+    for (int b = 0; b < kPix; ++b) {
+        if (!patch.inside[b]) continue;
+        const float inv = 1.f / (total[b].x + total[b].y + (float)igs::kNormEps);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (c < a.channels) a.out_img[c * plane + patch.p[b]] = (pix[b][c].x + pix[b][c].y) * inv;
+    }
 }
 
 __global__ void rng_used_kernel(const long long *rng, long long *rng_used) {
@@ -167,7 +190,7 @@ int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_po
         with_width(channels, [&](auto width) {
             constexpr int kWidth = decltype(width)::value;
             if (lay_out) igs::launch(dropout_rows_kernel<kWidth>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, a);
-            igs::launch(dropout_kernel<kWidth>, dim3(tiles_x * tiles_y), dim3(kTilePixels), 0, s, a);
+            igs::launch(dropout_kernel<kWidth>, dim3(tiles_x * tiles_y), dim3(igs::kPatchThreads), 0, s, a);
         });
     }
     return igs::check_launch("igs_topk_dropout_fwd");

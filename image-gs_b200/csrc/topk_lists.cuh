@@ -22,48 +22,73 @@ __device__ __forceinline__ uint4 philox4x32(uint4 c, uint2 key) {
     return c;
 }
 
-// The ten 24-bit draws of a pixel, compared with the threshold: bit k is set where slot k is kept. Two calls give eight words: slot k < 8
-// takes the upper 24 bits of word k, slots 8 and 9 the low bytes of words 0, 1, 2 and 3, 4, 5 (the first most significant), which no other
-// slot uses; a third call for two slots would cost half as much again.
-__device__ __forceinline__ unsigned keep_bits(uint32_t pixel, uint64_t seed, uint64_t offset, uint32_t threshold) {
-    const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
-    const uint32_t o0 = (uint32_t)offset, o1 = (uint32_t)(offset >> 32);
-    const uint4 a = philox4x32(make_uint4(pixel, 0u, o0, o1), key), b = philox4x32(make_uint4(pixel, 1u, o0, o1), key);
-    const uint32_t words[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    unsigned keep = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) keep |= (words[k] >> 8) >= threshold ? 1u << k : 0u;
-    const uint32_t d8 = (words[0] & 255u) << 16 | (words[1] & 255u) << 8 | (words[2] & 255u);
-    const uint32_t d9 = (words[3] & 255u) << 16 | (words[4] & 255u) << 8 | (words[5] & 255u);
-    keep |= d8 >= threshold ? 1u << 8 : 0u;
-    keep |= d9 >= threshold ? 1u << 9 : 0u;
-    return keep;
-}
+// Which slots of a pixel may be filled: all of them (one bit says whether the pixel counts at all), or those that a dropout draw keeps
+struct AllSlots {
+    bool counts;
+    __device__ __forceinline__ bool any() const { return counts; }
+    __device__ __forceinline__ bool operator()(int) const { return true; }
+};
+
+// The ten 24-bit draws of a pixel, kept where they are not below a threshold. Two calls give eight words: slot k < 8 takes the upper 24
+// bits of word k, slots 8 and 9 the low bytes of words 0, 1, 2 and 3, 4, 5 (the first most significant), which no other slot uses; a third
+// call for two slots would cost half as much again.
+struct Dropout {
+    uint64_t seed, offset;
+    uint32_t threshold;  // rint(p 2^24)
+};
+struct KeptSlots {
+    uint32_t words[8];
+    uint32_t threshold;
+    bool counts;
+    __device__ __forceinline__ KeptSlots(const Dropout &d, const uint32_t pixel, const bool inside) : threshold(d.threshold), counts(inside) {
+        if (threshold == 0) return;  // p = 0: nothing is drawn
+        const uint2 key = make_uint2((uint32_t)d.seed, (uint32_t)(d.seed >> 32));
+        const uint32_t o0 = (uint32_t)d.offset, o1 = (uint32_t)(d.offset >> 32);
+        const uint4 a = philox4x32(make_uint4(pixel, 0u, o0, o1), key), b = philox4x32(make_uint4(pixel, 1u, o0, o1), key);
+        words[0] = a.x, words[1] = a.y, words[2] = a.z, words[3] = a.w, words[4] = b.x, words[5] = b.y, words[6] = b.z, words[7] = b.w;
+    }
+    __device__ __forceinline__ bool any() const { return counts; }
+    __device__ __forceinline__ bool operator()(const int k) const {
+        if (threshold == 0) return true;
+        // for a whole word, word >> 8 >= threshold is word > 256 threshold - 1, which wraps to "never" at threshold 2^24
+        if (k < 8) return words[k] > 256u * threshold - 1u;
+        const int w = k == 8 ? 0 : 3;
+        return ((words[w] & 255u) << 16 | (words[w + 1] & 255u) << 8 | (words[w + 2] & 255u)) >= threshold;
+    }
+};
 
 // ---- a patch's Gaussians as rows -------------------------------------------------------------------------------------------------------
 //
-// A warp takes an 8x4 patch of pixels, a lane one pixel. Neighbouring pixels name nearly the same Gaussians (at a trained image's 100 pixels
-// per Gaussian the 320 slots of a patch name 13 to 14), so the patch's distinct IDs become rows, in the order of their IDs: every lane
-// sorts its ten slots (a 29-comparator network) into shared memory, and the warp then takes the smallest unconsumed ID of all its pixels
+// A warp takes an 8x8 patch of pixels, a lane two of them. Neighbouring pixels name nearly the same Gaussians (at a trained image's 100
+// pixels per Gaussian the 640 slots of a patch name 14 to 16, those of an 8x4 patch 13 to 14), so the patch's distinct IDs become rows, in the order of their IDs: every lane
+// sorts its pixels' ten slots (a 29-comparator network) into shared memory, and the warp then takes the smallest unconsumed ID of all its pixels
 // again and again. An ID twice in one list becomes two rows. What a row means to a pixel is a bit of the lane's mask; the rows' parameters
 // are read once, by a lane each, and laid side by side in pairs, so that the warp reads them as broadcasts, two rows per packed (f32x2)
 // instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need no other warp, so nothing waits at a
 // barrier. (The tile's IDs collected by its eight warps in one hash table took twice the instructions, and half the time at barriers.)
-constexpr int kRows = 32;      // rows of a group: a patch with more goes over them group by group
-constexpr int kWarps = 8;      // patches of a CTA: a 16x16 tile
+constexpr int kRows = 32;         // rows of a group: a patch with more goes over them group by group
+constexpr int kPix = 2;           // pixels of a lane: one above the other, four lines apart
+constexpr int kLines = 4 * kPix;  // a patch: 8 pixels by kLines
+constexpr int kPatchPixels = 32 * kPix;
+constexpr int kWarps = kTilePixels / kPatchPixels;  // patches of a CTA: a 16x16 tile
+constexpr int kPatchThreads = kWarps * 32;
 
-// The patch of a warp and the pixel of a lane
+// The patch of a warp and the pixels of a lane
 struct Patch {
-    int x0, y0, i, j, p;
-    bool inside;
+    int x0, y0, j, i[kPix], p[kPix];
+    bool inside[kPix];
 };
 __device__ __forceinline__ Patch patch_of(const int tiles_x, const int img_h, const int img_w) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Patch a;
-    a.x0 = (blockIdx.x % tiles_x) * kTile + (warp & 1) * 8, a.y0 = (blockIdx.x / tiles_x) * kTile + (warp >> 1) * 4;
-    a.i = a.y0 + (lane >> 3), a.j = a.x0 + (lane & 7);
-    a.inside = a.i < img_h && a.j < img_w;
-    a.p = a.inside ? a.i * img_w + a.j : 0;
+    a.x0 = (blockIdx.x % tiles_x) * kTile + (warp & 1) * 8, a.y0 = (blockIdx.x / tiles_x) * kTile + (warp >> 1) * kLines;
+    a.j = a.x0 + (lane & 7);
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) {
+        a.i[b] = a.y0 + (lane >> 3) + 4 * b;
+        a.inside[b] = a.i[b] < img_h && a.j < img_w;
+        a.p[b] = a.inside[b] ? a.i[b] * img_w + a.j : 0;
+    }
     return a;
 }
 
@@ -82,58 +107,75 @@ __device__ __forceinline__ void sort_slots(int (&key)[kTopK]) {
 
 // Rows [32 g, 32 g + 32) of the patch
 struct PatchRows {
-    int n;             // how many there are, at most 32
-    bool more;         // whether others follow
-    unsigned bits;     // the rows that this lane's pixel holds
-    int id;            // lane l < n: the ID of row l,
-    unsigned holders;  // and the pixels that hold it
-    bool filled;       // whether this lane's pixel has a slot at all
+    int n;                // how many there are, at most 32
+    bool more;            // whether others follow
+    unsigned bits[kPix];  // the rows that this lane's pixels hold
+    int id;               // lane l < n: the ID of row l,
+    int holders;          // and how many pixels hold it
+    int filled;           // how many of this lane's pixels have a slot at all
 };
 
-// keys: shared memory of this warp, [kTopK + 1][32]; keep: a bit for each slot that may be filled (kBits false: all or none of them). All
-// lanes together.
-template <bool kBits>
-__device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const int p, const int n_points, const unsigned keep, const int g,
+constexpr int kKeyWords = kPix * (kTopK + 1) * 32;  // shared memory of a warp for find_rows
+
+// slots(pixel, inside) says which of a pixel's slots may be filled. All lanes together.
+template <typename Slots>
+__device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const Patch &patch, const int n_points, const Slots slots, const int g,
                                                int *keys) {
     const int lane = threadIdx.x & 31;
     const int none = n_points;  // the key of an empty slot: behind every ID
-    int key[kTopK];
+    PatchRows rows = {};
+    int head[kPix];
+    const int *next[kPix];
+    __syncwarp();
 #pragma unroll
-    for (int k = 0; k < kTopK; ++k) key[k] = none;
-    if (keep != 0) {
-        const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)p * kTopK);
+    for (int b = 0; b < kPix; ++b) {
+        int key[kTopK];
+        const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)patch.p[b] * kTopK);  // (of some pixel, if it is outside)
 #pragma unroll
         for (int k = 0; k < kTopK; k += 2) {
             const int2 v = __ldg(&list[k / 2]);
-            key[k] = !kBits || (keep >> k & 1) ? (int)min((unsigned)v.x, (unsigned)none) : none;
-            key[k + 1] = !kBits || (keep >> (k + 1) & 1) ? (int)min((unsigned)v.y, (unsigned)none) : none;
+            key[k] = v.x, key[k + 1] = v.y;
         }
-    }
-    sort_slots(key);
-    __syncwarp();
+        const auto may = slots(patch.p[b], patch.inside[b]);
 #pragma unroll
-    for (int k = 1; k < kTopK; ++k) keys[k * 32 + lane] = key[k];
-    keys[kTopK * 32 + lane] = none;
-    __syncwarp();
-    PatchRows rows = {0, false, 0, 0, 0, key[0] != none};
-    int head = key[0];
-    const int *next = keys + 32 + lane;
+        for (int k = 0; k < kTopK; ++k) key[k] = may.any() && may(k) ? (int)min((unsigned)key[k], (unsigned)none) : none;
+        sort_slots(key);
+        int *const column = keys + b * (kTopK + 1) * 32 + lane;
+#pragma unroll
+        for (int k = 1; k < kTopK; ++k) column[k * 32] = key[k];
+        column[kTopK * 32] = none;
+        head[b] = key[0], next[b] = column + 32;
+        rows.filled += key[0] != none;
+    }
+    auto smallest = [&]() {
+        int m = head[0];
+#pragma unroll
+        for (int b = 1; b < kPix; ++b) m = min(m, head[b]);
+        return __reduce_min_sync(0xffffffffu, m);
+    };
     for (int skip = kRows * g; skip > 0; --skip) {
-        if (head == __reduce_min_sync(0xffffffffu, head) && head != none) head = *next, next += 32;
+        const int id = smallest();
+#pragma unroll
+        for (int b = 0; b < kPix; ++b)
+            if (head[b] == id && id != none) head[b] = *next[b], next[b] += 32;
     }
     const unsigned mine = 1u << lane;
     unsigned bit = 1;
     do {
-        const int id = __reduce_min_sync(0xffffffffu, head);
+        const int id = smallest();
         if (id == none) break;
-        const bool held = head == id;
-        const unsigned holders = __ballot_sync(0xffffffffu, held);
-        if (held) head = *next, next += 32, rows.bits |= bit;
+        int holders = 0;
+#pragma unroll
+        for (int b = 0; b < kPix; ++b) {
+            const bool held = head[b] == id;
+            holders += __popc(__ballot_sync(0xffffffffu, held));
+            if (held) head[b] = *next[b], next[b] += 32, rows.bits[b] |= bit;
+        }
         if (bit == mine) rows.id = id, rows.holders = holders;
         bit <<= 1;
     } while (bit != 0);
     rows.n = bit != 0 ? __ffs(bit) - 1 : kRows;
-    rows.more = bit == 0 && __reduce_min_sync(0xffffffffu, head) != none;
+    rows.more = bit == 0 && smallest() != none;
     __syncwarp();
     return rows;
 }
@@ -245,14 +287,19 @@ struct Rows {
         return gather(all, rows, pairs, [](int, float (&)[4 * kQuads]) {});
     }
 
-    // The weights of a pair's two rows at a pixel, bits 0 and 1 of held saying whether the pixel holds them
-    static __device__ __forceinline__ float2 weights(const float4 *pair, const unsigned held, const float2 minus_x, const float2 minus_y) {
+    // The weights of a pair's two rows at the lane's pixels, bits 0 and 1 of held saying which of them a pixel holds; minus_x is (-px, -px)
+    static __device__ __forceinline__ void weights(const float4 *pair, const unsigned (&held)[kPix], const float2 minus_x,
+                                                   const float2 (&minus_y)[kPix], float2 (&w)[kPix]) {
         const float4 xy = pair[0], ab = pair[1];
         const float2 c = *reinterpret_cast<const float2 *>(&pair[2]);
-        const float2 dx = add2(make_float2(xy.x, xy.y), minus_x), dy = add2(make_float2(xy.z, xy.w), minus_y);
-        const float2 slope = fma2(c, dy, mul2(make_float2(ab.z, ab.w), dx));
-        const float2 e = fma2(slope, dy, mul2(mul2(make_float2(ab.x, ab.y), dx), dx));
-        return make_float2((held & 1) && e.x <= 0.f ? exp2_approx(e.x) : 0.f, (held & 2) && e.y <= 0.f ? exp2_approx(e.y) : 0.f);
+        const float2 dx = add2(make_float2(xy.x, xy.y), minus_x);
+        const float2 bdx = mul2(make_float2(ab.z, ab.w), dx), adx2 = mul2(mul2(make_float2(ab.x, ab.y), dx), dx);
+#pragma unroll
+        for (int b = 0; b < kPix; ++b) {
+            const float2 dy = add2(make_float2(xy.z, xy.w), minus_y[b]);
+            const float2 e = fma2(fma2(c, dy, bdx), dy, adx2);
+            w[b] = make_float2((held[b] & 1) && e.x <= 0.f ? exp2_approx(e.x) : 0.f, (held[b] & 2) && e.y <= 0.f ? exp2_approx(e.y) : 0.f);
+        }
     }
     static __device__ __forceinline__ float2 value(const float4 *pair, const int c) {
         return reinterpret_cast<const float2 *>(pair)[5 + c];

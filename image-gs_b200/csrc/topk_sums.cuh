@@ -5,10 +5,10 @@
 // a Gaussian's sums are sum t dx, t dy, t dx^2, t dx dy, t dy^2 and (dropout) w v'_c, from which finish_kernel forms
 //   v_xy = (a Sx + b Sy, b Sx + c Sy),  v_conic = (Sxx / 2, Sxy, Syy / 2),  v_f = S_c.
 //
-// A warp (an 8x4 patch, topk_lists.cuh) goes over its rows twice. First a lane is a pixel: weights into shared memory (32 rows of 32), D
-// and the scores' sum in registers. Then a lane is half a row: lane l sums row l % 16 over 16 pixels (two patch rows of 8), reading the
-// weights four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per patch row, so t
-// and t dx are summed along it first. One shuffle joins the halves, and the sums go to global memory with one 16-byte vector atomic per
+// A warp (an 8x8 patch, topk_lists.cuh) goes over its rows twice. First a lane is two pixels: weights into shared memory (32 rows of 64), D
+// and the scores' sum in registers. Then a lane is half a row: lane l sums row l % 16 over 32 pixels (four lines of 8), reading the weights
+// four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per line, so t and
+// t dx are summed along it first. One shuffle joins the halves, and the sums go to global memory with one 16-byte vector atomic per
 // four values. A patch of more than 32 rows goes over its groups once for D and the scores and once more for the sums. Where a value is not
 // finite, the patch takes the per-slot path instead: zero times it would reach Gaussians that the pixel does not name.
 #pragma once
@@ -17,7 +17,7 @@
 
 namespace igs {
 
-constexpr int kWeightPitch = 36;  // words: the reads of four pixels by eight lanes (rows) fall on distinct banks
+constexpr int kWeightPitch = kPatchPixels + 4;  // words: the reads of four pixels by eight lanes (rows) fall on distinct banks
 
 struct SumArgs {
     int tiles_x, img_h, img_w, channels, n;
@@ -44,11 +44,11 @@ template <int C, bool kDropout>
 struct SumSmem {
     struct Warp {
         union {
-            int keys[(kTopK + 1) * 32];
+            int keys[kKeyWords];
             alignas(16) float weight[kRows * kWeightPitch];
         };
         float4 pairs[Rows<C>::kGroupQuads];
-        alignas(16) float pixel[C + 1][32];  // v'_c, m'
+        alignas(16) float pixel[C + 1][kPatchPixels];  // v'_c, m'
     } warp[kWarps];
 };
 
@@ -66,9 +66,20 @@ __device__ __forceinline__ float pixel_value(const SumArgs &a, const int p, cons
     return 1.f;
 }
 
+template <bool kDropout>
+__device__ __forceinline__ auto sum_slots(const SumArgs &a, const int p, const bool inside) {
+    if constexpr (kDropout) return KeptSlots({(uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold}, (uint32_t)p, inside);
+    else return AllSlots{inside && (a.mask == nullptr || a.mask[p] != 0)};
+}
+
 // One pixel's slots one by one, from global memory: a slot of weight 0 adds nothing
 template <int C, bool kDropout>
-__device__ __noinline__ void add_slots(const SumArgs &a, const int p, const unsigned keep) {
+__device__ __noinline__ void add_slots(const SumArgs &a, const int p, const bool inside) {
+    const auto may = sum_slots<kDropout>(a, p, inside);
+    if (!may.any()) return;
+    unsigned keep = 0;
+#pragma unroll
+    for (int k = 0; k < kTopK; ++k) keep |= may(k) ? 1u << k : 0u;
     constexpr int kValues = SumLayout<C, kDropout>::kValues;
     const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
     const int *list = a.pixel_topk + (size_t)p * kTopK;
@@ -113,7 +124,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ SumAr
 }
 
 template <int C, bool kDropout>
-__global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
+__global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : C <= 7 ? 4 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
     constexpr int kValues = SumLayout<C, kDropout>::kValues;
     constexpr int kPairQuads = Rows<C>::kPairQuads;
     extern __shared__ __align__(16) char smem_bytes[];
@@ -122,54 +133,71 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const
     wait_for_predecessor();
     const Patch patch = patch_of(a.tiles_x, a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
-    unsigned keep = 0;
-    if (patch.inside) {
-        if constexpr (kDropout) keep = keep_bits((uint32_t)patch.p, (uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold);
-        else keep = a.mask == nullptr || a.mask[patch.p] != 0 ? ~0u : 0u;
-    }
-    float v[C];
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
+    float2 minus_y[kPix], total2[kPix], scores2[kPix];
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = patch.inside ? pixel_value<kDropout>(a, patch.p, c) : 0.f;
-    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j), minus_y = make_float2(-(float)patch.i, -(float)patch.i);
+    for (int b = 0; b < kPix; ++b) {
+        minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]);
+        total2[b] = make_float2(0.f, 0.f), scores2[b] = make_float2(0.f, 0.f);
+    }
     const int half = lane >> 4;
-    const float x0 = (float)patch.x0, y0 = (float)(patch.y0 + half * 2);
-    float2 total2 = make_float2(0.f, 0.f), scores2 = make_float2(0.f, 0.f);
+    const float x0 = (float)patch.x0, y0 = (float)(patch.y0 + half * (kLines / 2));
     bool regular = true, have_totals = false;
     for (int g = 0;;) {
-        const PatchRows rows = find_rows<kDropout>(a.pixel_topk, patch.p, a.n, keep, g, sm.keys);
+        const PatchRows rows =
+            find_rows(a.pixel_topk, patch, a.n, [&](const int p, const bool inside) { return sum_slots<kDropout>(a, p, inside); }, g, sm.keys);
+        float v[kPix][C];
+#pragma unroll
+        for (int b = 0; b < kPix; ++b)
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[b][c] = patch.inside[b] && !have_totals ? pixel_value<kDropout>(a, patch.p[b], c) : 0.f;
         regular = Rows<C>::gather(a.rows, rows, sm.pairs) && regular;
         __syncwarp();
-        // a lane is a pixel: the group's weights, and the sums over all groups
-        unsigned held = rows.bits;
-#pragma unroll 1
-        for (int pair = 0; 2 * pair < rows.n; ++pair, held >>= 2) {
-            const float4 *q = sm.pairs + pair * kPairQuads;
-            const float2 w = Rows<C>::weights(q, held, minus_x, minus_y);
-            sm.weight[2 * pair * kWeightPitch + lane] = w.x, sm.weight[(2 * pair + 1) * kWeightPitch + lane] = w.y;
-            float2 score = make_float2(0.f, 0.f);  // (unused the second time)
+        // a lane is kPix pixels: the group's weights, and the sums over all groups
+        unsigned held[kPix];
 #pragma unroll
-            for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(q, c), make_float2(v[c], v[c]), score);
-            total2 = add2(total2, w);
-            scores2 = fma2(w, score, scores2);
+        for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
+#pragma unroll 1
+        for (int pair = 0; 2 * pair < rows.n; ++pair) {
+            const float4 *q = sm.pairs + pair * kPairQuads;
+            float *weight = sm.weight + 2 * pair * kWeightPitch + lane;
+            float2 w[kPix];
+            Rows<C>::weights(q, held, minus_x, minus_y, w);
+#pragma unroll
+            for (int b = 0; b < kPix; ++b) {
+                held[b] >>= 2;
+                weight[32 * b] = w[b].x, weight[kWeightPitch + 32 * b] = w[b].y;
+                float2 score = make_float2(0.f, 0.f);  // (unused the second time)
+#pragma unroll
+                for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(q, c), make_float2(v[b][c], v[b][c]), score);
+                total2[b] = add2(total2[b], w[b]);
+                scores2[b] = fma2(w[b], score, scores2[b]);
+            }
         }
         if (!have_totals) {
             if (rows.more) {
                 ++g;
                 continue;
             }
-            const float total = total2.x + total2.y, scores = scores2.x + scores2.y;
-            const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
-            const float inv = 1.f / (total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
-            float size = fabsf(m);
+            bool finite = regular;
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const float vc = some ? v[c] * inv : 0.f;
-                size += fabsf(vc);
-                sm.pixel[c][lane] = vc;
+            for (int b = 0; b < kPix; ++b) {
+                const float total = total2[b].x + total2[b].y, scores = scores2[b].x + scores2[b].y;
+                const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
+                const float inv = 1.f / (total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
+                float size = fabsf(m);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float vc = some ? v[b][c] * inv : 0.f;
+                    size += fabsf(vc);
+                    sm.pixel[c][32 * b + lane] = vc;
+                }
+                sm.pixel[C][32 * b + lane] = m;
+                finite = finite && isfinite(size);
             }
-            sm.pixel[C][lane] = m;
-            if (!__all_sync(0xffffffffu, regular && isfinite(size))) {
-                if (patch.inside) add_slots<C, kDropout>(a, patch.p, keep);
+            if (!__all_sync(0xffffffffu, finite)) {
+#pragma unroll 1
+                for (int b = 0; b < kPix; ++b) add_slots<C, kDropout>(a, patch.p[b], patch.inside[b]);
                 return;
             }
             have_totals = true;
@@ -194,12 +222,12 @@ __global__ void __launch_bounds__(kTilePixels, C <= 3 ? 4 : 3) sums_kernel(const
             for (int c = 0; c < C; ++c) f[c].x = -field(5 + c), f[c].y = f[c].x, color[c] = make_float2(0.f, 0.f);
             float2 xx = make_float2(0.f, 0.f);
             float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
-#pragma unroll
-            for (int line = 0; line < 2; ++line) {
+#pragma unroll 1
+            for (int line = 0; line < kLines / 2; ++line) {
                 float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int quad = 0; quad < 2; ++quad) {
-                    const int at = half * 16 + line * 8 + quad * 4;
+                    const int at = half * (kPatchPixels / 2) + line * 8 + quad * 4;
                     const float4 w4 = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + at]);
                     const float4 m4 = *reinterpret_cast<const float4 *>(&sm.pixel[C][at]);
                     float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
@@ -288,7 +316,7 @@ void launch_sums(SumArgs a, void *workspace, const bool accumulate, float *v_xy,
     if (a.img_h > 0 && a.img_w > 0) {
         // past 48 KB the kernel has to be told; the setting belongs to the device, so every call makes it
         if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        launch(sums_kernel<C, kDropout>, dim3(a.tiles_x * ceil_div(a.img_h, kTile)), dim3(kTilePixels), kBytes, s, a);
+        launch(sums_kernel<C, kDropout>, dim3(a.tiles_x * ceil_div(a.img_h, kTile)), dim3(kPatchThreads), kBytes, s, a);
     }
     launch(finish_sums_kernel<kValues>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a.n, a.channels, a.conics, (const float *)a.sums,
            accumulate, v_xy, v_conic, v_colors);
