@@ -15,10 +15,13 @@
 namespace {
 
 using igs::kTile;
-using igs::kWeightPitch;
 
 constexpr int kThreads = 256;
 constexpr int kRoutedSlots = 32;
+using igs::kPatchPixels;
+using igs::kPix;
+using igs::kWeightPitch;
+using Rows = igs::Rows<0>;
 
 struct BalanceWorkspace {
     unsigned long long filled;                // A
@@ -30,7 +33,7 @@ struct BalanceWorkspace {
 
 int finish_blocks(int n) { return n > 0 ? igs::ceil_div(n, kThreads) : 1; }
 size_t forward_bytes(int n) {
-    return sizeof(BalanceWorkspace) + (sizeof(unsigned long long) + sizeof(float4) * igs::Rows<0>::kQuads) * (size_t)n + 8 +
+    return sizeof(BalanceWorkspace) + (sizeof(unsigned long long) + sizeof(float4) * Rows::kQuads) * (size_t)n + 8 +
            sizeof(double) * (size_t)finish_blocks(n);
 }
 size_t workspace_bytes_of(int n) { return std::max(forward_bytes(n), igs::sum_bytes<1, false>(n)); }
@@ -43,7 +46,7 @@ int fraction_bits(int64_t pixels) {
 }
 
 struct BalanceArgs {
-    int tiles_x, img_h, img_w, n;
+    int img_h, img_w, n;
     const float *xys, *conics;
     const int *pixel_topk;
     const uint8_t *mask;
@@ -62,25 +65,45 @@ __global__ void __launch_bounds__(kThreads) balance_rows_kernel(const __grid_con
     if (id < kRoutedSlots) a.ws->routed[id] = 0;
     if (id >= a.n) return;
     a.counts[id] = 0, a.fixed[id] = 0;
-    igs::Rows<0>::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), {0.f});
+    Rows::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), {0.f});
+}
+
+// One pixel's slots one by one, from global memory (topk_sums.cuh says when)
+__device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
+    if (a.mask != nullptr && a.mask[p] == 0) return;
+    const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
+    const int *list = a.pixel_topk + (size_t)p * igs::kTopK;
+    float total = (float)igs::kNormEps;
+    for (int pass = 0; pass < 2; ++pass) {
+        const float inv = igs::reciprocal(total);
+        for (int k = 0; k < igs::kTopK; ++k) {
+            const int id = list[k];
+            if ((unsigned)id >= (unsigned)a.n) continue;
+            const float w = igs::slot_weight(igs::row_geometry(a.xys, a.conics, id), px, py);
+            if (pass == 0) {
+                total += w;
+            } else {
+                atomicAdd(&a.counts[id], 1);
+                atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(w * inv * a.scale));
+            }
+        }
+    }
 }
 
 // A warp is a patch, a lane first its pixels and then half a row, as in topk_sums.cuh
 __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
-    using Rows = igs::Rows<0>;
-    constexpr int kPix = igs::kPix;
     __shared__ struct {
         union {
             int keys[igs::kKeyWords];
             alignas(16) float weight[igs::kRows * kWeightPitch];
         };
         float4 pairs[Rows::kGroupQuads];
-        alignas(16) float inv[igs::kPatchPixels];
-    } smem[igs::kWarps];
+        alignas(16) float inv[kPatchPixels];
+    } smem[igs::kPatches];
     auto &sm = smem[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31;
     igs::wait_for_predecessor();
-    const igs::Patch patch = igs::patch_of(a.tiles_x, a.img_h, a.img_w);
+    const igs::Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
     const auto slots = [&](const int p, const bool inside) { return igs::AllSlots{inside && (a.mask == nullptr || a.mask[p] != 0)}; };
     const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
@@ -88,10 +111,10 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
 #pragma unroll
     for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), total[b] = make_float2(0.f, 0.f);
     const int half = lane >> 4;
-    bool have_total = false;
+    bool regular = true, have_total = false;
     for (int g = 0;;) {
         const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
-        Rows::gather(a.rows, rows, sm.pairs);
+        regular = Rows::gather(a.rows, rows, sm.pairs) && regular;
         __syncwarp();
         unsigned held[kPix];
 #pragma unroll
@@ -115,9 +138,16 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
             }
             have_total = true;
 #pragma unroll
-            for (int b = 0; b < kPix; ++b) sm.inv[32 * b + lane] = 1.f / (total[b].x + total[b].y + (float)igs::kNormEps);
+            for (int b = 0; b < kPix; ++b) sm.inv[32 * b + lane] = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
             const unsigned routed = __reduce_add_sync(0xffffffffu, (unsigned)rows.filled);
-            if (lane == 0 && routed > 0) atomicAdd(&a.ws->routed[blockIdx.x % kRoutedSlots], (unsigned long long)routed);
+            if (lane == 0 && routed > 0)
+                atomicAdd(&a.ws->routed[(blockIdx.x + blockIdx.y) % kRoutedSlots], (unsigned long long)routed);
+            if (!regular) {
+#pragma unroll 1
+                for (int b = 0; b < kPix; ++b)
+                    if (patch.inside[b]) count_slots(a, patch.p[b]);
+                return;
+            }
             if (g > 0) {
                 g = 0;
                 continue;
@@ -129,8 +159,8 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
             const int r = first + (lane & 15);
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < igs::kPatchPixels / 8; ++q) {
-                const int at = half * (igs::kPatchPixels / 2) + q * 4;
+            for (int q = 0; q < kPatchPixels / 8; ++q) {
+                const int at = half * (kPatchPixels / 2) + q * 4;
                 const float4 w = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + at]);
                 const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[at]);
                 sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
@@ -219,14 +249,13 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(base);
     unsigned long long *fixed = reinterpret_cast<unsigned long long *>(base + sizeof(BalanceWorkspace));
     float4 *rows = reinterpret_cast<float4 *>(fixed + (num_points + 1) / 2 * 2);
-    double *partials = reinterpret_cast<double *>(rows + (size_t)igs::Rows<0>::kQuads * num_points);
+    double *partials = reinterpret_cast<double *>(rows + (size_t)Rows::kQuads * num_points);
     const int bits = fraction_bits(pixels);
     const int blocks = finish_blocks(num_points);
-    const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
-    const BalanceArgs a = {tiles_x, img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
+    const BalanceArgs a = {img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
                            (float)((int64_t)1 << bits), counts, fixed, rows, ws};
     igs::launch(balance_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
-    if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, dim3(tiles_x * tiles_y), dim3(igs::kPatchThreads), 0, s, a);
+    if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
     igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
                 (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,
                 reinterpret_cast<long long *>(totals));
@@ -248,7 +277,7 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
     IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_balance_bwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
     igs::SumArgs a = {};
-    a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.n = num_points;
+    a.img_h = img_height, a.img_w = img_width, a.n = num_points;
     a.xys = xys, a.conics = conics, a.pixel_topk = pixel_topk, a.mask = pixel_mask;
     a.counts = counts, a.totals = reinterpret_cast<const long long *>(totals), a.v_loss = v_loss, a.v_importance = v_importance;
     igs::launch_sums<1, false>(a, workspace, accumulate != 0, v_xy, v_conic, nullptr, s);

@@ -10,13 +10,14 @@
 namespace {
 
 using igs::kMaxChannels;
+using igs::kPix;
 using igs::kTile;
 using igs::kTopK;
 
 constexpr int kLayOutTiles = 1024;
 
 struct DropoutArgs {
-    int tiles_x, img_h, img_w, channels, n;
+    int img_h, img_w, channels, n;
     const float *xys, *conics, *colors;
     const int *pixel_topk;
     uint32_t threshold;
@@ -66,16 +67,15 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
 template <int C>
 __global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 5) dropout_kernel(const __grid_constant__ DropoutArgs a) {
     using Rows = igs::Rows<C>;
-    constexpr int kPix = igs::kPix;
     __shared__ struct {
         int keys[igs::kKeyWords];
         float4 pairs[Rows::kGroupQuads];
-    } smem[igs::kWarps];
+    } smem[igs::kPatches];
     auto &sm = smem[threadIdx.x >> 5];
     igs::wait_for_predecessor();
     const long long seed = a.rng[0], offset = a.rng[1];
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
-    const igs::Patch patch = igs::patch_of(a.tiles_x, a.img_h, a.img_w);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
+    const igs::Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
     const auto slots = [&](const int p, const bool inside) {
         return igs::KeptSlots({(uint64_t)seed, (uint64_t)offset, a.threshold}, (uint32_t)p, inside);
@@ -90,14 +90,14 @@ __global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 
     }
     for (int g = 0;; ++g) {
         const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
-        const bool finite = Rows::gather(a.rows, rows, sm.pairs, [&](const int id, float(&q)[4 * Rows::kQuads]) {
+        const bool regular = Rows::gather(a.rows, rows, sm.pairs, [&](const int id, float(&q)[4 * Rows::kQuads]) {
             const igs::RowGeometry r = igs::row_geometry(a.xys, a.conics, id);
-            q[0] = r.x, q[1] = r.y, q[2] = r.a, q[3] = r.b, q[4] = r.c;
+            q[0] = r.regular ? r.x : __int_as_float(0x7fc00000), q[1] = r.y, q[2] = r.a, q[3] = r.b, q[4] = r.c;
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (c < a.channels && r.finite) q[5 + c] = __ldg(&a.colors[(size_t)id * a.channels + c]);
+                if (c < a.channels) q[5 + c] = __ldg(&a.colors[(size_t)id * a.channels + c]);
         });
-        if (!finite) {  // zero times a colour that is not finite would reach pixels that do not name it
+        if (!regular) {  // among others, zero times a colour that is not finite would reach pixels that do not name it
 #pragma unroll 1
             for (int b = 0; b < kPix; ++b)
                 if (patch.inside[b]) blend_slots(a, patch.p[b]);
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 
 #pragma unroll
     for (int b = 0; b < kPix; ++b) {
         if (!patch.inside[b]) continue;
-        const float inv = 1.f / (total[b].x + total[b].y + (float)igs::kNormEps);
+        const float inv = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
 #pragma unroll
         for (int c = 0; c < C; ++c)
             if (c < a.channels) a.out_img[c * plane + patch.p[b]] = (pix[b][c].x + pix[b][c].y) * inv;
@@ -138,19 +138,18 @@ __global__ void rng_used_kernel(const long long *rng, long long *rng_used) {
     rng_used[0] = rng[0], rng_used[1] = rng[1];
 }
 
-// The kernels' widths: channels are padded with zeros to one less than a multiple of four, so that a staged row (geometry 5, colours) and a
-// Gaussian's sums (5, colours) are whole 16-byte words. 12 stands for itself (12 + 5 = 17 of 20).
-template <typename F>
-void with_width(int channels, F f) {
-    if (channels <= 3) f(std::integral_constant<int, 3>());
-    else if (channels <= 7) f(std::integral_constant<int, 7>());
-    else if (channels <= 11) f(std::integral_constant<int, 11>());
-    else f(std::integral_constant<int, 12>());
+// One kernel for each number of channels
+template <int C = kMaxChannels, typename F>
+void with_channels(const int channels, F f) {
+    if constexpr (C > 1) {
+        if (channels < C) return with_channels<C - 1>(channels, f);
+    }
+    f(std::integral_constant<int, C>());
 }
 
 size_t workspace_bytes_of(int num_points, int channels) {
     size_t bytes = 0;
-    with_width(channels, [&](auto width) { bytes = igs::sum_bytes<decltype(width)::value, true>(num_points); });
+    with_channels(channels, [&](auto width) { bytes = igs::sum_bytes<decltype(width)::value, true>(num_points); });
     return bytes + 16;  // never nothing
 }
 
@@ -182,15 +181,15 @@ int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_po
     if (pixels == 0) {
         igs::launch(rng_used_kernel, dim3(1), dim3(1), 0, s, rng, used);
     } else {
-        const int tiles_x = igs::ceil_div(img_width, kTile), tiles_y = igs::ceil_div(img_height, kTile);
+        const dim3 grid = igs::tile_grid(img_height, img_width);
         // laying the rows out is a launch of its own, which a small image does not repay
-        const bool lay_out = num_points > 0 && tiles_x * tiles_y > kLayOutTiles;
-        const DropoutArgs a = {tiles_x, img_height, img_width, channels, num_points, xys, conics, colors, pixel_topk,
+        const bool lay_out = num_points > 0 && grid.x * grid.y > kLayOutTiles;
+        const DropoutArgs a = {img_height, img_width, channels, num_points, xys, conics, colors, pixel_topk,
                                (uint32_t)rint(p * 16777216.0), rng, out_img, used, lay_out ? static_cast<float4 *>(workspace) : nullptr};
-        with_width(channels, [&](auto width) {
+        with_channels(channels, [&](auto width) {
             constexpr int kWidth = decltype(width)::value;
             if (lay_out) igs::launch(dropout_rows_kernel<kWidth>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, a);
-            igs::launch(dropout_kernel<kWidth>, dim3(tiles_x * tiles_y), dim3(igs::kPatchThreads), 0, s, a);
+            igs::launch(dropout_kernel<kWidth>, grid, dim3(igs::kPatchThreads), 0, s, a);
         });
     }
     return igs::check_launch("igs_topk_dropout_fwd");
@@ -212,10 +211,10 @@ int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_po
     IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_dropout_bwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
     igs::SumArgs a = {};
-    a.tiles_x = igs::ceil_div(img_width, kTile), a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
+    a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
     a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
     a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0);
-    with_width(channels, [&](auto width) {
+    with_channels(channels, [&](auto width) {
         igs::launch_sums<decltype(width)::value, true>(a, workspace, false, v_xy, v_conic, v_colors, s);
     });
     return igs::check_launch("igs_topk_dropout_bwd");

@@ -40,18 +40,17 @@ struct KeptSlots {
     uint32_t words[8];
     uint32_t threshold;
     bool counts;
-    __device__ __forceinline__ KeptSlots(const Dropout &d, const uint32_t pixel, const bool inside) : threshold(d.threshold), counts(inside) {
-        if (threshold == 0) return;  // p = 0: nothing is drawn
+    __device__ __forceinline__ KeptSlots(const Dropout &d, const uint32_t pixel, const bool inside)
+        : words{}, threshold(d.threshold), counts(inside && d.threshold < 1u << 24) {
+        if (threshold == 0) return;  // p = 0: every word is high enough
         const uint2 key = make_uint2((uint32_t)d.seed, (uint32_t)(d.seed >> 32));
         const uint32_t o0 = (uint32_t)d.offset, o1 = (uint32_t)(d.offset >> 32);
         const uint4 a = philox4x32(make_uint4(pixel, 0u, o0, o1), key), b = philox4x32(make_uint4(pixel, 1u, o0, o1), key);
         words[0] = a.x, words[1] = a.y, words[2] = a.z, words[3] = a.w, words[4] = b.x, words[5] = b.y, words[6] = b.z, words[7] = b.w;
     }
     __device__ __forceinline__ bool any() const { return counts; }
-    __device__ __forceinline__ bool operator()(const int k) const {
-        if (threshold == 0) return true;
-        // for a whole word, word >> 8 >= threshold is word > 256 threshold - 1, which wraps to "never" at threshold 2^24
-        if (k < 8) return words[k] > 256u * threshold - 1u;
+    __device__ __forceinline__ bool operator()(const int k) const {  // where any()
+        if (k < 8) return words[k] >= threshold << 8;                // word >> 8 >= threshold
         const int w = k == 8 ? 0 : 3;
         return ((words[w] & 255u) << 16 | (words[w + 1] & 255u) << 8 | (words[w + 2] & 255u)) >= threshold;
     }
@@ -66,31 +65,31 @@ struct KeptSlots {
 // are read once, by a lane each, and laid side by side in pairs, so that the warp reads them as broadcasts, two rows per packed (f32x2)
 // instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need no other warp, so nothing waits at a
 // barrier. (The tile's IDs collected by its eight warps in one hash table took twice the instructions, and half the time at barriers.)
-constexpr int kRows = 32;         // rows of a group: a patch with more goes over them group by group
-constexpr int kPix = 2;           // pixels of a lane: one above the other, four lines apart
-constexpr int kLines = 4 * kPix;  // a patch: 8 pixels by kLines
+constexpr int kRows = 32;  // rows of a group: a patch with more goes over them group by group
+// The patch of a warp: 8 pixels by kLines, kPix of a lane, one above the other, four lines apart
+constexpr int kPix = 2;
+constexpr int kLines = 4 * kPix;
 constexpr int kPatchPixels = 32 * kPix;
-constexpr int kWarps = kTilePixels / kPatchPixels;  // patches of a CTA: a 16x16 tile
-constexpr int kPatchThreads = kWarps * 32;
+constexpr int kPatches = kTilePixels / kPatchPixels;  // of a CTA: a 16x16 tile
+constexpr int kPatchThreads = kPatches * 32;
+constexpr int kKeyWords = kPix * (kTopK + 1) * 32;    // shared memory of a warp for find_rows
+constexpr int kWeightPitch = kPatchPixels + 4;        // of a row of weights: four pixels by eight rows are read from distinct banks
 
-// The patch of a warp and the pixels of a lane
 struct Patch {
     int x0, y0, j, i[kPix], p[kPix];
     bool inside[kPix];
-};
-__device__ __forceinline__ Patch patch_of(const int tiles_x, const int img_h, const int img_w) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Patch a;
-    a.x0 = (blockIdx.x % tiles_x) * kTile + (warp & 1) * 8, a.y0 = (blockIdx.x / tiles_x) * kTile + (warp >> 1) * kLines;
-    a.j = a.x0 + (lane & 7);
+    __device__ __forceinline__ Patch(const int img_h, const int img_w) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        x0 = blockIdx.x * kTile + (warp & 1) * 8, y0 = blockIdx.y * kTile + (warp >> 1) * kLines;
+        j = x0 + (lane & 7);
 #pragma unroll
-    for (int b = 0; b < kPix; ++b) {
-        a.i[b] = a.y0 + (lane >> 3) + 4 * b;
-        a.inside[b] = a.i[b] < img_h && a.j < img_w;
-        a.p[b] = a.inside[b] ? a.i[b] * img_w + a.j : 0;
+        for (int b = 0; b < kPix; ++b) {
+            i[b] = y0 + (lane >> 3) + 4 * b;
+            inside[b] = i[b] < img_h && j < img_w;
+            p[b] = inside[b] ? i[b] * img_w + j : 0;
+        }
     }
-    return a;
-}
+};
 
 // A sorting network for ten keys (29 comparators, depth 8)
 __device__ __forceinline__ void sort_slots(int (&key)[kTopK]) {
@@ -115,67 +114,73 @@ struct PatchRows {
     int filled;           // how many of this lane's pixels have a slot at all
 };
 
-constexpr int kKeyWords = kPix * (kTopK + 1) * 32;  // shared memory of a warp for find_rows
-
-// slots(pixel, inside) says which of a pixel's slots may be filled. All lanes together.
+// slots(pixel, inside) says which of a pixel's slots may be filled; keys: kKeyWords of shared memory. All lanes together.
 template <typename Slots>
 __device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const Patch &patch, const int n_points, const Slots slots, const int g,
                                                int *keys) {
     const int lane = threadIdx.x & 31;
     const int none = n_points;  // the key of an empty slot: behind every ID
-    PatchRows rows = {};
-    int head[kPix];
-    const int *next[kPix];
-    __syncwarp();
+    int key[kPix][kTopK];
+    bool counts[kPix];
 #pragma unroll
     for (int b = 0; b < kPix; ++b) {
-        int key[kTopK];
         const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)patch.p[b] * kTopK);  // (of some pixel, if it is outside)
 #pragma unroll
         for (int k = 0; k < kTopK; k += 2) {
             const int2 v = __ldg(&list[k / 2]);
-            key[k] = v.x, key[k + 1] = v.y;
+            key[b][k] = v.x, key[b][k + 1] = v.y;
         }
+    }
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) {
         const auto may = slots(patch.p[b], patch.inside[b]);
 #pragma unroll
-        for (int k = 0; k < kTopK; ++k) key[k] = may.any() && may(k) ? (int)min((unsigned)key[k], (unsigned)none) : none;
-        sort_slots(key);
+        for (int k = 0; k < kTopK; ++k) key[b][k] = may(k) ? (int)min((unsigned)key[b][k], (unsigned)none) : none;
+        counts[b] = may.any();
+    }
+    PatchRows rows = {};
+    int head[kPix], next[kPix];
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) {
+        sort_slots(key[b]);
+        head[b] = counts[b] ? key[b][0] : none;  // a list is read on only where its head was taken
+        rows.filled += head[b] != none;
+        next[b] = (b * (kTopK + 1) + 1) * 32 + lane;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) {
         int *const column = keys + b * (kTopK + 1) * 32 + lane;
 #pragma unroll
-        for (int k = 1; k < kTopK; ++k) column[k * 32] = key[k];
+        for (int k = 1; k < kTopK; ++k) column[k * 32] = key[b][k];
         column[kTopK * 32] = none;
-        head[b] = key[0], next[b] = column + 32;
-        rows.filled += key[0] != none;
     }
-    auto smallest = [&]() {
-        int m = head[0];
-#pragma unroll
-        for (int b = 1; b < kPix; ++b) m = min(m, head[b]);
-        return __reduce_min_sync(0xffffffffu, m);
-    };
+    auto smallest = [&]() { return __reduce_min_sync(0xffffffffu, min(head[0], head[kPix - 1])); };
     for (int skip = kRows * g; skip > 0; --skip) {
         const int id = smallest();
 #pragma unroll
         for (int b = 0; b < kPix; ++b)
-            if (head[b] == id && id != none) head[b] = *next[b], next[b] += 32;
+            if (head[b] == id && id != none) head[b] = keys[next[b]], next[b] += 32;
     }
     const unsigned mine = 1u << lane;
-    unsigned bit = 1;
+    unsigned bit = 1, holders[kPix] = {};
     do {
         const int id = smallest();
         if (id == none) break;
-        int holders = 0;
 #pragma unroll
         for (int b = 0; b < kPix; ++b) {
             const bool held = head[b] == id;
-            holders += __popc(__ballot_sync(0xffffffffu, held));
-            if (held) head[b] = *next[b], next[b] += 32, rows.bits[b] |= bit;
+            const unsigned all = __ballot_sync(0xffffffffu, held);
+            if (held) head[b] = keys[next[b]], next[b] += 32, rows.bits[b] |= bit;
+            if (bit == mine) holders[b] = all;
         }
-        if (bit == mine) rows.id = id, rows.holders = holders;
+        if (bit == mine) rows.id = id;
         bit <<= 1;
     } while (bit != 0);
     rows.n = bit != 0 ? __ffs(bit) - 1 : kRows;
     rows.more = bit == 0 && smallest() != none;
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) rows.holders += __popc(holders[b]);
     __syncwarp();
     return rows;
 }
@@ -190,23 +195,25 @@ __device__ __forceinline__ float exp2_approx(const float x) {
 // A Gaussian's geometry as the kernels use it: centre, and the conic times -log2(e) (its outer terms halved too), so that the weight is
 // exp2 of
 //   (a' dx) dx + (c' dy + b' dx) dy
-// where that is not positive, and 0 where it is positive or NaN. A Gaussian whose parameters are not all finite has no finite sigma
-// anywhere; it stands at the origin with a NaN conic, so that its weights are 0 and its offsets finite.
+// With a positive definite conic that is never positive (but for its rounding) and needs no test. Other conics, and parameters that are
+// not finite or so large that the terms could overflow, are marked by a NaN centre in the laid-out row, and the patches that meet one take
+// the per-slot path, which tests.
 struct RowGeometry {
     float x, y, a, b, c;
-    bool finite;
+    bool regular;
 };
 
 __device__ __forceinline__ RowGeometry row_geometry(const float *xys, const float *conics, const int id) {
     constexpr float kLog2e = 1.4426950408889634f;
     const float x = __ldg(&xys[2 * (size_t)id]), y = __ldg(&xys[2 * (size_t)id + 1]);
     const float a = __ldg(&conics[3 * (size_t)id]), b = __ldg(&conics[3 * (size_t)id + 1]), c = __ldg(&conics[3 * (size_t)id + 2]);
-    if (isfinite(x) && isfinite(y) && isfinite(a) && isfinite(b) && isfinite(c))
-        return {x, y, -0.5f * kLog2e * a, -kLog2e * b, -0.5f * kLog2e * c, true};
-    return {0.f, 0.f, __int_as_float(0x7fc00000), 0.f, 0.f, false};
+    const float ac = a * c, bb = b * b;
+    const float det = (ac - bb) + (fmaf(a, c, -ac) - fmaf(b, b, -bb));  // with the products' roundings
+    const bool regular = fabsf(x) < 1e9f && fabsf(y) < 1e9f && a > 0.f && a < 1e15f && c > 0.f && c < 1e15f && det > 0.f;
+    return {x, y, -0.5f * kLog2e * a, -kLog2e * b, -0.5f * kLog2e * c, regular};
 }
 
-// The weight of one slot, from global memory: the per-slot path
+// The weight of one slot, for the per-slot path: 0 where sigma is negative, NaN or infinite
 __device__ __forceinline__ float slot_weight(const RowGeometry &g, const float px, const float py) {
     const float dx = g.x - px, dy = g.y - py;
     const float e = fmaf(fmaf(g.c, dy, g.b * dx), dy, (g.a * dx) * dx);
@@ -246,15 +253,15 @@ struct Rows {
     static constexpr int kGroupQuads = kRows / 2 * kPairQuads;
 
     static __device__ __forceinline__ void store(float4 *all, const int id, const RowGeometry &g, const float (&f)[C > 0 ? C : 1]) {
-        float q[4 * kQuads] = {g.x, g.y, g.a, g.b, g.c};
+        float q[4 * kQuads] = {g.regular ? g.x : __int_as_float(0x7fc00000), g.y, g.a, g.b, g.c};
 #pragma unroll
-        for (int c = 0; c < C; ++c) q[5 + c] = g.finite ? f[c] : 0.f;
+        for (int c = 0; c < C; ++c) q[5 + c] = f[c];
 #pragma unroll
         for (int e = 0; e < kQuads; ++e) all[(size_t)id * kQuads + e] = make_float4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
     }
 
     // The group's rows into the warp's pairs: from the rows of all Gaussians or, where all is NULL, from read(id, q). False, on all lanes,
-    // where a value f is not finite.
+    // where one is not regular or a value f is not finite.
     template <typename Read>
     static __device__ __forceinline__ bool gather(const float4 *all, const PatchRows &rows, float4 *pairs, Read read) {
         const int lane = threadIdx.x & 31;
@@ -272,7 +279,7 @@ struct Rows {
                 read(rows.id, q);
             }
         }
-        float size = 0.f;
+        float size = fabsf(q[0]);
 #pragma unroll
         for (int c = 0; c < C; ++c) size += fabsf(q[5 + c]);
         if (lane <= rows.n) {  // one more, of zeros, to pad the last pair
@@ -280,9 +287,8 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < 5 + C; ++e) pair[2 * e] = q[e];
         }
-        return C == 0 || __all_sync(0xffffffffu, isfinite(size));
+        return __all_sync(0xffffffffu, isfinite(size));
     }
-
     static __device__ __forceinline__ bool gather(const float4 *all, const PatchRows &rows, float4 *pairs) {
         return gather(all, rows, pairs, [](int, float (&)[4 * kQuads]) {});
     }
@@ -298,7 +304,7 @@ struct Rows {
         for (int b = 0; b < kPix; ++b) {
             const float2 dy = add2(make_float2(xy.z, xy.w), minus_y[b]);
             const float2 e = fma2(fma2(c, dy, bdx), dy, adx2);
-            w[b] = make_float2((held[b] & 1) && e.x <= 0.f ? exp2_approx(e.x) : 0.f, (held[b] & 2) && e.y <= 0.f ? exp2_approx(e.y) : 0.f);
+            w[b] = make_float2((held[b] & 1) ? exp2_approx(e.x) : 0.f, (held[b] & 2) ? exp2_approx(e.y) : 0.f);
         }
     }
     static __device__ __forceinline__ float2 value(const float4 *pair, const int c) {
@@ -306,10 +312,16 @@ struct Rows {
     }
 };
 
-// Host checks of the sizes, shared by the entry points: slots and Gaussians' sums indexed with 32 bits, coordinates exact in float
-constexpr const char *kListsLimit = "at most 2^31 / 10 pixels, 2^24 pixels a side and 2^26 Gaussians";
+// 1 / x to 2 ulp
+__device__ __forceinline__ float reciprocal(const float x) { return __fdividef(1.f, x); }
+
+// Host checks of the sizes, shared by the entry points: slots and Gaussians' sums indexed with 32 bits, coordinates exact in float, tiles
+// within a grid
+constexpr const char *kListsLimit = "at most 2^31 / 10 pixels, 65535 tiles a side and 2^26 Gaussians";
 inline bool lists_addressable(int img_height, int img_width, int num_points) {
-    return (int64_t)img_height * img_width <= INT32_MAX / kTopK && img_height <= 1 << 24 && img_width <= 1 << 24 && num_points <= 1 << 26;
+    return (int64_t)img_height * img_width <= INT32_MAX / kTopK && img_height <= 65535 * kTile && img_width <= 65535 * kTile &&
+           num_points <= 1 << 26;
 }
+inline dim3 tile_grid(int img_height, int img_width) { return dim3(ceil_div(img_width, kTile), ceil_div(img_height, kTile)); }
 
 }  // namespace igs

@@ -17,10 +17,8 @@
 
 namespace igs {
 
-constexpr int kWeightPitch = kPatchPixels + 4;  // words: the reads of four pixels by eight lanes (rows) fall on distinct banks
-
 struct SumArgs {
-    int tiles_x, img_h, img_w, channels, n;
+    int img_h, img_w, channels, n;
     const float *xys, *conics;
     const int *pixel_topk;
     const uint8_t *mask;         // balance: pixels that count (NULL: all)
@@ -49,7 +47,7 @@ struct SumSmem {
         };
         float4 pairs[Rows<C>::kGroupQuads];
         alignas(16) float pixel[C + 1][kPatchPixels];  // v'_c, m'
-    } warp[kWarps];
+    } warp[kPatches];
 };
 
 // Value c of a Gaussian's score
@@ -124,14 +122,15 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ SumAr
 }
 
 template <int C, bool kDropout>
-__global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : C <= 7 ? 4 : 3) sums_kernel(const __grid_constant__ SumArgs a) {
-    constexpr int kValues = SumLayout<C, kDropout>::kValues;
-    constexpr int kPairQuads = Rows<C>::kPairQuads;
+__global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4)
+    sums_kernel(const __grid_constant__ SumArgs a) {
+    using Rows = igs::Rows<C>;
+    constexpr int kValues = SumLayout<C, kDropout>::kValues, kPairQuads = Rows::kPairQuads;
     extern __shared__ __align__(16) char smem_bytes[];
     const int lane = threadIdx.x & 31;
     typename SumSmem<C, kDropout>::Warp &sm = reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes)->warp[threadIdx.x >> 5];
     wait_for_predecessor();
-    const Patch patch = patch_of(a.tiles_x, a.img_h, a.img_w);
+    const Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
     const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
     float2 minus_y[kPix], total2[kPix], scores2[kPix];
@@ -144,14 +143,14 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : C <= 7 ? 4 : 3) su
     const float x0 = (float)patch.x0, y0 = (float)(patch.y0 + half * (kLines / 2));
     bool regular = true, have_totals = false;
     for (int g = 0;;) {
-        const PatchRows rows =
-            find_rows(a.pixel_topk, patch, a.n, [&](const int p, const bool inside) { return sum_slots<kDropout>(a, p, inside); }, g, sm.keys);
+        const PatchRows rows = find_rows(
+            a.pixel_topk, patch, a.n, [&](const int p, const bool inside) { return sum_slots<kDropout>(a, p, inside); }, g, sm.keys);
         float v[kPix][C];
 #pragma unroll
         for (int b = 0; b < kPix; ++b)
 #pragma unroll
             for (int c = 0; c < C; ++c) v[b][c] = patch.inside[b] && !have_totals ? pixel_value<kDropout>(a, patch.p[b], c) : 0.f;
-        regular = Rows<C>::gather(a.rows, rows, sm.pairs) && regular;
+        regular = Rows::gather(a.rows, rows, sm.pairs) && regular;
         __syncwarp();
         // a lane is kPix pixels: the group's weights, and the sums over all groups
         unsigned held[kPix];
@@ -162,14 +161,14 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : C <= 7 ? 4 : 3) su
             const float4 *q = sm.pairs + pair * kPairQuads;
             float *weight = sm.weight + 2 * pair * kWeightPitch + lane;
             float2 w[kPix];
-            Rows<C>::weights(q, held, minus_x, minus_y, w);
+            Rows::weights(q, held, minus_x, minus_y, w);
 #pragma unroll
             for (int b = 0; b < kPix; ++b) {
                 held[b] >>= 2;
                 weight[32 * b] = w[b].x, weight[kWeightPitch + 32 * b] = w[b].y;
                 float2 score = make_float2(0.f, 0.f);  // (unused the second time)
 #pragma unroll
-                for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(q, c), make_float2(v[b][c], v[b][c]), score);
+                for (int c = 0; c < C; ++c) score = fma2(Rows::value(q, c), make_float2(v[b][c], v[b][c]), score);
                 total2[b] = add2(total2[b], w[b]);
                 scores2[b] = fma2(w[b], score, scores2[b]);
             }
@@ -184,7 +183,7 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : C <= 7 ? 4 : 3) su
             for (int b = 0; b < kPix; ++b) {
                 const float total = total2[b].x + total2[b].y, scores = scores2[b].x + scores2[b].y;
                 const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
-                const float inv = 1.f / (total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
+                const float inv = reciprocal(total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
                 float size = fabsf(m);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
@@ -316,7 +315,7 @@ void launch_sums(SumArgs a, void *workspace, const bool accumulate, float *v_xy,
     if (a.img_h > 0 && a.img_w > 0) {
         // past 48 KB the kernel has to be told; the setting belongs to the device, so every call makes it
         if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        launch(sums_kernel<C, kDropout>, dim3(a.tiles_x * ceil_div(a.img_h, kTile)), dim3(kPatchThreads), kBytes, s, a);
+        launch(sums_kernel<C, kDropout>, tile_grid(a.img_h, a.img_w), dim3(kPatchThreads), kBytes, s, a);
     }
     launch(finish_sums_kernel<kValues>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a.n, a.channels, a.conics, (const float *)a.sums,
            accumulate, v_xy, v_conic, v_colors);
