@@ -110,7 +110,6 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
     float2 minus_y[kPix], total[kPix];
 #pragma unroll
     for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), total[b] = make_float2(0.f, 0.f);
-    const int half = lane >> 4;
     bool regular = true, have_total = false;
     for (int g = 0;;) {
         const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
@@ -154,21 +153,20 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
             }
         }
         __syncwarp();
-#pragma unroll 1
-        for (int first = 0; first < rows.n; first += 16) {
-            const int r = first + (lane & 15);
-            float sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < kPatchPixels / 8; ++q) {
-                const int at = half * (kPatchPixels / 2) + q * 4;
-                const float4 w = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + at]);
-                const float4 inv = *reinterpret_cast<const float4 *>(&sm.inv[at]);
-                sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            const int id = __shfl_sync(0xffffffffu, rows.id, r);
-            if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
+        // a lane is a row or, up to 16 rows, half of one
+        const bool halves = rows.n <= 16;
+        const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
+        const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *inv_at = sm.inv + half * (kPatchPixels / 2);
+        float sum = 0.f;
+#pragma unroll 4
+        for (int q = 0; q < (halves ? kPatchPixels / 8 : kPatchPixels / 4); ++q, w_at += 4, inv_at += 4) {
+            const float4 w = *reinterpret_cast<const float4 *>(w_at);
+            const float4 inv = *reinterpret_cast<const float4 *>(inv_at);
+            sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
         }
+        const int id = __shfl_sync(0xffffffffu, rows.id, r);
+        if (halves) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
         if (lane < rows.n) atomicAdd(&a.counts[rows.id], rows.holders);
         if (!rows.more) return;
         ++g;

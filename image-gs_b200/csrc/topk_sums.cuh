@@ -139,8 +139,6 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4)
         minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]);
         total2[b] = make_float2(0.f, 0.f), scores2[b] = make_float2(0.f, 0.f);
     }
-    const int half = lane >> 4;
-    const float x0 = (float)patch.x0, y0 = (float)(patch.y0 + half * (kLines / 2));
     bool regular = true, have_totals = false;
     for (int g = 0;;) {
         const PatchRows rows = find_rows(
@@ -206,65 +204,65 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4)
             }
         }
         __syncwarp();
-        // a lane is half a row
+        // a lane is a row or, up to 16 rows, half of one
+        const bool halves = rows.n <= 16;
+        const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
+        const int lines = halves ? kLines / 2 : kLines;
+        const float *mine = reinterpret_cast<const float *>(sm.pairs + (r >> 1) * kPairQuads) + (r & 1);
+        auto field = [&](const int e) { return mine[2 * e]; };
+        const float x = field(0) - (float)patch.x0;
+        float dy = field(1) - (float)(patch.y0 + half * lines);
+        float2 dx[4], f[C], color[C];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dx[e] = make_float2(x - (float)(2 * e), x - (float)(2 * e + 1));
+#pragma unroll
+        for (int c = 0; c < C; ++c) f[c].x = -field(5 + c), f[c].y = f[c].x, color[c] = make_float2(0.f, 0.f);
+        float2 xx = make_float2(0.f, 0.f);
+        float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
+        const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *v_at = &sm.pixel[0][half * (kPatchPixels / 2)];
 #pragma unroll 1
-        for (int first = 0; first < rows.n; first += 16) {
-            asm volatile("" ::: "memory");  // the pixels' values stay in shared memory: carried over this loop, they would spill
-            const int r = first + (lane & 15);
-            const float *mine = reinterpret_cast<const float *>(sm.pairs + (r >> 1) * kPairQuads) + (r & 1);
-            auto field = [&](const int e) { return mine[2 * e]; };
-            const float x = field(0), y = field(1);
-            float2 dx[4], f[C], color[C];
+        for (int line = 0; line < lines; ++line, dy -= 1.f, w_at += 8, v_at += 8) {
+            float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dx[e] = make_float2(x - (x0 + (float)(2 * e)), x - (x0 + (float)(2 * e + 1)));
+            for (int quad = 0; quad < 2; ++quad) {
+                const float4 w4 = *reinterpret_cast<const float4 *>(w_at + quad * 4);
+                const float4 m4 = *reinterpret_cast<const float4 *>(v_at + C * kPatchPixels + quad * 4);
+                float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
+                const float2 w0 = make_float2(w4.x, w4.y), w1 = make_float2(w4.z, w4.w);
 #pragma unroll
-            for (int c = 0; c < C; ++c) f[c].x = -field(5 + c), f[c].y = f[c].x, color[c] = make_float2(0.f, 0.f);
-            float2 xx = make_float2(0.f, 0.f);
-            float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
-#pragma unroll 1
-            for (int line = 0; line < kLines / 2; ++line) {
-                float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
-#pragma unroll
-                for (int quad = 0; quad < 2; ++quad) {
-                    const int at = half * (kPatchPixels / 2) + line * 8 + quad * 4;
-                    const float4 w4 = *reinterpret_cast<const float4 *>(&sm.weight[r * kWeightPitch + at]);
-                    const float4 m4 = *reinterpret_cast<const float4 *>(&sm.pixel[C][at]);
-                    float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
-                    const float2 w0 = make_float2(w4.x, w4.y), w1 = make_float2(w4.z, w4.w);
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const float4 v4 = *reinterpret_cast<const float4 *>(&sm.pixel[c][at]);
-                        const float2 v0 = make_float2(v4.x, v4.y), v1 = make_float2(v4.z, v4.w);
-                        d0 = fma2(f[c], v0, d0), d1 = fma2(f[c], v1, d1);
-                        if constexpr (kDropout) color[c] = fma2(w1, v1, fma2(w0, v0, color[c]));
-                    }
-                    const float2 t0 = mul2(w0, d0), t1 = mul2(w1, d1);
-                    const float2 u0 = mul2(t0, dx[2 * quad]), u1 = mul2(t1, dx[2 * quad + 1]);
-                    ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
-                    xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
+                for (int c = 0; c < C; ++c) {
+                    const float4 v4 = *reinterpret_cast<const float4 *>(v_at + c * kPatchPixels + quad * 4);
+                    const float2 v0 = make_float2(v4.x, v4.y), v1 = make_float2(v4.z, v4.w);
+                    d0 = fma2(f[c], v0, d0), d1 = fma2(f[c], v1, d1);
+                    if constexpr (kDropout) color[c] = fma2(w1, v1, fma2(w0, v0, color[c]));
                 }
-                const float dy = y - (y0 + (float)line);
-                const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
-                sx += ur, sy += ty;
-                sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
+                const float2 t0 = mul2(w0, d0), t1 = mul2(w1, d1);
+                const float2 u0 = mul2(t0, dx[2 * quad]), u1 = mul2(t1, dx[2 * quad + 1]);
+                ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
+                xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
             }
-            float sum[kValues];
+            const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
+            sx += ur, sy += ty;
+            sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
+        }
+        float sum[kValues];
 #pragma unroll
-            for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
-            sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
-            if constexpr (kDropout) {
+        for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
+        sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
+        if constexpr (kDropout) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
-            }
+            for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
+        }
+        const int id = __shfl_sync(0xffffffffu, rows.id, r);
+        if (halves) {
 #pragma unroll
             for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
-            const int id = __shfl_sync(0xffffffffu, rows.id, r);
-            if (r < rows.n) {
-                float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)id * kValues);
+        }
+        if (r < rows.n) {
+            float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)id * kValues);
 #pragma unroll
-                for (int e = 0; e < kValues / 4; ++e)
-                    if ((e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
-            }
+            for (int e = 0; e < kValues / 4; ++e)
+                if (!halves || (e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
         }
         if (!rows.more) return;
         ++g;
