@@ -240,7 +240,7 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     IGS_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(num_points), "igs_topk_balance_fwd: workspace too small");
     IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_balance_fwd: workspace must be 16-byte aligned");
     const int pixels = img_height * img_width;
-    IGS_REQUIRE(pixels == 0 || num_points == 0 || (xys && conics && pixel_topk), "igs_topk_balance_fwd: null pointer");
+    IGS_REQUIRE(num_points == 0 || (xys && conics && (pixels == 0 || pixel_topk)), "igs_topk_balance_fwd: null pointer");
     IGS_REQUIRE(igs::aligned(pixel_topk, 8), "igs_topk_balance_fwd: pixel_topk must be 8-byte aligned");
     cudaStream_t s = igs::as_stream(stream);
     char *base = static_cast<char *>(workspace);

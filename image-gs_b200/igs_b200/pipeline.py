@@ -7,6 +7,8 @@ path of Image-GS's CUDA-graph step (model.py:1160-1209) for the hot path only:
 
 The top-K forward, the L1 loss with its gradient and the top-K backward run as one kernel per tile (igs_raster_step_l1), so the top-K
 lists and the image gradient never go through HBM; fused=False runs them as the separate forward (with the loss) and backward kernels.
+With gate dropout or the balance term the step keeps the [H, W, 10] lists and runs from them: lists -> [dropout render] -> L1 loss +
+gradient -> backward from the lists [-> balance term forward/backward].
 
 The intersection buffers hold `capacity` entries (capacity_ratio times the count of the first step, at least 1024, as model.py:110,1186),
 so nothing is read back to the host inside the step; the true count is kept on the device (num_intersects) for overflow checks.
@@ -28,11 +30,18 @@ class RasterStep:
 
     def __init__(self, means, scales, rotations, features, target, capacity: Optional[int] = None, capacity_ratio: float = 2.0,
                  l1_ratio: float = 1.0, quant: Optional[dict] = None, loss_transform=None, rate: Optional[dict] = None,
-                 fused: bool = True):
+                 fused: bool = True, balance: Optional[dict] = None, gate_dropout: Optional[dict] = None):
         """quant: dict(pos_steps [2], scale_step, rot_step, feat_steps [C]) puts the straight-through quantizer in front (scales must be
         the canonical, non-negative ones); loss_transform [C,C]: render feat T^T (YUV loss space, needs quant); rate: dict(model (the
         fields of compress.rate.RateModel), inv_rot_step, factor) adds the rate term on the raw features and rotations. fused=False:
-        separate forward and backward kernels, with the top-K lists and the image gradient (v_image) kept in HBM."""
+        separate forward and backward kernels, with the top-K lists and the image gradient (v_image) kept in HBM.
+        balance: dict(factor, mask (optional, [H,W] bool or uint8)) adds the gradient of factor * the balance loss of the pixels over the
+        Gaussians to the geometry's; the loss itself, the counts and the importance are in balance_loss, counts and importance.
+        gate_dropout: dict(p, rng_state (int64 [2] on the device: seed and offset)) renders with gates dropped; the step ends by moving the
+        offset on by one, so that every launch and every replay draws another mask. Both run from the [H, W, 10] lists, not fused."""
+        self.balance, self.gate_dropout = balance, gate_dropout
+        self.lists = balance is not None or gate_dropout is not None
+        fused = fused and not self.lists
         self.fused = fused
         self.lib = _lib.load()
         self.device = means.device
@@ -89,7 +98,7 @@ class RasterStep:
         self.max_list = min(self.n, self.capacity)
         # top-K lists in the 16-bit tile-list form between the separate kernels (tiles with 65535+ entries are selected again by the
         # backward pass)
-        self.topk = None if fused else torch.empty(self.num_tiles, TOP_K, TILE * TILE, device=dev, dtype=torch.int16)
+        self.topk = None if fused or self.lists else torch.empty(self.num_tiles, TOP_K, TILE * TILE, device=dev, dtype=torch.int16)
         # the fused step's workspace (igs_train_step_l1: the stages below in one call, eight kernels, no memset)
         self.step_ws_bytes = self.lib.igs_train_step_workspace(n, self.capacity, self.tb[0], self.tb[1])
         self.step_ws = torch.empty(self.step_ws_bytes, device=dev, dtype=torch.uint8) if fused else None
@@ -105,6 +114,32 @@ class RasterStep:
             self.rate_ws = torch.zeros(self.rate_ws_bytes, device=dev, dtype=torch.uint8)
             self.rate_refs = ((ctypes.c_int32 * nc)(*m.color_refs), (ctypes.c_int32 * nc)(*m.pred_channels))
             self.grad_one = torch.ones((), device=dev, dtype=f32)
+        if self.lists:
+            self.pixel_topk = torch.empty(self.h, self.w, TOP_K, device=dev, dtype=i32)
+            self.image_ws_bytes = self.lib.igs_l1_workspace(self.image.numel())
+            self.image_ws = torch.zeros(self.image_ws_bytes, device=dev, dtype=torch.uint8)
+        if self.gate_dropout is not None:
+            self.drop_p, self.rng_state = float(self.gate_dropout["p"]), self.gate_dropout["rng_state"]
+            if not 0.0 <= self.drop_p <= 1.0:
+                raise ValueError(f"p must lie in [0, 1], got {self.drop_p}")
+            if self.rng_state.dtype != torch.int64 or self.rng_state.numel() != 2 or self.rng_state.device != dev:
+                raise ValueError(f"rng_state must be two int64 values on {dev}")
+            self.rng_used = torch.empty(2, device=dev, dtype=torch.int64)
+            self.drop_ws_bytes = self.lib.igs_topk_dropout_workspace(n, nc)
+            self.drop_ws = torch.empty(self.drop_ws_bytes, device=dev, dtype=torch.uint8)
+        if self.balance is not None:
+            self.mask = self.balance.get("mask")
+            if self.mask is not None:
+                if self.mask.dtype not in (torch.bool, torch.uint8) or tuple(self.mask.shape) != (self.h, self.w) or self.mask.device != dev:
+                    raise ValueError(f"the balance mask must be [{self.h}, {self.w}] bool or uint8 on {dev}")
+                self.mask = self.mask.contiguous()
+            self.balance_factor = torch.full((), float(self.balance["factor"]), device=dev, dtype=f32)
+            self.balance_loss = torch.empty((), device=dev, dtype=f32)
+            self.counts = torch.empty(n, device=dev, dtype=i32)
+            self.importance = torch.empty(n, device=dev, dtype=f32)
+            self.totals = torch.empty(2, device=dev, dtype=torch.int64)
+            self.balance_ws_bytes = self.lib.igs_topk_balance_workspace(n)
+            self.balance_ws = torch.empty(self.balance_ws_bytes, device=dev, dtype=torch.uint8)
         if self.transform is not None or self.rate is not None:
             self.v_feat = torch.empty_like(features)  # gradient of the raw features
         self.graph = None
@@ -180,6 +215,48 @@ class RasterStep:
                                                        ptr(self.conics), ptr(self.features), ptr(self.v_image), ptr(self.topk), ptr(self.v_xy),
                                                        ptr(self.v_conic), ptr(self.v_colors), self._stream()), "backward")
 
+    def _lists_forward(self):
+        """The top-K lists as IDs, with the render unless it is the dropout's."""
+        channels = self.c if self.gate_dropout is None else 0
+        self._check(self.lib.igs_raster_fwd_topk(self.tb[0], self.tb[1], self.h, self.w, channels, ptr(self.ids), ptr(self.bins),
+                                                 ptr(self.xys), ptr(self.conics), ptr(self.features), ptr(self.image),
+                                                 ptr(self.pixel_topk), self._stream()), "lists")
+
+    def _dropout_forward(self):
+        self._check(self.lib.igs_topk_dropout_fwd(self.h, self.w, self.c, self.n, ptr(self.xys), ptr(self.conics), ptr(self.features),
+                                                  ptr(self.pixel_topk), self.drop_p, ptr(self.rng_state), ptr(self.image),
+                                                  ptr(self.rng_used), ptr(self.drop_ws), self.drop_ws_bytes, self._stream()),
+                    "dropout forward")
+
+    def _image_loss(self):
+        self._check(self.lib.igs_l1_loss(self.image.numel(), ptr(self.image), ptr(self.target), self.l1_ratio, ptr(self.loss),
+                                         ptr(self.v_image), ptr(self.image_ws), self.image_ws_bytes, self._stream()), "image loss")
+
+    def _dropout_backward(self):
+        self._check(self.lib.igs_topk_dropout_bwd(self.h, self.w, self.c, self.n, ptr(self.xys), ptr(self.conics), ptr(self.features),
+                                                  ptr(self.v_image), ptr(self.pixel_topk), self.drop_p, ptr(self.rng_used), ptr(self.v_xy),
+                                                  ptr(self.v_conic), ptr(self.v_colors), ptr(self.drop_ws), self.drop_ws_bytes,
+                                                  self._stream()), "dropout backward")
+
+    def _lists_backward(self):
+        self._check(self.lib.igs_raster_bwd_topk(self.h, self.w, self.c, self.n, ptr(self.xys), ptr(self.conics), ptr(self.features),
+                                                 ptr(self.v_image), ptr(self.pixel_topk), ptr(self.v_xy), ptr(self.v_conic),
+                                                 ptr(self.v_colors), self._stream()), "backward from the lists")
+
+    def _balance_term(self):
+        """The balance loss, and factor times its gradient added to v_xy and v_conic."""
+        self._check(self.lib.igs_topk_balance_fwd(self.h, self.w, self.n, ptr(self.xys), ptr(self.conics), ptr(self.pixel_topk),
+                                                  ptr(self.mask), ptr(self.balance_loss), ptr(self.counts), ptr(self.importance),
+                                                  ptr(self.totals), ptr(self.balance_ws), self.balance_ws_bytes, self._stream()),
+                    "balance forward")
+        self._check(self.lib.igs_topk_balance_bwd(self.h, self.w, self.n, ptr(self.xys), ptr(self.conics), ptr(self.pixel_topk),
+                                                  ptr(self.mask), ptr(self.counts), ptr(self.totals), ptr(self.balance_factor), None, 1,
+                                                  ptr(self.v_xy), ptr(self.v_conic), ptr(self.balance_ws), self.balance_ws_bytes,
+                                                  self._stream()), "balance backward")
+
+    def _next_mask(self):
+        self.rng_state[1:].add_(1)
+
     def _project_backward(self):
         self._check(self.lib.igs_project_bwd(self.n, ptr(self.scales), ptr(self.rotations), self.h, self.w, ptr(self.radii), ptr(self.conics),
                                              ptr(self.v_xy), ptr(self.v_conic), ptr(self.v_cov2d), ptr(self.v_mean2d), ptr(self.v_scale),
@@ -197,12 +274,18 @@ class RasterStep:
 
     # kernels each stage launches (memsets excluded)
     KERNELS = {"_quantize": 1, "_project": 1, "_cumsum": 2, "_bin": 4, "_raster": 2, "_forward": 2, "_backward": 1, "_project_backward": 1,
-               "_rate_term": 2, "_feature_grads": 1, "_train_step": 8}
+               "_rate_term": 2, "_feature_grads": 1, "_train_step": 8, "_lists_forward": 1, "_dropout_forward": 2, "_image_loss": 1,
+               "_dropout_backward": 3, "_lists_backward": 1, "_balance_term": 6, "_next_mask": 0}
 
     @property
     def BREAKDOWN_STAGES(self):
         """The step's stages as separate calls (the fused step's kernels, one stage at a time, for per-stage timing)."""
-        raster = ("_raster",) if self.fused else ("_forward", "_backward")
+        if self.lists:
+            raster = (("_lists_forward", "_dropout_forward", "_image_loss", "_dropout_backward") if self.gate_dropout is not None
+                      else ("_lists_forward", "_image_loss", "_lists_backward"))
+            raster += ("_balance_term",) if self.balance is not None else ()
+        else:
+            raster = ("_raster",) if self.fused else ("_forward", "_backward")
         return ("_project", "_cumsum", "_bin") + raster + ("_project_backward",)
 
     @property
@@ -216,6 +299,8 @@ class RasterStep:
             stages += ("_rate_term",)
         if self.rate is not None or self.transform is not None:
             stages += ("_feature_grads",)
+        if self.gate_dropout is not None:
+            stages += ("_next_mask",)
         return stages
 
     def launch(self):

@@ -115,6 +115,7 @@ def test_entry_points_refuse_invalid_arguments():
     refused(fwd(size=lib.igs_topk_balance_workspace(3) - 1), "workspace")
     refused(fwd(ws=odd), "aligned")
     refused(fwd(topk=null), "null")
+    refused(fwd(h=0, xys=null), "null")  # the Gaussians are read without pixels too
     refused(fwd(topk=ctypes.c_void_p(260)), "aligned")
     bwd = lambda h=4, n=3, counts=fake, ws=fake, size=big: lib.igs_topk_balance_bwd(  # noqa: E731
         h, 4, n, fake, fake, fake, null, counts, fake, null, null, 0, fake, fake, ws, size, null)
@@ -122,6 +123,7 @@ def test_entry_points_refuse_invalid_arguments():
     refused(bwd(counts=null), "null")
     refused(bwd(ws=odd), "aligned")
     refused(bwd(size=lib.igs_topk_balance_workspace(3) - 1), "workspace")
+    assert lib.igs_topk_balance_bwd(0, 4, 3, null, fake, null, null, fake, fake, null, null, 0, fake, fake, fake, big, null) == 1
     assert bwd(n=0) == 0
     drop = lambda h=4, c=3, n=3, p=0.1, topk=fake, rng=fake, ws=fake, size=big: lib.igs_topk_dropout_fwd(  # noqa: E731
         h, 4, c, n, fake, fake, fake, topk, p, rng, fake, fake, ws, size, null)
@@ -141,6 +143,7 @@ def test_entry_points_refuse_invalid_arguments():
     refused(back(v=null), "null output")
     refused(back(ws=null), "workspace")
     refused(back(size=lib.igs_topk_dropout_workspace(3, 3) - 1), "workspace")
+    assert lib.igs_topk_dropout_bwd(0, 4, 3, 3, null, fake, fake, fake, fake, 0.1, fake, fake, fake, fake, fake, big, null) == 1
     assert back(n=0) == 0
 
 
