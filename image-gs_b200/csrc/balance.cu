@@ -28,13 +28,12 @@ struct BalanceWorkspace {
     unsigned int ticket;
     unsigned int pad;
     unsigned long long routed[kRoutedSlots];  // T, over this many words, so that no one word takes every patch's atomic
-    // then uint64 fixed [n], float4 rows [n, 2], double partials [blocks of the finish kernel]
+    // then uint64 fixed [n], double partials [blocks of the finish kernel]
 };
 
 int finish_blocks(int n) { return n > 0 ? igs::ceil_div(n, kThreads) : 1; }
 size_t forward_bytes(int n) {
-    return sizeof(BalanceWorkspace) + (sizeof(unsigned long long) + sizeof(float4) * Rows::kQuads) * (size_t)n + 8 +
-           sizeof(double) * (size_t)finish_blocks(n);
+    return sizeof(BalanceWorkspace) + sizeof(unsigned long long) * (size_t)n + sizeof(double) * (size_t)finish_blocks(n);
 }
 size_t workspace_bytes_of(int n) { return std::max(forward_bytes(n), igs::sum_bytes<1, false>(n)); }
 
@@ -53,19 +52,15 @@ struct BalanceArgs {
     float scale;  // 2^fraction bits
     int *counts;
     unsigned long long *fixed;
-    float4 *rows;
     BalanceWorkspace *ws;
 };
 
-// The rows of all Gaussians (topk_lists.cuh), and what the patches add to zeroed
-__global__ void __launch_bounds__(kThreads) balance_rows_kernel(const __grid_constant__ BalanceArgs a) {
+__global__ void __launch_bounds__(kThreads) balance_zero_kernel(const __grid_constant__ BalanceArgs a) {
     igs::wait_for_predecessor();
     const int id = blockIdx.x * kThreads + threadIdx.x;
     if (id == 0) a.ws->filled = 0, a.ws->ticket = 0;
     if (id < kRoutedSlots) a.ws->routed[id] = 0;
-    if (id >= a.n) return;
-    a.counts[id] = 0, a.fixed[id] = 0;
-    Rows::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), {0.f});
+    if (id < a.n) a.counts[id] = 0, a.fixed[id] = 0;
 }
 
 // One pixel's slots one by one, from global memory (topk_sums.cuh says when)
@@ -113,7 +108,7 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
     bool regular = true, have_total = false;
     for (int g = 0;;) {
         const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
-        regular = Rows::gather(a.rows, rows, sm.pairs) && regular;
+        regular = Rows::gather(rows, a.xys, a.conics, [](int, int) { return 0.f; }, sm.pairs) && regular;
         __syncwarp();
         unsigned held[kPix];
 #pragma unroll
@@ -246,13 +241,12 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     char *base = static_cast<char *>(workspace);
     BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(base);
     unsigned long long *fixed = reinterpret_cast<unsigned long long *>(base + sizeof(BalanceWorkspace));
-    float4 *rows = reinterpret_cast<float4 *>(fixed + (num_points + 1) / 2 * 2);
-    double *partials = reinterpret_cast<double *>(rows + (size_t)Rows::kQuads * num_points);
+    double *partials = reinterpret_cast<double *>(fixed + num_points);
     const int bits = fraction_bits(pixels);
     const int blocks = finish_blocks(num_points);
     const BalanceArgs a = {img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
-                           (float)((int64_t)1 << bits), counts, fixed, rows, ws};
-    igs::launch(balance_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
+                           (float)((int64_t)1 << bits), counts, fixed, ws};
+    igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
     if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
     igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
                 (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,

@@ -14,8 +14,6 @@ using igs::kPix;
 using igs::kTile;
 using igs::kTopK;
 
-constexpr int kLayOutTiles = 1024;
-
 struct DropoutArgs {
     int img_h, img_w, channels, n;
     const float *xys, *conics, *colors;
@@ -24,7 +22,6 @@ struct DropoutArgs {
     const long long *rng;
     float *out_img;
     long long *rng_used;
-    float4 *rows;  // of all Gaussians, or NULL
 };
 
 // One pixel's slots one by one, from global memory
@@ -49,18 +46,6 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p) {
         }
         out[c * plane] = pix / total;
     }
-}
-
-// The rows of all Gaussians (topk_lists.cuh)
-template <int C>
-__global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant__ DropoutArgs a) {
-    igs::wait_for_predecessor();
-    const int id = blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.n) return;
-    float f[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) f[c] = c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
-    igs::Rows<C>::store(a.rows, id, igs::row_geometry(a.xys, a.conics, id), f);
 }
 
 // A warp is a patch, a lane its pixels
@@ -90,13 +75,8 @@ __global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 
     }
     for (int g = 0;; ++g) {
         const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
-        const bool regular = Rows::gather(a.rows, rows, sm.pairs, [&](const int id, float(&q)[4 * Rows::kQuads]) {
-            const igs::RowGeometry r = igs::row_geometry(a.xys, a.conics, id);
-            q[0] = r.regular ? r.x : __int_as_float(0x7fc00000), q[1] = r.y, q[2] = r.a, q[3] = r.b, q[4] = r.c;
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (c < a.channels) q[5 + c] = __ldg(&a.colors[(size_t)id * a.channels + c]);
-        });
+        const bool regular = Rows::gather(
+            rows, a.xys, a.conics, [&](const int id, const int c) { return __ldg(&a.colors[(size_t)id * C + c]); }, sm.pairs);
         if (!regular) {  // among others, zero times a colour that is not finite would reach pixels that do not name it
 #pragma unroll 1
             for (int b = 0; b < kPix; ++b)
@@ -129,7 +109,7 @@ __global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 
         const float inv = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (c < a.channels) a.out_img[c * plane + patch.p[b]] = (pix[b][c].x + pix[b][c].y) * inv;
+            a.out_img[c * plane + patch.p[b]] = (pix[b][c].x + pix[b][c].y) * inv;
     }
 }
 
@@ -149,8 +129,8 @@ void with_channels(const int channels, F f) {
 
 size_t workspace_bytes_of(int num_points, int channels) {
     size_t bytes = 0;
-    with_channels(channels, [&](auto width) { bytes = igs::sum_bytes<decltype(width)::value, true>(num_points); });
-    return bytes + 16;  // never nothing
+    with_channels(channels, [&](auto count) { bytes = igs::sum_bytes<decltype(count)::value, true>(num_points); });
+    return bytes;
 }
 
 }  // namespace
@@ -163,13 +143,11 @@ size_t igs_topk_dropout_workspace(int num_points, int channels) {
 
 int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
                          const float *colors, const int32_t *pixel_topk, double p, const int64_t *rng_state, float *out_img,
-                         int64_t *rng_used, void *workspace, size_t workspace_bytes, void *stream) {
+                         int64_t *rng_used, void *stream) {
     IGS_REQUIRE(img_height >= 0 && img_width >= 0 && num_points >= 0, "igs_topk_dropout_fwd: negative size");
     IGS_REQUIRE(channels >= 1 && channels <= kMaxChannels, "igs_topk_dropout_fwd: 1 to %d channels", kMaxChannels);
     IGS_REQUIRE(igs::lists_addressable(img_height, img_width, num_points), "igs_topk_dropout_fwd: %s", igs::kListsLimit);
     IGS_REQUIRE(p >= 0.0 && p <= 1.0, "igs_topk_dropout_fwd: p must lie in [0, 1]");
-    IGS_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(num_points, channels), "igs_topk_dropout_fwd: workspace too small");
-    IGS_REQUIRE(igs::aligned(workspace, 16), "igs_topk_dropout_fwd: workspace must be 16-byte aligned");
     IGS_REQUIRE(rng_state && rng_used, "igs_topk_dropout_fwd: null rng state");
     const int pixels = img_height * img_width;
     IGS_REQUIRE(pixels == 0 || (pixel_topk && out_img && (num_points == 0 || (xys && conics && colors))),
@@ -181,15 +159,10 @@ int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_po
     if (pixels == 0) {
         igs::launch(rng_used_kernel, dim3(1), dim3(1), 0, s, rng, used);
     } else {
-        const dim3 grid = igs::tile_grid(img_height, img_width);
-        // laying the rows out is a launch of its own, which a small image does not repay
-        const bool lay_out = num_points > 0 && grid.x * grid.y > kLayOutTiles;
         const DropoutArgs a = {img_height, img_width, channels, num_points, xys, conics, colors, pixel_topk,
-                               (uint32_t)rint(p * 16777216.0), rng, out_img, used, lay_out ? static_cast<float4 *>(workspace) : nullptr};
-        with_channels(channels, [&](auto width) {
-            constexpr int kWidth = decltype(width)::value;
-            if (lay_out) igs::launch(dropout_rows_kernel<kWidth>, dim3(igs::ceil_div(num_points, 256)), dim3(256), 0, s, a);
-            igs::launch(dropout_kernel<kWidth>, grid, dim3(igs::kPatchThreads), 0, s, a);
+                               (uint32_t)rint(p * 16777216.0), rng, out_img, used};
+        with_channels(channels, [&](auto count) {
+            igs::launch(dropout_kernel<decltype(count)::value>, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
         });
     }
     return igs::check_launch("igs_topk_dropout_fwd");
@@ -214,8 +187,8 @@ int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_po
     a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
     a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
     a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0);
-    with_channels(channels, [&](auto width) {
-        igs::launch_sums<decltype(width)::value, true>(a, workspace, false, v_xy, v_conic, v_colors, s);
+    with_channels(channels, [&](auto count) {
+        igs::launch_sums<decltype(count)::value, true>(a, workspace, false, v_xy, v_conic, v_colors, s);
     });
     return igs::check_launch("igs_topk_dropout_bwd");
 }

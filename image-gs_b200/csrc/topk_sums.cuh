@@ -22,17 +22,17 @@ struct SumArgs {
     const float *xys, *conics;
     const int *pixel_topk;
     const uint8_t *mask;         // balance: pixels that count (NULL: all)
-    const int *counts;           // balance: alpha = v_loss N / (A T) counts + v_importance
+    const int *counts;           // balance: alpha = *scale counts + v_importance, *scale = v_loss N / (A T)
     const long long *totals;
     const float *v_loss, *v_importance;
+    float *scale;
     const float *colors, *v_output;  // dropout
     const long long *rng;
     uint32_t threshold;
-    float4 *rows;                // all Gaussians' rows
     float *sums;                 // [N, SumLayout::kValues]
 };
 
-// C: the values per row and pixel (1 for balance; 3, 7, 11 or 12 channels, the unused ones zero)
+// C: the values per row and pixel (balance: 1; dropout: the channels)
 template <int C, bool kDropout>
 struct SumLayout {
     static constexpr int kValues = ((5 + (kDropout ? C : 0)) + 3) / 4 * 4;  // Sx, Sy, Sxx, Sxy, Syy, S_c
@@ -53,14 +53,13 @@ struct SumSmem {
 // Value c of a Gaussian's score
 template <bool kDropout>
 __device__ __forceinline__ float row_value(const SumArgs &a, const int id, const int c) {
-    if constexpr (kDropout) return c < a.channels ? __ldg(&a.colors[(size_t)id * a.channels + c]) : 0.f;
-    const double slots = (double)a.totals[0], pixels = (double)a.totals[1];
-    const float scale = a.v_loss != nullptr && slots > 0.0 ? (float)((double)a.n / (slots * pixels)) * *a.v_loss : 0.f;
+    if constexpr (kDropout) return __ldg(&a.colors[(size_t)id * a.channels + c]);
+    const float scale = *a.scale;
     return scale * (float)a.counts[id] + (a.v_importance != nullptr ? a.v_importance[id] : 0.f);
 }
 template <bool kDropout>
 __device__ __forceinline__ float pixel_value(const SumArgs &a, const int p, const int c) {
-    if constexpr (kDropout) return c < a.channels ? __ldg(&a.v_output[(size_t)c * (a.img_h * a.img_w) + p]) : 0.f;
+    if constexpr (kDropout) return __ldg(&a.v_output[(size_t)c * (a.img_h * a.img_w) + p]);
     return 1.f;
 }
 
@@ -106,19 +105,16 @@ __device__ __noinline__ void add_slots(const SumArgs &a, const int p, const bool
     }
 }
 
-// The rows of all Gaussians, and their sums zeroed
-template <int C, bool kDropout>
-__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ SumArgs a) {
+// The sums zeroed, and balance's scale
+template <int kValues, bool kDropout>
+__global__ void __launch_bounds__(256) zero_sums_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
-    const int id = blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.n) return;
-    float f[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) f[c] = row_value<kDropout>(a, id, c);
-    Rows<C>::store(a.rows, id, row_geometry(a.xys, a.conics, id), f);
-    constexpr int kValues = SumLayout<C, kDropout>::kValues;
-#pragma unroll
-    for (int e = 0; e < kValues / 4; ++e) reinterpret_cast<float4 *>(a.sums)[(size_t)id * (kValues / 4) + e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int e = blockIdx.x * 256 + threadIdx.x;
+    if (!kDropout && e == 0) {
+        const double slots = (double)a.totals[0], pixels = (double)a.totals[1];
+        *a.scale = a.v_loss != nullptr && slots > 0.0 ? (float)((double)a.n / (slots * pixels)) * *a.v_loss : 0.f;
+    }
+    if (e < a.n * (kValues / 4)) reinterpret_cast<float4 *>(a.sums)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 template <int C, bool kDropout>
@@ -148,7 +144,8 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4)
         for (int b = 0; b < kPix; ++b)
 #pragma unroll
             for (int c = 0; c < C; ++c) v[b][c] = patch.inside[b] && !have_totals ? pixel_value<kDropout>(a, patch.p[b], c) : 0.f;
-        regular = Rows::gather(a.rows, rows, sm.pairs) && regular;
+        regular = Rows::gather(rows, a.xys, a.conics, [&](const int id, const int c) { return row_value<kDropout>(a, id, c); }, sm.pairs) &&
+                  regular;
         __syncwarp();
         // a lane is kPix pixels: the group's weights, and the sums over all groups
         unsigned held[kPix];
@@ -297,19 +294,19 @@ __global__ void __launch_bounds__(256) finish_sums_kernel(const int n, const int
         if (e - 5 < channels) v_colors[(size_t)g * channels + e - 5] = s[e];
 }
 
-// The backward pass: rows, sums, gradients. a.rows and a.sums are in the workspace, of sum_bytes.
+// The backward pass; its workspace holds balance's scale (16 bytes) and the sums
 template <int C, bool kDropout>
 constexpr size_t sum_bytes(const int n) {
-    return (sizeof(float4) * Rows<C>::kQuads + sizeof(float) * SumLayout<C, kDropout>::kValues) * (size_t)n;
+    return 16 + sizeof(float) * SumLayout<C, kDropout>::kValues * (size_t)n;
 }
 
 template <int C, bool kDropout>
 void launch_sums(SumArgs a, void *workspace, const bool accumulate, float *v_xy, float *v_conic, float *v_colors, cudaStream_t s) {
     constexpr int kValues = SumLayout<C, kDropout>::kValues;
     constexpr int kBytes = (int)sizeof(SumSmem<C, kDropout>);
-    a.rows = static_cast<float4 *>(workspace);
-    a.sums = reinterpret_cast<float *>(a.rows + (size_t)Rows<C>::kQuads * a.n);
-    launch(rows_kernel<C, kDropout>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a);
+    a.scale = static_cast<float *>(workspace);
+    a.sums = a.scale + 4;
+    launch(zero_sums_kernel<kValues, kDropout>, dim3(ceil_div(a.n * (kValues / 4), 256)), dim3(256), 0, s, a);
     if (a.img_h > 0 && a.img_w > 0) {
         // past 48 KB the kernel has to be told; the setting belongs to the device, so every call makes it
         if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);

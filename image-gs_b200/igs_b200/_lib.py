@@ -61,7 +61,7 @@ SIGNATURES = {
     "igs_topk_balance_fwd": (c_int, [c_int, c_int, c_int, P, P, P, P, P, P, P, P, P, c_size_t, P]),
     "igs_topk_balance_bwd": (c_int, [c_int, c_int, c_int, P, P, P, P, P, P, P, P, c_int, P, P, P, c_size_t, P]),
     "igs_topk_dropout_workspace": (c_size_t, [c_int, c_int]),
-    "igs_topk_dropout_fwd": (c_int, [c_int, c_int, c_int, c_int, P, P, P, P, c_double, P, P, P, P, c_size_t, P]),
+    "igs_topk_dropout_fwd": (c_int, [c_int, c_int, c_int, c_int, P, P, P, P, c_double, P, P, P, P]),
     "igs_topk_dropout_bwd": (c_int, [c_int, c_int, c_int, c_int, P, P, P, P, P, c_double, P, P, P, P, P, c_size_t, P]),
     "igs_neighbors_workspace": (c_size_t, [c_int]),
     "igs_nearest_neighbors": (c_int, [c_int, P, c_int, P, P, P, c_size_t, P]),

@@ -408,10 +408,7 @@ def topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk,
     channels, p = _check_dropout(h, w, n, colors, p, rng_state)
     out_img = torch.empty(channels, h, w, device=dev, dtype=torch.float32)
     rng_used = torch.empty(2, device=dev, dtype=torch.int64)
-    ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
-    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_dropout_fwd", h, w, channels, n, xys, conics, colors, pixel_topk, p, rng_state,
-         out_img, rng_used, ws, ws_bytes)
+    _run(dev, "igs_topk_dropout_fwd", h, w, channels, n, xys, conics, colors, pixel_topk, p, rng_state, out_img, rng_used)
     return out_img, rng_used
 
 

@@ -225,8 +225,7 @@ class RasterStep:
     def _dropout_forward(self):
         self._check(self.lib.igs_topk_dropout_fwd(self.h, self.w, self.c, self.n, ptr(self.xys), ptr(self.conics), ptr(self.features),
                                                   ptr(self.pixel_topk), self.drop_p, ptr(self.rng_state), ptr(self.image),
-                                                  ptr(self.rng_used), ptr(self.drop_ws), self.drop_ws_bytes, self._stream()),
-                    "dropout forward")
+                                                  ptr(self.rng_used), self._stream()), "dropout forward")
 
     def _image_loss(self):
         self._check(self.lib.igs_l1_loss(self.image.numel(), ptr(self.image), ptr(self.target), self.l1_ratio, ptr(self.loss),
@@ -274,7 +273,7 @@ class RasterStep:
 
     # kernels each stage launches (memsets excluded)
     KERNELS = {"_quantize": 1, "_project": 1, "_cumsum": 2, "_bin": 4, "_raster": 2, "_forward": 2, "_backward": 1, "_project_backward": 1,
-               "_rate_term": 2, "_feature_grads": 1, "_train_step": 8, "_lists_forward": 1, "_dropout_forward": 2, "_image_loss": 1,
+               "_rate_term": 2, "_feature_grads": 1, "_train_step": 8, "_lists_forward": 1, "_dropout_forward": 1, "_image_loss": 1,
                "_dropout_backward": 3, "_lists_backward": 1, "_balance_term": 6, "_next_mask": 0}
 
     @property

@@ -296,12 +296,12 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
  * counters (i, j, offset low, offset high), j = 0 and 1, slot k < 8 draws the upper 24 bits of word k, slots 8 and 9 the low bytes of words
  * 0, 1, 2 and 3, 4, 5 (the first most significant). rng_used [2] gets the values that the pass saw; the backward pass takes them, so the
  * caller may move rng_state on in between, in a captured graph too. igs_topk_dropout_bwd writes v_xy [N,2], v_conic [N,3] and v_colors
- * [N,C] whole, from v_output [C,H,W]. 1 to 12 channels, sizes as above. workspace: igs_topk_dropout_workspace(N, C) bytes,
- * 16-byte aligned, whose content need not survive between the two calls. */
+ * [N,C] whole, from v_output [C,H,W]; its workspace: igs_topk_dropout_workspace(N, C) bytes, 16-byte aligned. 1 to 12 channels, sizes as
+ * above. */
 size_t igs_topk_dropout_workspace(int num_points, int channels);
 int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
                          const float *colors, const int32_t *pixel_topk, double p, const int64_t *rng_state, float *out_img,
-                         int64_t *rng_used, void *workspace, size_t workspace_bytes, void *stream);
+                         int64_t *rng_used, void *stream);
 int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
                          const float *colors, const float *v_output, const int32_t *pixel_topk, double p, const int64_t *rng_used,
                          float *v_xy, float *v_conic, float *v_colors, void *workspace, size_t workspace_bytes, void *stream);

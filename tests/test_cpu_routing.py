@@ -125,8 +125,8 @@ def test_entry_points_refuse_invalid_arguments():
     refused(bwd(size=lib.igs_topk_balance_workspace(3) - 1), "workspace")
     assert lib.igs_topk_balance_bwd(0, 4, 3, null, fake, null, null, fake, fake, null, null, 0, fake, fake, fake, big, null) == 1
     assert bwd(n=0) == 0
-    drop = lambda h=4, c=3, n=3, p=0.1, topk=fake, rng=fake, ws=fake, size=big: lib.igs_topk_dropout_fwd(  # noqa: E731
-        h, 4, c, n, fake, fake, fake, topk, p, rng, fake, fake, ws, size, null)
+    drop = lambda h=4, c=3, n=3, p=0.1, topk=fake, rng=fake: lib.igs_topk_dropout_fwd(  # noqa: E731
+        h, 4, c, n, fake, fake, fake, topk, p, rng, fake, fake, null)
     refused(drop(h=-1), "negative")
     refused(drop(c=0), "channels")
     refused(drop(c=13), "channels")
@@ -134,8 +134,7 @@ def test_entry_points_refuse_invalid_arguments():
         refused(drop(p=p), "[0, 1]")
     refused(drop(rng=null), "rng")
     refused(drop(topk=null), "null")
-    refused(drop(ws=odd), "aligned")
-    refused(drop(size=lib.igs_topk_dropout_workspace(3, 3) - 1), "workspace")
+    refused(drop(topk=odd), "aligned")
     back = lambda c=3, n=3, p=0.1, v=fake, ws=fake, size=big: lib.igs_topk_dropout_bwd(  # noqa: E731
         4, 4, c, n, fake, fake, fake, fake, fake, p, fake, v, fake, fake, ws, size, null)
     refused(back(c=13), "channels")
