@@ -53,6 +53,12 @@ struct BalanceArgs {
     int *counts;
     unsigned long long *fixed;
     BalanceWorkspace *ws;
+    double inv_scale;
+    float *importance;
+    double *partials;  // a sum for each block of the finish kernel
+    float *loss;
+    long long *totals;
+    bool finish_in_last;
 };
 
 __global__ void __launch_bounds__(kThreads) balance_zero_kernel(const __grid_constant__ BalanceArgs a) {
@@ -85,8 +91,8 @@ __device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
     }
 }
 
-// A warp is a patch, a lane first its pixels and then half a row, as in topk_sums.cuh
-__global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
+// A warp is a patch, a lane first its pixels and then a row or half of one, as in topk_sums.cuh
+__device__ __forceinline__ void count_patch(const BalanceArgs &a) {
     __shared__ struct {
         union {
             int keys[igs::kKeyWords];
@@ -97,7 +103,6 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
     } smem[igs::kPatches];
     auto &sm = smem[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31;
-    igs::wait_for_predecessor();
     const igs::Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
     const auto slots = [&](const int p, const bool inside) { return igs::AllSlots{inside && (a.mask == nullptr || a.mask[p] != 0)}; };
@@ -168,56 +173,59 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __
     }
 }
 
-// importance from the fixed-point sums, and the loss: each block's sums of counts and of counts * importance (in double, in thread order),
-// the last block to finish adds them in block order
-__global__ void __launch_bounds__(kThreads) balance_finish_kernel(const int n, const int *__restrict__ counts,
-                                                                  const unsigned long long *__restrict__ fixed, const double inv_scale,
-                                                                  float *__restrict__ importance, double *__restrict__ partials,
-                                                                  BalanceWorkspace *__restrict__ ws, float *__restrict__ loss,
-                                                                  long long *__restrict__ totals) {
-    igs::wait_for_predecessor();
-    __shared__ double s_sum[kThreads / 32];
-    __shared__ bool last;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int g = blockIdx.x * kThreads + threadIdx.x;
-    double v = 0.0;
-    int c = 0;
-    if (g < n) {
-        const double imp = (double)(long long)fixed[g] * inv_scale;
-        importance[g] = (float)imp;
-        c = counts[g];
-        v = imp * c;
-    }
-    auto block_sum = [&](double x) {
+// This thread's sum over the CTA, in one order, on all threads
+template <int kCta>
+__device__ __forceinline__ double cta_sum(double x) {
+    __shared__ double s_sum[kCta / 32];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        __syncthreads();
-        if (lane == 0) s_sum[warp] = x;
-        __syncthreads();
-        double total = 0.0;
-        for (int w = 0; w < kThreads / 32; ++w) total += s_sum[w];
-        return total;
-    };
-    const double block = block_sum(v), filled = block_sum((double)c);
-    if (threadIdx.x == 0) {
-        partials[blockIdx.x] = block;
-        atomicAdd(&ws->filled, (unsigned long long)filled);
-        __threadfence();
-        last = atomicAdd(&ws->ticket, 1u) == gridDim.x - 1;
-    }
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     __syncthreads();
-    if (!last) return;
-    __threadfence();
-    double sum = 0.0;
-    for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) sum += __ldcg(&partials[b]);
-    const double all = block_sum(sum);
-    if (threadIdx.x == 0) {
-        const unsigned long long a = __ldcg(&ws->filled);
-        unsigned long long t = 0;
-        for (int q = 0; q < kRoutedSlots; ++q) t += __ldcg(&ws->routed[q]);
-        *loss = a ? (float)((double)n / ((double)a * (double)t) * all) : 0.f;
-        totals[0] = (long long)a, totals[1] = (long long)t;
-    }
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = x;
+    __syncthreads();
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kCta / 32; ++w) total += s_sum[w];
+    return total;
+}
+
+// A Gaussian's importance, from its fixed-point sum; its counts and its term of the loss are added to filled and sum
+__device__ __forceinline__ void finish_gaussian(const BalanceArgs &a, const int g, double &filled, double &sum) {
+    const double importance = (double)(long long)__ldcg(&a.fixed[g]) * a.inv_scale;
+    a.importance[g] = (float)importance;
+    const int count = __ldcg(&a.counts[g]);
+    filled += count, sum += importance * count;
+}
+
+__device__ __forceinline__ void finish_loss(const BalanceArgs &a, const double filled, const double sum) {
+    unsigned long long routed = 0;
+    for (int q = 0; q < kRoutedSlots; ++q) routed += __ldcg(&a.ws->routed[q]);
+    *a.loss = filled > 0.0 ? (float)((double)a.n / (filled * (double)routed) * sum) : 0.f;
+    a.totals[0] = (long long)filled, a.totals[1] = (long long)routed;
+}
+
+__global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
+    igs::wait_for_predecessor();
+    count_patch(a);
+    if (!a.finish_in_last || !igs::last_cta(&a.ws->ticket)) return;
+    double filled = 0.0, sum = 0.0;
+    for (int g = threadIdx.x; g < a.n; g += igs::kPatchThreads) finish_gaussian(a, g, filled, sum);
+    filled = cta_sum<igs::kPatchThreads>(filled), sum = cta_sum<igs::kPatchThreads>(sum);
+    if (threadIdx.x == 0) finish_loss(a, filled, sum);
+}
+
+// Each block's sums, added in block order by the last block to finish
+__global__ void __launch_bounds__(kThreads) balance_finish_kernel(const __grid_constant__ BalanceArgs a) {
+    igs::wait_for_predecessor();
+    const int g = blockIdx.x * kThreads + threadIdx.x;
+    double filled = 0.0, sum = 0.0;
+    if (g < a.n) finish_gaussian(a, g, filled, sum);
+    filled = cta_sum<kThreads>(filled), sum = cta_sum<kThreads>(sum);
+    if (threadIdx.x == 0) a.partials[blockIdx.x] = sum, atomicAdd(&a.ws->filled, (unsigned long long)filled);
+    if (!igs::last_cta(&a.ws->ticket)) return;
+    sum = 0.0;
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) sum += __ldcg(&a.partials[b]);
+    sum = cta_sum<kThreads>(sum);
+    if (threadIdx.x == 0) finish_loss(a, (double)__ldcg(&a.ws->filled), sum);
 }
 
 }  // namespace
@@ -244,13 +252,13 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     double *partials = reinterpret_cast<double *>(fixed + num_points);
     const int bits = fraction_bits(pixels);
     const int blocks = finish_blocks(num_points);
-    const BalanceArgs a = {img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask,
-                           (float)((int64_t)1 << bits), counts, fixed, ws};
+    const bool patches = pixels > 0 && num_points > 0, in_last = patches && num_points <= igs::kFinishInLast;
+    const BalanceArgs a = {img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask, (float)((int64_t)1 << bits), counts,
+                           fixed, ws, 1.0 / (double)((int64_t)1 << bits), importance, partials, loss,
+                           reinterpret_cast<long long *>(totals), in_last};
     igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
-    if (pixels > 0 && num_points > 0) igs::launch(balance_kernel, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
-    igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, num_points, (const int *)counts,
-                (const unsigned long long *)fixed, 1.0 / (double)((int64_t)1 << bits), importance, partials, ws, loss,
-                reinterpret_cast<long long *>(totals));
+    if (patches) igs::launch(balance_kernel, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
+    if (!in_last) igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
     return igs::check_launch("igs_topk_balance_fwd");
 }
 
@@ -272,7 +280,8 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
     a.img_h = img_height, a.img_w = img_width, a.n = num_points;
     a.xys = xys, a.conics = conics, a.pixel_topk = pixel_topk, a.mask = pixel_mask;
     a.counts = counts, a.totals = reinterpret_cast<const long long *>(totals), a.v_loss = v_loss, a.v_importance = v_importance;
-    igs::launch_sums<1, false>(a, workspace, accumulate != 0, v_xy, v_conic, nullptr, s);
+    a.accumulate = accumulate != 0, a.v_xy = v_xy, a.v_conic = v_conic;
+    igs::launch_sums<1, false>(a, workspace, s);
     return igs::check_launch("igs_topk_balance_bwd");
 }
 

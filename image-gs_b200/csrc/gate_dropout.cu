@@ -187,8 +187,9 @@ int igs_topk_dropout_bwd(int img_height, int img_width, int channels, int num_po
     a.img_h = img_height, a.img_w = img_width, a.channels = channels, a.n = num_points;
     a.xys = xys, a.conics = conics, a.colors = colors, a.v_output = v_output, a.pixel_topk = pixel_topk;
     a.rng = reinterpret_cast<const long long *>(rng_used), a.threshold = (uint32_t)rint(p * 16777216.0);
+    a.v_xy = v_xy, a.v_conic = v_conic, a.v_colors = v_colors;
     with_channels(channels, [&](auto count) {
-        igs::launch_sums<decltype(count)::value, true>(a, workspace, false, v_xy, v_conic, v_colors, s);
+        igs::launch_sums<decltype(count)::value, true>(a, workspace, s);
     });
     return igs::check_launch("igs_topk_dropout_bwd");
 }

@@ -30,6 +30,9 @@ struct SumArgs {
     const long long *rng;
     uint32_t threshold;
     float *sums;                 // [N, SumLayout::kValues]
+    unsigned *ticket;            // NULL: the gradients are finished by a kernel of their own
+    bool accumulate;
+    float *v_xy, *v_conic, *v_colors;
 };
 
 // C: the values per row and pixel (balance: 1; dropout: the channels)
@@ -105,11 +108,12 @@ __device__ __noinline__ void add_slots(const SumArgs &a, const int p, const bool
     }
 }
 
-// The sums zeroed, and balance's scale
+// The sums zeroed, and balance's scale and the ticket
 template <int kValues, bool kDropout>
 __global__ void __launch_bounds__(256) zero_sums_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
     const int e = blockIdx.x * 256 + threadIdx.x;
+    if (e == 0 && a.ticket != nullptr) *a.ticket = 0;
     if (!kDropout && e == 0) {
         const double slots = (double)a.totals[0], pixels = (double)a.totals[1];
         *a.scale = a.v_loss != nullptr && slots > 0.0 ? (float)((double)a.n / (slots * pixels)) * *a.v_loss : 0.f;
@@ -117,15 +121,46 @@ __global__ void __launch_bounds__(256) zero_sums_kernel(const __grid_constant__ 
     if (e < a.n * (kValues / 4)) reinterpret_cast<float4 *>(a.sums)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
+// Zero times a conic that is not finite is nothing here: a Gaussian without a weight has no gradient
+__device__ __forceinline__ float times(const float conic, const float sum) { return sum != 0.f ? conic * sum : 0.f; }
+
+// A Gaussian's gradients from its sums
 template <int C, bool kDropout>
-__global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4)
-    sums_kernel(const __grid_constant__ SumArgs a) {
+__device__ __forceinline__ void finish_gaussian(const SumArgs &a, const int g) {
+    constexpr int kValues = SumLayout<C, kDropout>::kValues;
+    float s[kValues];
+#pragma unroll
+    for (int e = 0; e < kValues / 4; ++e) {
+        const float4 q = __ldcg(&reinterpret_cast<const float4 *>(a.sums)[(size_t)g * (kValues / 4) + e]);
+        s[4 * e] = q.x, s[4 * e + 1] = q.y, s[4 * e + 2] = q.z, s[4 * e + 3] = q.w;
+    }
+    const float ca = a.conics[3 * (size_t)g], cb = a.conics[3 * (size_t)g + 1], cc = a.conics[3 * (size_t)g + 2];
+    const float out[5] = {times(ca, s[0]) + times(cb, s[1]), times(cb, s[0]) + times(cc, s[1]), 0.5f * s[2], s[3], 0.5f * s[4]};
+#pragma unroll
+    for (int e = 0; e < 5; ++e) {
+        float *dst = e < 2 ? &a.v_xy[2 * (size_t)g + e] : &a.v_conic[3 * (size_t)g + e - 2];
+        *dst = a.accumulate ? *dst + out[e] : out[e];
+    }
+    if constexpr (kDropout) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) a.v_colors[(size_t)g * C + c] = s[5 + c];
+    }
+}
+
+template <int C, bool kDropout>
+__global__ void __launch_bounds__(256) finish_sums_kernel(const __grid_constant__ SumArgs a) {
+    wait_for_predecessor();
+    const int g = blockIdx.x * 256 + threadIdx.x;
+    if (g < a.n) finish_gaussian<C, kDropout>(a, g);
+}
+
+template <int C, bool kDropout>
+__device__ __forceinline__ void sum_patch(const SumArgs &a) {
     using Rows = igs::Rows<C>;
     constexpr int kValues = SumLayout<C, kDropout>::kValues, kPairQuads = Rows::kPairQuads;
     extern __shared__ __align__(16) char smem_bytes[];
     const int lane = threadIdx.x & 31;
     typename SumSmem<C, kDropout>::Warp &sm = reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes)->warp[threadIdx.x >> 5];
-    wait_for_predecessor();
     const Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
     const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
@@ -266,54 +301,35 @@ __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4)
     }
 }
 
-// Zero times a conic that is not finite is nothing here: a Gaussian without a weight has no gradient
-__device__ __forceinline__ float times(const float conic, const float sum) { return sum != 0.f ? conic * sum : 0.f; }
-
-template <int kValues>
-__global__ void __launch_bounds__(256) finish_sums_kernel(const int n, const int channels, const float *__restrict__ conics,
-                                                          const float *__restrict__ sums, const bool accumulate, float *__restrict__ v_xy,
-                                                          float *__restrict__ v_conic, float *__restrict__ v_colors) {
+template <int C, bool kDropout>
+__global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4) sums_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
-    const int g = blockIdx.x * 256 + threadIdx.x;
-    if (g >= n) return;
-    float s[kValues];
-#pragma unroll
-    for (int e = 0; e < kValues / 4; ++e) {
-        const float4 q = reinterpret_cast<const float4 *>(sums)[(size_t)g * (kValues / 4) + e];
-        s[4 * e] = q.x, s[4 * e + 1] = q.y, s[4 * e + 2] = q.z, s[4 * e + 3] = q.w;
-    }
-    const float a = conics[3 * (size_t)g], b = conics[3 * (size_t)g + 1], c = conics[3 * (size_t)g + 2];
-    const float out[5] = {times(a, s[0]) + times(b, s[1]), times(b, s[0]) + times(c, s[1]), 0.5f * s[2], s[3], 0.5f * s[4]};
-#pragma unroll
-    for (int e = 0; e < 5; ++e) {
-        float *dst = e < 2 ? &v_xy[2 * (size_t)g + e] : &v_conic[3 * (size_t)g + e - 2];
-        *dst = accumulate ? *dst + out[e] : out[e];
-    }
-#pragma unroll
-    for (int e = 5; e < kValues; ++e)
-        if (e - 5 < channels) v_colors[(size_t)g * channels + e - 5] = s[e];
+    sum_patch<C, kDropout>(a);
+    if (a.ticket == nullptr || !last_cta(a.ticket)) return;
+    for (int g = threadIdx.x; g < a.n; g += kPatchThreads) finish_gaussian<C, kDropout>(a, g);
 }
 
-// The backward pass; its workspace holds balance's scale (16 bytes) and the sums
+// The backward pass; its workspace holds balance's scale and the ticket (16 bytes) and the sums
 template <int C, bool kDropout>
 constexpr size_t sum_bytes(const int n) {
     return 16 + sizeof(float) * SumLayout<C, kDropout>::kValues * (size_t)n;
 }
 
 template <int C, bool kDropout>
-void launch_sums(SumArgs a, void *workspace, const bool accumulate, float *v_xy, float *v_conic, float *v_colors, cudaStream_t s) {
+void launch_sums(SumArgs a, void *workspace, cudaStream_t s) {
     constexpr int kValues = SumLayout<C, kDropout>::kValues;
     constexpr int kBytes = (int)sizeof(SumSmem<C, kDropout>);
+    const bool pixels = a.img_h > 0 && a.img_w > 0, in_last = pixels && a.n <= kFinishInLast;
     a.scale = static_cast<float *>(workspace);
+    a.ticket = in_last ? reinterpret_cast<unsigned *>(a.scale + 1) : nullptr;
     a.sums = a.scale + 4;
     launch(zero_sums_kernel<kValues, kDropout>, dim3(ceil_div(a.n * (kValues / 4), 256)), dim3(256), 0, s, a);
-    if (a.img_h > 0 && a.img_w > 0) {
-        // past 48 KB the kernel has to be told; the setting belongs to the device, so every call makes it
-        if (kBytes > 48 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (pixels) {
+        // past 48 KB (with a few bytes that the kernel has besides) the kernel has to be told; the setting is the device's: made every call
+        if (kBytes > 47 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
         launch(sums_kernel<C, kDropout>, tile_grid(a.img_h, a.img_w), dim3(kPatchThreads), kBytes, s, a);
     }
-    launch(finish_sums_kernel<kValues>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a.n, a.channels, a.conics, (const float *)a.sums,
-           accumulate, v_xy, v_conic, v_colors);
+    if (!in_last) launch(finish_sums_kernel<C, kDropout>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a);
 }
 
 }  // namespace igs
