@@ -58,7 +58,6 @@ struct BalanceArgs {
     double *partials;  // a sum for each block of the finish kernel
     float *loss;
     long long *totals;
-    bool finish_in_last;
 };
 
 __global__ void __launch_bounds__(kThreads) balance_zero_kernel(const __grid_constant__ BalanceArgs a) {
@@ -92,16 +91,16 @@ __device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
 }
 
 // A warp is a patch, a lane first its pixels and then a row or half of one, as in topk_sums.cuh
-__device__ __forceinline__ void count_patch(const BalanceArgs &a) {
-    __shared__ struct {
-        union {
-            int keys[igs::kKeyWords];
-            alignas(16) float weight[igs::kRows * kWeightPitch];
-        };
-        float4 pairs[Rows::kGroupQuads];
-        alignas(16) float inv[kPatchPixels];
-    } smem[igs::kPatches];
-    auto &sm = smem[threadIdx.x >> 5];
+struct BalanceSmem {
+    union {
+        int keys[igs::kKeyWords];
+        alignas(16) float weight[igs::kRows * kWeightPitch];
+    };
+    float4 pairs[Rows::kGroupQuads];
+    alignas(16) float inv[kPatchPixels];
+};
+
+__device__ __forceinline__ void count_patch(const BalanceArgs &a, BalanceSmem &sm) {
     const int lane = threadIdx.x & 31;
     const igs::Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
@@ -173,10 +172,9 @@ __device__ __forceinline__ void count_patch(const BalanceArgs &a) {
     }
 }
 
-// This thread's sum over the CTA, in one order, on all threads
+// The sum over the CTA, in one order, on all threads; s_sum: a word per warp
 template <int kCta>
-__device__ __forceinline__ double cta_sum(double x) {
-    __shared__ double s_sum[kCta / 32];
+__device__ __forceinline__ double cta_sum(double x, double *s_sum) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     __syncthreads();
@@ -203,14 +201,20 @@ __device__ __forceinline__ void finish_loss(const BalanceArgs &a, const double f
     a.totals[0] = (long long)filled, a.totals[1] = (long long)routed;
 }
 
+// kFinish: the last CTA finishes
+template <bool kFinish>
 __global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
+    __shared__ BalanceSmem smem[igs::kPatches];
     igs::wait_for_predecessor();
-    count_patch(a);
-    if (!a.finish_in_last || !igs::last_cta(&a.ws->ticket)) return;
-    double filled = 0.0, sum = 0.0;
-    for (int g = threadIdx.x; g < a.n; g += igs::kPatchThreads) finish_gaussian(a, g, filled, sum);
-    filled = cta_sum<igs::kPatchThreads>(filled), sum = cta_sum<igs::kPatchThreads>(sum);
-    if (threadIdx.x == 0) finish_loss(a, filled, sum);
+    count_patch(a, smem[threadIdx.x >> 5]);
+    if constexpr (kFinish) {
+        if (!igs::last_cta(&a.ws->ticket)) return;
+        double filled = 0.0, sum = 0.0;
+        for (int g = threadIdx.x; g < a.n; g += igs::kPatchThreads) finish_gaussian(a, g, filled, sum);
+        double *const s_sum = reinterpret_cast<double *>(smem);
+        filled = cta_sum<igs::kPatchThreads>(filled, s_sum), sum = cta_sum<igs::kPatchThreads>(sum, s_sum);
+        if (threadIdx.x == 0) finish_loss(a, filled, sum);
+    }
 }
 
 // Each block's sums, added in block order by the last block to finish
@@ -219,12 +223,13 @@ __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const __grid_c
     const int g = blockIdx.x * kThreads + threadIdx.x;
     double filled = 0.0, sum = 0.0;
     if (g < a.n) finish_gaussian(a, g, filled, sum);
-    filled = cta_sum<kThreads>(filled), sum = cta_sum<kThreads>(sum);
+    __shared__ double s_sum[kThreads / 32];
+    filled = cta_sum<kThreads>(filled, s_sum), sum = cta_sum<kThreads>(sum, s_sum);
     if (threadIdx.x == 0) a.partials[blockIdx.x] = sum, atomicAdd(&a.ws->filled, (unsigned long long)filled);
     if (!igs::last_cta(&a.ws->ticket)) return;
     sum = 0.0;
     for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) sum += __ldcg(&a.partials[b]);
-    sum = cta_sum<kThreads>(sum);
+    sum = cta_sum<kThreads>(sum, s_sum);
     if (threadIdx.x == 0) finish_loss(a, (double)__ldcg(&a.ws->filled), sum);
 }
 
@@ -255,9 +260,9 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     const bool patches = pixels > 0 && num_points > 0, in_last = patches && num_points <= igs::kFinishInLast;
     const BalanceArgs a = {img_height, img_width, num_points, xys, conics, pixel_topk, pixel_mask, (float)((int64_t)1 << bits), counts,
                            fixed, ws, 1.0 / (double)((int64_t)1 << bits), importance, partials, loss,
-                           reinterpret_cast<long long *>(totals), in_last};
+                           reinterpret_cast<long long *>(totals)};
     igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
-    if (patches) igs::launch(balance_kernel, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
+    if (patches) igs::launch(in_last ? balance_kernel<true> : balance_kernel<false>, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
     if (!in_last) igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
     return igs::check_launch("igs_topk_balance_fwd");
 }

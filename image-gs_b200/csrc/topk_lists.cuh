@@ -299,12 +299,11 @@ struct Rows {
 constexpr int kFinishInLast = 400;
 
 // Whether this CTA is the last to come here, of all CTAs of the grid; what the others wrote before is then visible. All threads together.
+// (No shared memory: the patches' kernels fill it to where a few bytes more would cost them a resident CTA or the L1 its share.)
 __device__ __forceinline__ bool last_cta(unsigned *ticket) {
-    __shared__ bool last;
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(ticket, 1u) == gridDim.x * gridDim.y - 1;
-    __syncthreads();
+    const bool last = __syncthreads_or(threadIdx.x == 0 && atomicAdd(ticket, 1u) == gridDim.x * gridDim.y - 1);
     if (last) __threadfence();
     return last;
 }

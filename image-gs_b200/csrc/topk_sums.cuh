@@ -30,7 +30,7 @@ struct SumArgs {
     const long long *rng;
     uint32_t threshold;
     float *sums;                 // [N, SumLayout::kValues]
-    unsigned *ticket;            // NULL: the gradients are finished by a kernel of their own
+    unsigned *ticket;
     bool accumulate;
     float *v_xy, *v_conic, *v_colors;
 };
@@ -113,7 +113,7 @@ template <int kValues, bool kDropout>
 __global__ void __launch_bounds__(256) zero_sums_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
     const int e = blockIdx.x * 256 + threadIdx.x;
-    if (e == 0 && a.ticket != nullptr) *a.ticket = 0;
+    if (e == 0) *a.ticket = 0;
     if (!kDropout && e == 0) {
         const double slots = (double)a.totals[0], pixels = (double)a.totals[1];
         *a.scale = a.v_loss != nullptr && slots > 0.0 ? (float)((double)a.n / (slots * pixels)) * *a.v_loss : 0.f;
@@ -301,12 +301,16 @@ __device__ __forceinline__ void sum_patch(const SumArgs &a) {
     }
 }
 
-template <int C, bool kDropout>
+// kFinish: the last CTA finishes the gradients. (A kernel of its own: with the barrier behind it, even never reached, the patch's code took
+// 18 % more instructions.)
+template <int C, bool kDropout, bool kFinish>
 __global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4) sums_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
     sum_patch<C, kDropout>(a);
-    if (a.ticket == nullptr || !last_cta(a.ticket)) return;
-    for (int g = threadIdx.x; g < a.n; g += kPatchThreads) finish_gaussian<C, kDropout>(a, g);
+    if constexpr (kFinish) {
+        if (!last_cta(a.ticket)) return;
+        for (int g = threadIdx.x; g < a.n; g += kPatchThreads) finish_gaussian<C, kDropout>(a, g);
+    }
 }
 
 // The backward pass; its workspace holds balance's scale and the ticket (16 bytes) and the sums
@@ -321,13 +325,14 @@ void launch_sums(SumArgs a, void *workspace, cudaStream_t s) {
     constexpr int kBytes = (int)sizeof(SumSmem<C, kDropout>);
     const bool pixels = a.img_h > 0 && a.img_w > 0, in_last = pixels && a.n <= kFinishInLast;
     a.scale = static_cast<float *>(workspace);
-    a.ticket = in_last ? reinterpret_cast<unsigned *>(a.scale + 1) : nullptr;
+    a.ticket = reinterpret_cast<unsigned *>(a.scale + 1);
     a.sums = a.scale + 4;
     launch(zero_sums_kernel<kValues, kDropout>, dim3(ceil_div(a.n * (kValues / 4), 256)), dim3(256), 0, s, a);
     if (pixels) {
-        // past 48 KB (with a few bytes that the kernel has besides) the kernel has to be told; the setting is the device's: made every call
-        if (kBytes > 47 * 1024) cudaFuncSetAttribute(sums_kernel<C, kDropout>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        launch(sums_kernel<C, kDropout>, tile_grid(a.img_h, a.img_w), dim3(kPatchThreads), kBytes, s, a);
+        const auto kernel = in_last ? sums_kernel<C, kDropout, true> : sums_kernel<C, kDropout, false>;
+        // past 48 KB the kernel has to be told; the setting belongs to the device, so every call makes it
+        if (kBytes > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        launch(kernel, tile_grid(a.img_h, a.img_w), dim3(kPatchThreads), kBytes, s, a);
     }
     if (!in_last) launch(finish_sums_kernel<C, kDropout>, dim3(ceil_div(a.n, 256)), dim3(256), 0, s, a);
 }
