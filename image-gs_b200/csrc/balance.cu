@@ -90,7 +90,6 @@ __device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
     }
 }
 
-// A warp is a patch, a lane first its pixels and then a row or half of one, as in topk_sums.cuh
 struct BalanceSmem {
     union {
         int keys[igs::kKeyWords];
@@ -100,75 +99,103 @@ struct BalanceSmem {
     alignas(16) float inv[kPatchPixels];
 };
 
-__device__ __forceinline__ void count_patch(const BalanceArgs &a, BalanceSmem &sm) {
+__device__ __forceinline__ igs::PatchRows balance_rows(const BalanceArgs &a, const igs::Patch &patch, const int g, int *keys) {
+    return igs::find_rows(
+        a.pixel_topk, patch, a.n,
+        [&](const int p, const bool inside) { return igs::AllSlots{inside && (a.mask == nullptr || a.mask[p] != 0)}; }, g, keys);
+}
+
+// A lane is its pixels: the group's weights into shared memory, and into the pixels' sums
+__device__ __forceinline__ void weigh_rows(const igs::PatchRows &rows, const igs::Patch &patch, BalanceSmem &sm, float2 (&total)[kPix]) {
+    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
+    float2 minus_y[kPix];
+    unsigned held[kPix];
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), held[b] = rows.bits[b];
+    const float4 *pairs = sm.pairs;
+    float *weight = sm.weight + (threadIdx.x & 31);
+#pragma unroll 1
+    for (int pair = 0; 2 * pair < rows.n; ++pair, pairs += Rows::kPairQuads, weight += 2 * kWeightPitch) {
+        float2 w[kPix];
+        Rows::weights(pairs, held, minus_x, minus_y, w);
+#pragma unroll
+        for (int b = 0; b < kPix; ++b) {
+            held[b] >>= 2;
+            weight[32 * b] = w[b].x, weight[kWeightPitch + 32 * b] = w[b].y;
+            total[b] = igs::add2(total[b], w[b]);
+        }
+    }
+}
+
+__device__ __forceinline__ void invert_totals(BalanceSmem &sm, const float2 (&total)[kPix]) {
+#pragma unroll
+    for (int b = 0; b < kPix; ++b)
+        sm.inv[32 * b + (threadIdx.x & 31)] = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
+}
+
+// A lane is a row or, up to 16 rows, half of one (as in topk_sums.cuh): its gates' sum and its holders
+__device__ __forceinline__ void count_rows(const BalanceArgs &a, const igs::PatchRows &rows, const BalanceSmem &sm) {
     const int lane = threadIdx.x & 31;
+    const bool halves = rows.n <= 16;
+    const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
+    const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *inv_at = sm.inv + half * (kPatchPixels / 2);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int q = 0; q < (halves ? kPatchPixels / 8 : kPatchPixels / 4); ++q, w_at += 4, inv_at += 4) {
+        const float4 w = *reinterpret_cast<const float4 *>(w_at);
+        const float4 inv = *reinterpret_cast<const float4 *>(inv_at);
+        sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
+    }
+    const int id = __shfl_sync(0xffffffffu, rows.id, r);
+    if (halves) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
+    if (lane < rows.n) atomicAdd(&a.counts[rows.id], rows.holders);
+}
+
+// A patch of more than 32 rows: all groups for the pixels' sums, then all again for the rows'
+__device__ __noinline__ bool count_groups(const BalanceArgs &a, const igs::Patch &patch, BalanceSmem &sm) {
+    float2 total[kPix] = {};
+    for (int pass = 0; pass < 2; ++pass) {
+        bool more = true;
+        for (int g = 0; more; ++g) {
+            const igs::PatchRows rows = balance_rows(a, patch, g, sm.keys);
+            more = rows.more;
+            if (!Rows::gather(rows, a.xys, a.conics, [](int, int) { return 0.f; }, sm.pairs)) return false;
+            __syncwarp();
+            weigh_rows(rows, patch, sm, total);
+            __syncwarp();
+            if (pass == 1) count_rows(a, rows, sm);
+        }
+        if (pass == 0) invert_totals(sm, total);
+        __syncwarp();
+    }
+    return true;
+}
+
+// A warp is a patch
+__device__ __forceinline__ void count_patch(const BalanceArgs &a, BalanceSmem &sm) {
     const igs::Patch patch(a.img_h, a.img_w);
     if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
-    const auto slots = [&](const int p, const bool inside) { return igs::AllSlots{inside && (a.mask == nullptr || a.mask[p] != 0)}; };
-    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
-    float2 minus_y[kPix], total[kPix];
-#pragma unroll
-    for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), total[b] = make_float2(0.f, 0.f);
-    bool regular = true, have_total = false;
-    for (int g = 0;;) {
-        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
-        regular = Rows::gather(rows, a.xys, a.conics, [](int, int) { return 0.f; }, sm.pairs) && regular;
+    const igs::PatchRows rows = balance_rows(a, patch, 0, sm.keys);
+    const unsigned routed = __reduce_add_sync(0xffffffffu, (unsigned)rows.filled);
+    if ((threadIdx.x & 31) == 0 && routed > 0)
+        atomicAdd(&a.ws->routed[(blockIdx.x + blockIdx.y) % kRoutedSlots], (unsigned long long)routed);
+    bool regular;
+    if (rows.more) {
+        regular = count_groups(a, patch, sm);
+    } else {
+        regular = Rows::gather(rows, a.xys, a.conics, [](int, int) { return 0.f; }, sm.pairs);
         __syncwarp();
-        unsigned held[kPix];
-#pragma unroll
-        for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
-#pragma unroll 1
-        for (int pair = 0; 2 * pair < rows.n; ++pair) {
-            float *weight = sm.weight + 2 * pair * kWeightPitch + lane;
-            float2 w[kPix];
-            Rows::weights(sm.pairs + pair * Rows::kPairQuads, held, minus_x, minus_y, w);
-#pragma unroll
-            for (int b = 0; b < kPix; ++b) {
-                held[b] >>= 2;
-                weight[32 * b] = w[b].x, weight[kWeightPitch + 32 * b] = w[b].y;
-                total[b] = igs::add2(total[b], w[b]);  // (unused the second time)
-            }
-        }
-        if (!have_total) {
-            if (rows.more) {
-                ++g;
-                continue;
-            }
-            have_total = true;
-#pragma unroll
-            for (int b = 0; b < kPix; ++b) sm.inv[32 * b + lane] = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
-            const unsigned routed = __reduce_add_sync(0xffffffffu, (unsigned)rows.filled);
-            if (lane == 0 && routed > 0)
-                atomicAdd(&a.ws->routed[(blockIdx.x + blockIdx.y) % kRoutedSlots], (unsigned long long)routed);
-            if (!regular) {
-#pragma unroll 1
-                for (int b = 0; b < kPix; ++b)
-                    if (patch.inside[b]) count_slots(a, patch.p[b]);
-                return;
-            }
-            if (g > 0) {
-                g = 0;
-                continue;
-            }
-        }
+        float2 total[kPix] = {};
+        weigh_rows(rows, patch, sm, total);
+        invert_totals(sm, total);
         __syncwarp();
-        // a lane is a row or, up to 16 rows, half of one
-        const bool halves = rows.n <= 16;
-        const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
-        const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *inv_at = sm.inv + half * (kPatchPixels / 2);
-        float sum = 0.f;
-#pragma unroll 4
-        for (int q = 0; q < (halves ? kPatchPixels / 8 : kPatchPixels / 4); ++q, w_at += 4, inv_at += 4) {
-            const float4 w = *reinterpret_cast<const float4 *>(w_at);
-            const float4 inv = *reinterpret_cast<const float4 *>(inv_at);
-            sum = fmaf(w.x, inv.x, fmaf(w.y, inv.y, fmaf(w.z, inv.z, fmaf(w.w, inv.w, sum))));
-        }
-        const int id = __shfl_sync(0xffffffffu, rows.id, r);
-        if (halves) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
-        if (lane < rows.n) atomicAdd(&a.counts[rows.id], rows.holders);
-        if (!rows.more) return;
-        ++g;
+        if (regular) count_rows(a, rows, sm);
+    }
+    if (!regular) {
+#pragma unroll 1
+        for (int b = 0; b < kPix; ++b)
+            if (patch.inside[b]) count_slots(a, patch.p[b]);
     }
 }
 

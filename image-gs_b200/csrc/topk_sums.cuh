@@ -155,149 +155,186 @@ __global__ void __launch_bounds__(256) finish_sums_kernel(const __grid_constant_
 }
 
 template <int C, bool kDropout>
-__device__ __forceinline__ void sum_patch(const SumArgs &a) {
-    using Rows = igs::Rows<C>;
-    constexpr int kValues = SumLayout<C, kDropout>::kValues, kPairQuads = Rows::kPairQuads;
-    extern __shared__ __align__(16) char smem_bytes[];
-    const int lane = threadIdx.x & 31;
-    typename SumSmem<C, kDropout>::Warp &sm = reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes)->warp[threadIdx.x >> 5];
-    const Patch patch(a.img_h, a.img_w);
-    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
-    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
-    float2 minus_y[kPix], total2[kPix], scores2[kPix];
+__device__ __forceinline__ PatchRows sum_rows(const SumArgs &a, const Patch &patch, const int g, int *keys) {
+    return find_rows(a.pixel_topk, patch, a.n, [&](const int p, const bool inside) { return sum_slots<kDropout>(a, p, inside); }, g, keys);
+}
+
+// A lane is kPix pixels: the sums over the rows of its pixels' weights and of the weights times the scores
+template <int C>
+struct PixelSums {
+    float v[kPix][C];
+    float2 minus_x, minus_y[kPix], total[kPix], scores[kPix];
+
+    template <bool kDropout>
+    __device__ __forceinline__ void start(const SumArgs &a, const Patch &patch) {
+        minus_x = make_float2(-(float)patch.j, -(float)patch.j);
 #pragma unroll
-    for (int b = 0; b < kPix; ++b) {
-        minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]);
-        total2[b] = make_float2(0.f, 0.f), scores2[b] = make_float2(0.f, 0.f);
+        for (int b = 0; b < kPix; ++b) {
+            minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]);
+            total[b] = make_float2(0.f, 0.f), scores[b] = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[b][c] = patch.inside[b] ? pixel_value<kDropout>(a, patch.p[b], c) : 0.f;
+        }
     }
-    bool regular = true, have_totals = false;
-    for (int g = 0;;) {
-        const PatchRows rows = find_rows(
-            a.pixel_topk, patch, a.n, [&](const int p, const bool inside) { return sum_slots<kDropout>(a, p, inside); }, g, sm.keys);
-        float v[kPix][C];
-#pragma unroll
-        for (int b = 0; b < kPix; ++b)
-#pragma unroll
-            for (int c = 0; c < C; ++c) v[b][c] = patch.inside[b] && !have_totals ? pixel_value<kDropout>(a, patch.p[b], c) : 0.f;
-        regular = Rows::gather(rows, a.xys, a.conics, [&](const int id, const int c) { return row_value<kDropout>(a, id, c); }, sm.pairs) &&
-                  regular;
-        __syncwarp();
-        // a lane is kPix pixels: the group's weights, and the sums over all groups
+
+    // The group's weights into shared memory, and into the sums
+    __device__ __forceinline__ void add(const PatchRows &rows, const float4 *pairs, float *weight) {
+        weight += threadIdx.x & 31;
         unsigned held[kPix];
 #pragma unroll
         for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
 #pragma unroll 1
-        for (int pair = 0; 2 * pair < rows.n; ++pair) {
-            const float4 *q = sm.pairs + pair * kPairQuads;
-            float *weight = sm.weight + 2 * pair * kWeightPitch + lane;
+        for (int pair = 0; 2 * pair < rows.n; ++pair, pairs += Rows<C>::kPairQuads, weight += 2 * kWeightPitch) {
             float2 w[kPix];
-            Rows::weights(q, held, minus_x, minus_y, w);
+            Rows<C>::weights(pairs, held, minus_x, minus_y, w);
 #pragma unroll
             for (int b = 0; b < kPix; ++b) {
                 held[b] >>= 2;
                 weight[32 * b] = w[b].x, weight[kWeightPitch + 32 * b] = w[b].y;
-                float2 score = make_float2(0.f, 0.f);  // (unused the second time)
+                float2 score = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int c = 0; c < C; ++c) score = fma2(Rows::value(q, c), make_float2(v[b][c], v[b][c]), score);
-                total2[b] = add2(total2[b], w[b]);
-                scores2[b] = fma2(w[b], score, scores2[b]);
+                for (int c = 0; c < C; ++c) score = fma2(Rows<C>::value(pairs, c), make_float2(v[b][c], v[b][c]), score);
+                total[b] = add2(total[b], w[b]);
+                scores[b] = fma2(w[b], score, scores[b]);
             }
         }
-        if (!have_totals) {
-            if (rows.more) {
-                ++g;
-                continue;
-            }
-            bool finite = regular;
+    }
+
+    // v' and m' into shared memory; false, on all lanes, where one is not finite
+    __device__ __forceinline__ bool finish(float (&pixel)[C + 1][kPatchPixels]) {
+        bool finite = true;
 #pragma unroll
-            for (int b = 0; b < kPix; ++b) {
-                const float total = total2[b].x + total2[b].y, scores = scores2[b].x + scores2[b].y;
-                const bool some = total > 0.f;  // a pixel without a weight adds nothing, whatever its values
-                const float inv = reciprocal(total + (float)kNormEps), m = some ? scores * inv * inv : 0.f;
-                float size = fabsf(m);
+        for (int b = 0; b < kPix; ++b) {
+            const float t = total[b].x + total[b].y;
+            const bool some = t > 0.f;  // a pixel without a weight adds nothing, whatever its values
+            const float inv = reciprocal(t + (float)kNormEps), m = some ? (scores[b].x + scores[b].y) * inv * inv : 0.f;
+            float size = fabsf(m);
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float vc = some ? v[b][c] * inv : 0.f;
-                    size += fabsf(vc);
-                    sm.pixel[c][32 * b + lane] = vc;
-                }
-                sm.pixel[C][32 * b + lane] = m;
-                finite = finite && isfinite(size);
+            for (int c = 0; c < C; ++c) {
+                const float vc = some ? v[b][c] * inv : 0.f;
+                size += fabsf(vc);
+                pixel[c][32 * b + (threadIdx.x & 31)] = vc;
             }
-            if (!__all_sync(0xffffffffu, finite)) {
+            pixel[C][32 * b + (threadIdx.x & 31)] = m;
+            finite = finite && isfinite(size);
+        }
+        return __all_sync(0xffffffffu, finite);
+    }
+};
+
+// A lane is a row or, up to 16 rows, half of one: the group's sums into global memory
+template <int C, bool kDropout>
+__device__ __forceinline__ void add_rows(const SumArgs &a, const Patch &patch, const PatchRows &rows,
+                                         const typename SumSmem<C, kDropout>::Warp &sm) {
+    constexpr int kValues = SumLayout<C, kDropout>::kValues;
+    const int lane = threadIdx.x & 31;
+    const bool halves = rows.n <= 16;
+    const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
+    const int lines = halves ? kLines / 2 : kLines;
+    const float *mine = reinterpret_cast<const float *>(sm.pairs + (r >> 1) * Rows<C>::kPairQuads) + (r & 1);
+    auto field = [&](const int e) { return mine[2 * e]; };
+    const float x = field(0) - (float)patch.x0;
+    float dy = field(1) - (float)(patch.y0 + half * lines);
+    float2 dx[4], f[C], color[C];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dx[e] = make_float2(x - (float)(2 * e), x - (float)(2 * e + 1));
+#pragma unroll
+    for (int c = 0; c < C; ++c) f[c].x = -field(5 + c), f[c].y = f[c].x, color[c] = make_float2(0.f, 0.f);
+    float2 xx = make_float2(0.f, 0.f);
+    float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
+    const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *v_at = &sm.pixel[0][half * (kPatchPixels / 2)];
 #pragma unroll 1
-                for (int b = 0; b < kPix; ++b) add_slots<C, kDropout>(a, patch.p[b], patch.inside[b]);
-                return;
+    for (int line = 0; line < lines; ++line, dy -= 1.f, w_at += 8, v_at += 8) {
+        float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int quad = 0; quad < 2; ++quad) {
+            const float4 w4 = *reinterpret_cast<const float4 *>(w_at + quad * 4);
+            const float4 m4 = *reinterpret_cast<const float4 *>(v_at + C * kPatchPixels + quad * 4);
+            float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
+            const float2 w0 = make_float2(w4.x, w4.y), w1 = make_float2(w4.z, w4.w);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float4 v4 = *reinterpret_cast<const float4 *>(v_at + c * kPatchPixels + quad * 4);
+                const float2 v0 = make_float2(v4.x, v4.y), v1 = make_float2(v4.z, v4.w);
+                d0 = fma2(f[c], v0, d0), d1 = fma2(f[c], v1, d1);
+                if constexpr (kDropout) color[c] = fma2(w1, v1, fma2(w0, v0, color[c]));
             }
-            have_totals = true;
-            if (g > 0) {
-                g = 0;
-                continue;
-            }
+            const float2 t0 = mul2(w0, d0), t1 = mul2(w1, d1);
+            const float2 u0 = mul2(t0, dx[2 * quad]), u1 = mul2(t1, dx[2 * quad + 1]);
+            ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
+            xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
         }
+        const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
+        sx += ur, sy += ty;
+        sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
+    }
+    float sum[kValues];
+#pragma unroll
+    for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
+    sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
+    if constexpr (kDropout) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
+    }
+    const int id = __shfl_sync(0xffffffffu, rows.id, r);
+    if (halves) {
+#pragma unroll
+        for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
+    }
+    if (r < rows.n) {
+        float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)id * kValues);
+#pragma unroll
+        for (int e = 0; e < kValues / 4; ++e)
+            if (!halves || (e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
+    }
+}
+
+// A patch of more than 32 rows: all groups for the pixels' sums, then all again for the rows'
+template <int C, bool kDropout>
+__device__ __noinline__ bool sum_groups(const SumArgs &a, const Patch &patch, typename SumSmem<C, kDropout>::Warp &sm) {
+    PixelSums<C> pixels;
+    pixels.template start<kDropout>(a, patch);
+    for (int pass = 0; pass < 2; ++pass) {
+        bool more = true;
+        for (int g = 0; more; ++g) {
+            const PatchRows rows = sum_rows<C, kDropout>(a, patch, g, sm.keys);
+            more = rows.more;
+            if (!Rows<C>::gather(rows, a.xys, a.conics, [&](const int id, const int c) { return row_value<kDropout>(a, id, c); }, sm.pairs))
+                return false;
+            __syncwarp();
+            pixels.add(rows, sm.pairs, sm.weight);
+            __syncwarp();
+            if (pass == 1) add_rows<C, kDropout>(a, patch, rows, sm);
+        }
+        if (pass == 0 && !pixels.finish(sm.pixel)) return false;
         __syncwarp();
-        // a lane is a row or, up to 16 rows, half of one
-        const bool halves = rows.n <= 16;
-        const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
-        const int lines = halves ? kLines / 2 : kLines;
-        const float *mine = reinterpret_cast<const float *>(sm.pairs + (r >> 1) * kPairQuads) + (r & 1);
-        auto field = [&](const int e) { return mine[2 * e]; };
-        const float x = field(0) - (float)patch.x0;
-        float dy = field(1) - (float)(patch.y0 + half * lines);
-        float2 dx[4], f[C], color[C];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dx[e] = make_float2(x - (float)(2 * e), x - (float)(2 * e + 1));
-#pragma unroll
-        for (int c = 0; c < C; ++c) f[c].x = -field(5 + c), f[c].y = f[c].x, color[c] = make_float2(0.f, 0.f);
-        float2 xx = make_float2(0.f, 0.f);
-        float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
-        const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *v_at = &sm.pixel[0][half * (kPatchPixels / 2)];
+    }
+    return true;
+}
+
+template <int C, bool kDropout>
+__device__ __forceinline__ void sum_patch(const SumArgs &a) {
+    extern __shared__ __align__(16) char smem_bytes[];
+    typename SumSmem<C, kDropout>::Warp &sm = reinterpret_cast<SumSmem<C, kDropout> *>(smem_bytes)->warp[threadIdx.x >> 5];
+    const Patch patch(a.img_h, a.img_w);
+    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
+    const PatchRows rows = sum_rows<C, kDropout>(a, patch, 0, sm.keys);
+    bool regular;
+    if (rows.more) {
+        regular = sum_groups<C, kDropout>(a, patch, sm);
+    } else {
+        PixelSums<C> pixels;
+        pixels.template start<kDropout>(a, patch);
+        regular = Rows<C>::gather(rows, a.xys, a.conics, [&](const int id, const int c) { return row_value<kDropout>(a, id, c); }, sm.pairs);
+        __syncwarp();
+        pixels.add(rows, sm.pairs, sm.weight);
+        regular = pixels.finish(sm.pixel) && regular;
+        __syncwarp();
+        if (regular) add_rows<C, kDropout>(a, patch, rows, sm);
+    }
+    if (!regular) {
 #pragma unroll 1
-        for (int line = 0; line < lines; ++line, dy -= 1.f, w_at += 8, v_at += 8) {
-            float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int quad = 0; quad < 2; ++quad) {
-                const float4 w4 = *reinterpret_cast<const float4 *>(w_at + quad * 4);
-                const float4 m4 = *reinterpret_cast<const float4 *>(v_at + C * kPatchPixels + quad * 4);
-                float2 d0 = make_float2(m4.x, m4.y), d1 = make_float2(m4.z, m4.w);
-                const float2 w0 = make_float2(w4.x, w4.y), w1 = make_float2(w4.z, w4.w);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float4 v4 = *reinterpret_cast<const float4 *>(v_at + c * kPatchPixels + quad * 4);
-                    const float2 v0 = make_float2(v4.x, v4.y), v1 = make_float2(v4.z, v4.w);
-                    d0 = fma2(f[c], v0, d0), d1 = fma2(f[c], v1, d1);
-                    if constexpr (kDropout) color[c] = fma2(w1, v1, fma2(w0, v0, color[c]));
-                }
-                const float2 t0 = mul2(w0, d0), t1 = mul2(w1, d1);
-                const float2 u0 = mul2(t0, dx[2 * quad]), u1 = mul2(t1, dx[2 * quad + 1]);
-                ts = add2(ts, add2(t0, t1)), us = add2(us, add2(u0, u1));
-                xx = fma2(u1, dx[2 * quad + 1], fma2(u0, dx[2 * quad], xx));
-            }
-            const float tr = ts.x + ts.y, ur = us.x + us.y, ty = tr * dy;
-            sx += ur, sy += ty;
-            sxy = fmaf(ur, dy, sxy), syy = fmaf(ty, dy, syy);
-        }
-        float sum[kValues];
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) sum[e] = 0.f;
-        sum[0] = sx, sum[1] = sy, sum[2] = xx.x + xx.y, sum[3] = sxy, sum[4] = syy;
-        if constexpr (kDropout) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) sum[5 + c] = color[c].x + color[c].y;
-        }
-        const int id = __shfl_sync(0xffffffffu, rows.id, r);
-        if (halves) {
-#pragma unroll
-            for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
-        }
-        if (r < rows.n) {
-            float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)id * kValues);
-#pragma unroll
-            for (int e = 0; e < kValues / 4; ++e)
-                if (!halves || (e & 1) == half) atomicAdd(&out[e], make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]));
-        }
-        if (!rows.more) return;
-        ++g;
+        for (int b = 0; b < kPix; ++b) add_slots<C, kDropout>(a, patch.p[b], patch.inside[b]);
     }
 }
 
