@@ -137,7 +137,7 @@ __device__ __forceinline__ void invert_totals(BalanceSmem &sm, const float2 (&to
 __device__ __forceinline__ void count_rows(const BalanceArgs &a, const igs::PatchRows &rows, const BalanceSmem &sm) {
     const int lane = threadIdx.x & 31;
     const bool halves = rows.n <= 16;
-    const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
+    const int r = halves ? lane & 15 : min(lane, igs::kRows - 1), half = halves ? lane >> 4 : 0;
     const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *inv_at = sm.inv + half * (kPatchPixels / 2);
     float sum = 0.f;
 #pragma unroll 4
@@ -148,7 +148,7 @@ __device__ __forceinline__ void count_rows(const BalanceArgs &a, const igs::Patc
     }
     const int id = __shfl_sync(0xffffffffu, rows.id, r);
     if (halves) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-    if (half == 0 && r < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
+    if (half == 0 && (halves ? r : lane) < rows.n) atomicAdd(&a.fixed[id], (unsigned long long)__float2ll_rn(sum * a.scale));
     if (lane < rows.n) atomicAdd(&a.counts[rows.id], rows.holders);
 }
 
@@ -230,7 +230,7 @@ __device__ __forceinline__ void finish_loss(const BalanceArgs &a, const double f
 
 // kFinish: the last CTA finishes
 template <bool kFinish>
-__global__ void __launch_bounds__(igs::kPatchThreads, 5) balance_kernel(const __grid_constant__ BalanceArgs a) {
+__global__ void __launch_bounds__(igs::kPatchThreads, 6) balance_kernel(const __grid_constant__ BalanceArgs a) {
     __shared__ BalanceSmem smem[igs::kPatches];
     igs::wait_for_predecessor();
     count_patch(a, smem[threadIdx.x >> 5]);

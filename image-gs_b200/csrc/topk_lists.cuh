@@ -65,7 +65,8 @@ struct KeptSlots {
 // are read once, by a lane each, and laid side by side in pairs, so that the warp reads them as broadcasts, two rows per packed (f32x2)
 // instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need no other warp, so nothing waits at a
 // barrier. (The tile's IDs collected by its eight warps in one hash table took twice the instructions, and half the time at barriers.)
-constexpr int kRows = 32;  // rows of a group: a patch with more goes over them group by group
+constexpr int kRows = 28;  // rows of a group: a patch with more goes over them group by group
+constexpr unsigned kRowsEnd = kRows < 32 ? 1u << (kRows & 31) : 0u;
 // The patch of a warp: 8 pixels by kLines, kPix of a lane, one above the other, four lines apart
 constexpr int kPix = 2;
 constexpr int kLines = 4 * kPix;
@@ -176,9 +177,9 @@ __device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const Patc
         }
         if (bit == mine) rows.id = id;
         bit <<= 1;
-    } while (bit != 0);
-    rows.n = bit != 0 ? __ffs(bit) - 1 : kRows;
-    rows.more = bit == 0 && smallest() != none;
+    } while (bit != kRowsEnd);
+    rows.n = bit != kRowsEnd ? __ffs(bit) - 1 : kRows;
+    rows.more = bit == kRowsEnd && smallest() != none;
 #pragma unroll
     for (int b = 0; b < kPix; ++b) rows.holders += __popc(holders[b]);
     __syncwarp();
@@ -266,7 +267,7 @@ struct Rows {
             for (int c = 0; c < C; ++c) q[5 + c] = value(rows.id, c), size += fabsf(q[5 + c]);
             good = g.regular && isfinite(size);
         }
-        if (lane <= rows.n) {  // one more, of zeros, to pad the last pair
+        if (lane <= rows.n && lane < kRows) {  // one more, of zeros, to pad the last pair
             float *pair = reinterpret_cast<float *>(pairs + (lane >> 1) * kPairQuads) + (lane & 1);
 #pragma unroll
             for (int e = 0; e < 5 + C; ++e) pair[2 * e] = q[e];

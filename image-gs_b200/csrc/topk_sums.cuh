@@ -229,7 +229,7 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Patch &patch, c
     constexpr int kValues = SumLayout<C, kDropout>::kValues;
     const int lane = threadIdx.x & 31;
     const bool halves = rows.n <= 16;
-    const int r = halves ? lane & 15 : lane, half = halves ? lane >> 4 : 0;
+    const int r = halves ? lane & 15 : min(lane, kRows - 1), half = halves ? lane >> 4 : 0;
     const int lines = halves ? kLines / 2 : kLines;
     const float *mine = reinterpret_cast<const float *>(sm.pairs + (r >> 1) * Rows<C>::kPairQuads) + (r & 1);
     auto field = [&](const int e) { return mine[2 * e]; };
@@ -281,7 +281,7 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Patch &patch, c
 #pragma unroll
         for (int e = 0; e < 5 + (kDropout ? C : 0); ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
     }
-    if (r < rows.n) {
+    if ((halves ? r : lane) < rows.n) {
         float4 *out = reinterpret_cast<float4 *>(a.sums + (size_t)id * kValues);
 #pragma unroll
         for (int e = 0; e < kValues / 4; ++e)
@@ -341,7 +341,7 @@ __device__ __forceinline__ void sum_patch(const SumArgs &a) {
 // kFinish: the last CTA finishes the gradients. (A kernel of its own: with the barrier behind it, even never reached, the patch's code took
 // 18 % more instructions.)
 template <int C, bool kDropout, bool kFinish>
-__global__ void __launch_bounds__(kPatchThreads, C <= 3 ? 5 : 4) sums_kernel(const __grid_constant__ SumArgs a) {
+__global__ void __launch_bounds__(kPatchThreads, C <= 1 ? 6 : C <= 3 ? 5 : 4) sums_kernel(const __grid_constant__ SumArgs a) {
     wait_for_predecessor();
     sum_patch<C, kDropout>(a);
     if constexpr (kFinish) {
