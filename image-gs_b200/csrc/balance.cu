@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kThreads) balance_zero_kernel(const __grid_con
 }
 
 // One pixel's slots one by one, from global memory (topk_sums.cuh says when)
-__device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
+__device__ __forceinline__ void count_pixel_slots(const BalanceArgs &a, const int p) {
     if (a.mask != nullptr && a.mask[p] == 0) return;
     const float px = (float)(p % a.img_w), py = (float)(p / a.img_w);
     const int *list = a.pixel_topk + (size_t)p * igs::kTopK;
@@ -88,6 +88,13 @@ __device__ __noinline__ void count_slots(const BalanceArgs &a, const int p) {
             }
         }
     }
+}
+
+__device__ __noinline__ void count_slots(const BalanceArgs &a) {
+    const igs::Patch patch(a.img_h, a.img_w);  // (made again: passed from the caller, it would live in the caller's local memory)
+#pragma unroll
+    for (int b = 0; b < kPix; ++b)
+        if (patch.inside[b]) count_pixel_slots(a, patch.p[b]);
 }
 
 struct BalanceSmem {
@@ -153,7 +160,8 @@ __device__ __forceinline__ void count_rows(const BalanceArgs &a, const igs::Patc
 }
 
 // A patch of more than 32 rows: all groups for the pixels' sums, then all again for the rows'
-__device__ __noinline__ bool count_groups(const BalanceArgs &a, const igs::Patch &patch, BalanceSmem &sm) {
+__device__ __noinline__ bool count_groups(const BalanceArgs &a, BalanceSmem &sm) {
+    const igs::Patch patch(a.img_h, a.img_w);
     float2 total[kPix] = {};
     for (int pass = 0; pass < 2; ++pass) {
         bool more = true;
@@ -182,7 +190,7 @@ __device__ __forceinline__ void count_patch(const BalanceArgs &a, BalanceSmem &s
         atomicAdd(&a.ws->routed[(blockIdx.x + blockIdx.y) % kRoutedSlots], (unsigned long long)routed);
     bool regular;
     if (rows.more) {
-        regular = count_groups(a, patch, sm);
+        regular = count_groups(a, sm);
     } else {
         regular = Rows::gather(rows, a.xys, a.conics, [](int, int) { return 0.f; }, sm.pairs);
         __syncwarp();
@@ -192,11 +200,7 @@ __device__ __forceinline__ void count_patch(const BalanceArgs &a, BalanceSmem &s
         __syncwarp();
         if (regular) count_rows(a, rows, sm);
     }
-    if (!regular) {
-#pragma unroll 1
-        for (int b = 0; b < kPix; ++b)
-            if (patch.inside[b]) count_slots(a, patch.p[b]);
-    }
+    if (!regular) count_slots(a);
 }
 
 // The sum over the CTA, in one order, on all threads; s_sum: a word per warp

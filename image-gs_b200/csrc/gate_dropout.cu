@@ -25,7 +25,7 @@ struct DropoutArgs {
 };
 
 // One pixel's slots one by one, from global memory
-__device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p) {
+__device__ __forceinline__ void blend_pixel_slots(const DropoutArgs &a, const int p) {
     const igs::KeptSlots kept({(uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold}, (uint32_t)p, true);
     unsigned keep = 0;
 #pragma unroll
@@ -46,6 +46,13 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a, const int p) {
         }
         out[c * plane] = pix / total;
     }
+}
+
+__device__ __noinline__ void blend_slots(const DropoutArgs &a) {
+    const igs::Patch patch(a.img_h, a.img_w);  // (made again: passed from the caller, it would live in the caller's local memory)
+#pragma unroll
+    for (int b = 0; b < kPix; ++b)
+        if (patch.inside[b]) blend_pixel_slots(a, patch.p[b]);
 }
 
 // A warp is a patch, a lane its pixels
@@ -78,9 +85,7 @@ __global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 
         const bool regular = Rows::gather(
             rows, a.xys, a.conics, [&](const int id, const int c) { return __ldg(&a.colors[(size_t)id * C + c]); }, sm.pairs);
         if (!regular) {  // among others, zero times a colour that is not finite would reach pixels that do not name it
-#pragma unroll 1
-            for (int b = 0; b < kPix; ++b)
-                if (patch.inside[b]) blend_slots(a, patch.p[b]);
+            blend_slots(a);
             return;
         }
         __syncwarp();

@@ -74,7 +74,7 @@ __device__ __forceinline__ auto sum_slots(const SumArgs &a, const int p, const b
 
 // One pixel's slots one by one, from global memory: a slot of weight 0 adds nothing
 template <int C, bool kDropout>
-__device__ __noinline__ void add_slots(const SumArgs &a, const int p, const bool inside) {
+__device__ __forceinline__ void add_pixel_slots(const SumArgs &a, const int p, const bool inside) {
     const auto may = sum_slots<kDropout>(a, p, inside);
     if (!may.any()) return;
     unsigned keep = 0;
@@ -152,6 +152,13 @@ __global__ void __launch_bounds__(256) finish_sums_kernel(const __grid_constant_
     wait_for_predecessor();
     const int g = blockIdx.x * 256 + threadIdx.x;
     if (g < a.n) finish_gaussian<C, kDropout>(a, g);
+}
+
+template <int C, bool kDropout>
+__device__ __noinline__ void add_slots(const SumArgs &a) {
+    const Patch patch(a.img_h, a.img_w);  // (made again: passed from the caller, it would live in the caller's local memory)
+#pragma unroll
+    for (int b = 0; b < kPix; ++b) add_pixel_slots<C, kDropout>(a, patch.p[b], patch.inside[b]);
 }
 
 template <int C, bool kDropout>
@@ -291,7 +298,8 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Patch &patch, c
 
 // A patch of more than 32 rows: all groups for the pixels' sums, then all again for the rows'
 template <int C, bool kDropout>
-__device__ __noinline__ bool sum_groups(const SumArgs &a, const Patch &patch, typename SumSmem<C, kDropout>::Warp &sm) {
+__device__ __noinline__ bool sum_groups(const SumArgs &a, typename SumSmem<C, kDropout>::Warp &sm) {
+    const Patch patch(a.img_h, a.img_w);
     PixelSums<C> pixels;
     pixels.template start<kDropout>(a, patch);
     for (int pass = 0; pass < 2; ++pass) {
@@ -321,7 +329,7 @@ __device__ __forceinline__ void sum_patch(const SumArgs &a) {
     const PatchRows rows = sum_rows<C, kDropout>(a, patch, 0, sm.keys);
     bool regular;
     if (rows.more) {
-        regular = sum_groups<C, kDropout>(a, patch, sm);
+        regular = sum_groups<C, kDropout>(a, sm);
     } else {
         PixelSums<C> pixels;
         pixels.template start<kDropout>(a, patch);
@@ -332,10 +340,7 @@ __device__ __forceinline__ void sum_patch(const SumArgs &a) {
         __syncwarp();
         if (regular) add_rows<C, kDropout>(a, patch, rows, sm);
     }
-    if (!regular) {
-#pragma unroll 1
-        for (int b = 0; b < kPix; ++b) add_slots<C, kDropout>(a, patch.p[b], patch.inside[b]);
-    }
+    if (!regular) add_slots<C, kDropout>(a);
 }
 
 // kFinish: the last CTA finishes the gradients. (A kernel of its own: with the barrier behind it, even never reached, the patch's code took
