@@ -55,67 +55,110 @@ __device__ __noinline__ void blend_slots(const DropoutArgs &a) {
         if (patch.inside[b]) blend_pixel_slots(a, patch.p[b]);
 }
 
-// A warp is a patch, a lane its pixels
 template <int C>
-__global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 7 : C <= 7 ? 6 : 5) dropout_kernel(const __grid_constant__ DropoutArgs a) {
-    using Rows = igs::Rows<C>;
-    __shared__ struct {
-        int keys[igs::kKeyWords];
-        float4 pairs[Rows::kGroupQuads];
-    } smem[igs::kPatches];
-    auto &sm = smem[threadIdx.x >> 5];
-    igs::wait_for_predecessor();
-    const long long seed = a.rng[0], offset = a.rng[1];
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.rng_used[0] = seed, a.rng_used[1] = offset;
-    const igs::Patch patch(a.img_h, a.img_w);
-    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
-    const auto slots = [&](const int p, const bool inside) {
-        return igs::KeptSlots({(uint64_t)seed, (uint64_t)offset, a.threshold}, (uint32_t)p, inside);
-    };
-    const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
-    float2 minus_y[kPix], total[kPix], pix[kPix][C];
+struct DropoutSmem {
+    int keys[igs::kKeyWords];
+    float4 pairs[igs::Rows<C>::kGroupQuads];
+};
+
+__device__ __forceinline__ igs::PatchRows dropout_rows(const DropoutArgs &a, const igs::Patch &patch, const int g, int *keys) {
+    return igs::find_rows(
+        a.pixel_topk, patch, a.n,
+        [&](const int p, const bool inside) {
+            return igs::KeptSlots({(uint64_t)a.rng[0], (uint64_t)a.rng[1], a.threshold}, (uint32_t)p, inside);
+        },
+        g, keys);
+}
+
+template <int C>
+__device__ __forceinline__ bool dropout_gather(const DropoutArgs &a, const igs::PatchRows &rows, float4 *pairs) {
+    return igs::Rows<C>::gather(
+        rows, a.xys, a.conics, [&](const int id, const int c) { return __ldg(&a.colors[(size_t)id * C + c]); }, pairs);
+}
+
+// A lane is its pixels: their weights' and weighted colours' sums over the rows
+template <int C>
+struct Blend {
+    float2 total[kPix], pix[kPix][C];
+    __device__ __forceinline__ Blend() {
 #pragma unroll
-    for (int b = 0; b < kPix; ++b) {
-        minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), total[b] = make_float2(0.f, 0.f);
+        for (int b = 0; b < kPix; ++b) {
+            total[b] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < C; ++c) pix[b][c] = make_float2(0.f, 0.f);
-    }
-    for (int g = 0;; ++g) {
-        const igs::PatchRows rows = igs::find_rows(a.pixel_topk, patch, a.n, slots, g, sm.keys);
-        const bool regular = Rows::gather(
-            rows, a.xys, a.conics, [&](const int id, const int c) { return __ldg(&a.colors[(size_t)id * C + c]); }, sm.pairs);
-        if (!regular) {  // among others, zero times a colour that is not finite would reach pixels that do not name it
-            blend_slots(a);
-            return;
+            for (int c = 0; c < C; ++c) pix[b][c] = make_float2(0.f, 0.f);
         }
-        __syncwarp();
+    }
+    __device__ __forceinline__ void add(const igs::Patch &patch, const igs::PatchRows &rows, const float4 *pairs) {
+        const float2 minus_x = make_float2(-(float)patch.j, -(float)patch.j);
+        float2 minus_y[kPix];
         unsigned held[kPix];
 #pragma unroll
-        for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
+        for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), held[b] = rows.bits[b];
 #pragma unroll 1
-        for (int pair = 0; 2 * pair < rows.n; ++pair) {
-            const float4 *q = sm.pairs + pair * Rows::kPairQuads;
+        for (int pair = 0; 2 * pair < rows.n; ++pair, pairs += igs::Rows<C>::kPairQuads) {
             float2 w[kPix];
-            Rows::weights(q, held, minus_x, minus_y, w);
+            igs::Rows<C>::weights(pairs, held, minus_x, minus_y, w);
 #pragma unroll
             for (int b = 0; b < kPix; ++b) {
                 held[b] >>= 2;
                 total[b] = igs::add2(total[b], w[b]);
 #pragma unroll
-                for (int c = 0; c < C; ++c) pix[b][c] = igs::fma2(w[b], Rows::value(q, c), pix[b][c]);
+                for (int c = 0; c < C; ++c) pix[b][c] = igs::fma2(w[b], igs::Rows<C>::value(pairs, c), pix[b][c]);
             }
         }
-        if (!rows.more) break;
     }
-    const size_t plane = (size_t)a.img_h * a.img_w;
+    __device__ __forceinline__ void store(const DropoutArgs &a, const igs::Patch &patch) const {
+        const size_t plane = (size_t)a.img_h * a.img_w;
 #pragma unroll
-    for (int b = 0; b < kPix; ++b) {
-        if (!patch.inside[b]) continue;
-        const float inv = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
+        for (int b = 0; b < kPix; ++b) {
+            if (!patch.inside[b]) continue;
+            const float inv = igs::reciprocal(total[b].x + total[b].y + (float)igs::kNormEps);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            a.out_img[c * plane + patch.p[b]] = (pix[b][c].x + pix[b][c].y) * inv;
+            for (int c = 0; c < C; ++c) a.out_img[c * plane + patch.p[b]] = (pix[b][c].x + pix[b][c].y) * inv;
+        }
     }
+};
+
+// A patch of more rows than a group's
+template <int C>
+__device__ __noinline__ bool blend_groups(const DropoutArgs &a, DropoutSmem<C> &sm) {
+    const igs::Patch patch(a.img_h, a.img_w);
+    Blend<C> blend;
+    bool more = true;
+    for (int g = 0; more; ++g) {
+        const igs::PatchRows rows = dropout_rows(a, patch, g, sm.keys);
+        more = rows.more;
+        if (!dropout_gather<C>(a, rows, sm.pairs)) return false;
+        __syncwarp();
+        blend.add(patch, rows, sm.pairs);
+    }
+    blend.store(a, patch);
+    return true;
+}
+
+// A warp is a patch
+template <int C>
+__global__ void __launch_bounds__(igs::kPatchThreads, C <= 3 ? 8 : C <= 7 ? 7 : 6) dropout_kernel(const __grid_constant__ DropoutArgs a) {
+    __shared__ DropoutSmem<C> smem[igs::kPatches];
+    DropoutSmem<C> &sm = smem[threadIdx.x >> 5];
+    igs::wait_for_predecessor();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 2) a.rng_used[threadIdx.x] = a.rng[threadIdx.x];
+    const igs::Patch patch(a.img_h, a.img_w);
+    if (patch.x0 >= a.img_w || patch.y0 >= a.img_h) return;
+    const igs::PatchRows rows = dropout_rows(a, patch, 0, sm.keys);
+    bool regular;
+    if (rows.more) {
+        regular = blend_groups<C>(a, sm);
+    } else {
+        regular = dropout_gather<C>(a, rows, sm.pairs);
+        __syncwarp();
+        if (regular) {
+            Blend<C> blend;
+            blend.add(patch, rows, sm.pairs);
+            blend.store(a, patch);
+        }
+    }
+    if (!regular) blend_slots(a);  // among others, zero times a colour that is not finite would reach pixels that do not name it
 }
 
 __global__ void rng_used_kernel(const long long *rng, long long *rng_used) {
