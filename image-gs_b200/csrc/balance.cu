@@ -121,7 +121,7 @@ __device__ __forceinline__ void weigh_rows(const igs::PatchRows &rows, const igs
     for (int b = 0; b < kPix; ++b) minus_y[b] = make_float2(-(float)patch.i[b], -(float)patch.i[b]), held[b] = rows.bits[b];
     const float4 *pairs = sm.pairs;
     float *weight = sm.weight + (threadIdx.x & 31);
-#pragma unroll 1
+#pragma unroll 2
     for (int pair = 0; 2 * pair < rows.n; ++pair, pairs += Rows::kPairQuads, weight += 2 * kWeightPitch) {
         float2 w[kPix];
         Rows::weights(pairs, held, minus_x, minus_y, w);

@@ -190,7 +190,7 @@ struct PixelSums {
         unsigned held[kPix];
 #pragma unroll
         for (int b = 0; b < kPix; ++b) held[b] = rows.bits[b];
-#pragma unroll 1
+#pragma unroll 2
         for (int pair = 0; 2 * pair < rows.n; ++pair, pairs += Rows<C>::kPairQuads, weight += 2 * kWeightPitch) {
             float2 w[kPix];
             Rows<C>::weights(pairs, held, minus_x, minus_y, w);
@@ -250,7 +250,7 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Patch &patch, c
     float2 xx = make_float2(0.f, 0.f);
     float sx = 0.f, sy = 0.f, sxy = 0.f, syy = 0.f;
     const float *w_at = sm.weight + r * kWeightPitch + half * (kPatchPixels / 2), *v_at = &sm.pixel[0][half * (kPatchPixels / 2)];
-#pragma unroll 1
+#pragma unroll 4
     for (int line = 0; line < lines; ++line, dy -= 1.f, w_at += 8, v_at += 8) {
         float2 ts = make_float2(0.f, 0.f), us = make_float2(0.f, 0.f);
 #pragma unroll
