@@ -299,32 +299,37 @@ def _run(dev, name, *args):
     """One entry point on dev's current stream, the arguments (tensors as pointers) before the stream. These operators are used on small
     images too, where the host's time is the time: the device is only changed where it is not the current one."""
     args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    call = getattr(_lib.load(), name)
     if torch.cuda.current_device() == dev.index:
-        _lib_call(name, *args, stream_of(dev))
+        status = call(*args, stream_of(dev))
     else:
         with torch.cuda.device(dev):
-            _lib_call(name, *args, stream_of(dev))
+            status = call(*args, stream_of(dev))
+    if status:
+        check(status, name)
 
 
-def _check_lists(img_height, img_width, xys, conics, pixel_topk, **others):
-    """The inputs shared by the operators over pixel_topk: shapes, types, one device. Returns (H, W, N, device)."""
+def _check_lists(img_height, img_width, xys, conics, pixel_topk, *others):
+    """The inputs shared by the operators over pixel_topk: shapes, types, one device (others: further tensors, or None). Returns
+    (H, W, N, device)."""
     h, w = int(img_height), int(img_width)
     if h < 0 or w < 0:
         raise ValueError(f"negative image size {w}x{h}")
     _check_input(xys, "xys", torch.float32)
     _check_input(conics, "conics", torch.float32)
     _check_input(pixel_topk, "pixel_topk", torch.int32)
-    if xys.ndim != 2 or xys.size(1) != 2:
+    n = xys.size(0) if xys.ndim == 2 else -1
+    if n < 0 or xys.size(1) != 2:
         raise RuntimeError("xys must have dimensions (num_points, 2)")
-    n = xys.size(0)
-    if tuple(conics.shape) != (n, 3):
+    if conics.ndim != 2 or conics.size(0) != n or conics.size(1) != 3:
         raise RuntimeError("conics must have dimensions (num_points, 3)")
     if pixel_topk.numel() != h * w * TOP_K:
         raise RuntimeError("pixel_topk must be [H, W, TOP_K]")
-    for name, t in dict(conics=conics, pixel_topk=pixel_topk, **others).items():
-        if t is not None and t.device != xys.device:
-            raise RuntimeError(f"{name} must be on {xys.device}, as xys")
-    return h, w, n, xys.device
+    dev = xys.device
+    for t in (conics, pixel_topk) + others:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"every tensor must be on {dev}, as xys; got one on {t.device}")
+    return h, w, n, dev
 
 
 def _check_mask(pixel_mask, h, w):
@@ -342,7 +347,7 @@ def topk_balance_forward(img_height, img_width, xys, conics, pixel_topk, pixel_m
     pixel_topk that hold each Gaussian, importance the sum of their gates exp(-sigma) / (sum + 1e-4), totals the filled slots A and the
     pixels T with one, loss = N / (A T) * sum(counts * importance): 1 for an even spread, 0 without slots. pixel_mask [H, W] (bool or uint8)
     leaves pixels out. The results do not depend on the order of the atomics."""
-    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, pixel_mask=pixel_mask)
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, pixel_mask)
     _check_mask(pixel_mask, h, w)
     loss = torch.empty((), device=dev, dtype=torch.float32)
     counts = torch.empty(n, device=dev, dtype=torch.int32)
@@ -350,8 +355,7 @@ def topk_balance_forward(img_height, img_width, xys, conics, pixel_topk, pixel_m
     totals = torch.empty(2, device=dev, dtype=torch.int64)
     ws_bytes = _lib.load().igs_topk_balance_workspace(n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_balance_fwd", h, w, n, xys, conics, pixel_topk, pixel_mask, loss, counts,
-         importance, totals, ws, ws_bytes)
+    _run(dev, "igs_topk_balance_fwd", h, w, n, xys, conics, pixel_topk, pixel_mask, loss, counts, importance, totals, ws, ws_bytes)
     return loss, counts, importance, totals
 
 
@@ -359,8 +363,7 @@ def topk_balance_backward(img_height, img_width, xys, conics, pixel_topk, counts
                           pixel_mask=None):
     """v_xy [N, 2], v_conic [N, 3] of grad_loss * loss + sum(grad_importance * importance), the counts held constant; counts, totals and
     pixel_mask as topk_balance_forward returned and took them, grad_loss a device scalar, grad_importance [N]."""
-    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, counts=counts, totals=totals, grad_loss=grad_loss,
-                                grad_importance=grad_importance, pixel_mask=pixel_mask)
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, counts, totals, grad_loss, grad_importance, pixel_mask)
     _check_mask(pixel_mask, h, w)
     _check_input(counts, "counts", torch.int32)
     _check_input(totals, "totals", torch.int64)
@@ -374,12 +377,11 @@ def topk_balance_backward(img_height, img_width, xys, conics, pixel_topk, counts
         _check_input(grad_importance, "grad_importance", torch.float32)
         if grad_importance.numel() != n:
             raise RuntimeError("grad_importance must be [N]")
-    v_xy = torch.empty(n, 2, device=dev, dtype=torch.float32)
-    v_conic = torch.empty(n, 3, device=dev, dtype=torch.float32)
+    v_xy, v_conic = torch.empty_like(xys), torch.empty_like(conics)
     ws_bytes = _lib.load().igs_topk_balance_workspace(n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_balance_bwd", h, w, n, xys, conics, pixel_topk, pixel_mask, counts, totals,
-         grad_loss, grad_importance, 0, v_xy, v_conic, ws, ws_bytes)
+    _run(dev, "igs_topk_balance_bwd", h, w, n, xys, conics, pixel_topk, pixel_mask, counts, totals, grad_loss,
+         grad_importance, 0, v_xy, v_conic, ws, ws_bytes)
     return v_xy, v_conic
 
 
@@ -404,7 +406,7 @@ def topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk,
     (a pixel with nothing left is 0), and rng_used [2], the seed and offset that the pass saw in rng_state (int64 [2] on the device): the
     backward pass takes rng_used, and draws the same mask from it. Move the offset on between passes (rng_state[1] += 1, in a captured graph
     too) for a new mask."""
-    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, colors=colors, rng_state=rng_state)
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, colors, rng_state)
     channels, p = _check_dropout(h, w, n, colors, p, rng_state)
     out_img = torch.empty(channels, h, w, device=dev, dtype=torch.float32)
     rng_used = torch.empty(2, device=dev, dtype=torch.int64)
@@ -414,16 +416,16 @@ def topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk,
 
 def topk_dropout_backward(img_height, img_width, xys, conics, colors, v_output, pixel_topk, p, rng_used):
     """v_xy [N, 2], v_conic [N, 3], v_colors [N, C] of topk_dropout_forward, for v_output [C, H, W] and the rng_used it returned."""
-    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, colors=colors, v_output=v_output, rng_used=rng_used)
+    h, w, n, dev = _check_lists(img_height, img_width, xys, conics, pixel_topk, colors, v_output, rng_used)
     channels, p = _check_dropout(h, w, n, colors, p, rng_used)
     _check_input(v_output, "v_output", torch.float32)
     if v_output.numel() != channels * h * w:
         raise RuntimeError("v_output must be [C, H, W]")
-    v_xy, v_conic, v_colors = (torch.empty(n, c, device=dev, dtype=torch.float32) for c in (2, 3, channels))
+    v_xy, v_conic, v_colors = torch.empty_like(xys), torch.empty_like(conics), torch.empty_like(colors)
     ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_dropout_bwd", h, w, channels, n, xys, conics, colors, v_output, pixel_topk, p,
-         rng_used, v_xy, v_conic, v_colors, ws, ws_bytes)
+    _run(dev, "igs_topk_dropout_bwd", h, w, channels, n, xys, conics, colors, v_output, pixel_topk, p, rng_used,
+         v_xy, v_conic, v_colors, ws, ws_bytes)
     return v_xy, v_conic, v_colors
 
 
