@@ -159,7 +159,7 @@ __device__ __forceinline__ void count_rows(const BalanceArgs &a, const igs::Patc
     if (lane < rows.n) atomicAdd(&a.counts[rows.id], rows.holders);
 }
 
-// A patch of more than 32 rows: all groups for the pixels' sums, then all again for the rows'
+// A patch of more rows than a group: all groups for the pixels' sums, then all again for the rows'
 __device__ __noinline__ bool count_groups(const BalanceArgs &a, BalanceSmem &sm) {
     const igs::Patch patch(a.img_h, a.img_w);
     float2 total[kPix] = {};

@@ -22,20 +22,21 @@ __device__ __forceinline__ uint4 philox4x32(uint4 c, uint2 key) {
     return c;
 }
 
-// Which slots of a pixel may be filled: all of them (one bit says whether the pixel counts at all), or those that a dropout draw keeps
+// Which slots of a pixel may be filled: all of them (counts says whether the pixel does at all), or those that a dropout draw keeps
 struct AllSlots {
     bool counts;
     __device__ __forceinline__ bool any() const { return counts; }
     __device__ __forceinline__ bool operator()(int) const { return true; }
 };
 
-// The ten 24-bit draws of a pixel, kept where they are not below a threshold. Two calls give eight words: slot k < 8 takes the upper 24
-// bits of word k, slots 8 and 9 the low bytes of words 0, 1, 2 and 3, 4, 5 (the first most significant), which no other slot uses; a third
-// call for two slots would cost half as much again.
 struct Dropout {
     uint64_t seed, offset;
     uint32_t threshold;  // rint(p 2^24)
 };
+
+// The ten 24-bit draws of a pixel, kept where they are not below the threshold. Two calls give eight words: slot k < 8 takes the upper 24
+// bits of word k, slots 8 and 9 the low bytes of words 0, 1, 2 and 3, 4, 5 (the first most significant), which no other slot uses; a third
+// call for two slots would cost half as much again.
 struct KeptSlots {
     uint32_t words[8];
     uint32_t threshold;
@@ -59,14 +60,26 @@ struct KeptSlots {
 // ---- a patch's Gaussians as rows -------------------------------------------------------------------------------------------------------
 //
 // A warp takes an 8x8 patch of pixels, a lane two of them. Neighbouring pixels name nearly the same Gaussians (at a trained image's 100
-// pixels per Gaussian the 640 slots of a patch name 14 to 16, those of an 8x4 patch 13 to 14), so the patch's distinct IDs become rows, in the order of their IDs: every lane
-// sorts its pixels' ten slots (a 29-comparator network) into shared memory, and the warp then takes the smallest unconsumed ID of all its pixels
-// again and again. An ID twice in one list becomes two rows. What a row means to a pixel is a bit of the lane's mask; the rows' parameters
-// are read once, by a lane each, and laid side by side in pairs, so that the warp reads them as broadcasts, two rows per packed (f32x2)
-// instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need no other warp, so nothing waits at a
-// barrier. (The tile's IDs collected by its eight warps in one hash table took twice the instructions, and half the time at barriers.)
+// pixels per Gaussian the 640 slots of a patch name 14 to 16, those of an 8x4 patch 13 to 14), so the patch's distinct IDs become rows, in
+// the order of their IDs: every lane sorts its pixels' ten slots (a 29-comparator network) into shared memory, and the warp takes the
+// smallest unconsumed ID of all its pixels again and again. An ID twice in one list becomes two rows. What a row means to a pixel is a bit
+// of the lane's mask; the rows' parameters are read once, by a lane each, and laid side by side in pairs, so that the warp reads them as
+// broadcasts, two rows per packed (f32x2) instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need
+// no other warp, so nothing waits at a barrier.
+//
+// The kernels are bound by instruction issue and the shared-memory pipe (60 to 75 % of both, DRAM 15 to 20 %): of a patch's 1150
+// instructions (counts and importance), 210 load the lists, 120 sort, 410 walk to the rows, 330 weigh, 80 sum along the rows. Measured on
+// the way, counts and importance of 1920x1080 pixels and 20,000 Gaussians: one thread per pixel and an atomic per slot 330 us; the tile's
+// IDs collected by its warps in one hash table in shared memory 88 us (twice the instructions, and time at barriers); patches of 8x4 pixels
+// 63 us; 8x8 57 us.
+//
+// kRows is the shared memory of a patch's weights against the patches that do not fit it: 32 rows leave 5 CTAs on an SM, 28 leave 6 (125
+// and 118 us for both passes of the balance loss at 100 pixels per Gaussian, 142 and 137 at 40, 153 and 171 at 25), 24 leave 7 (116, 157
+// and 262 us).
 constexpr int kRows = 28;  // rows of a group: a patch with more goes over them group by group
-constexpr unsigned kRowsEnd = kRows < 32 ? 1u << (kRows & 31) : 0u;
+constexpr unsigned kRowsEnd = 1u << kRows;
+static_assert(kRows % 2 == 0 && kRows < 32, "whole pairs, and a bit for each row with one to spare");
+
 // The patch of a warp: 8 pixels by kLines, kPix of a lane, one above the other, four lines apart
 constexpr int kPix = 2;
 constexpr int kLines = 4 * kPix;
@@ -105,9 +118,9 @@ __device__ __forceinline__ void sort_slots(int (&key)[kTopK]) {
     }
 }
 
-// Rows [32 g, 32 g + 32) of the patch
+// Rows [kRows g, kRows (g + 1)) of the patch
 struct PatchRows {
-    int n;                // how many there are, at most 32
+    int n;                // how many there are, at most kRows
     bool more;            // whether others follow
     unsigned bits[kPix];  // the rows that this lane's pixels hold
     int id;               // lane l < n: the ID of row l,
@@ -196,8 +209,10 @@ __device__ __forceinline__ float exp2_approx(const float x) {
 // A Gaussian's geometry as the kernels use it: centre, and the conic times -log2(e) (its outer terms halved too), so that the weight is
 // exp2 of
 //   (a' dx) dx + (c' dy + b' dx) dy
-// With a positive definite conic that is never positive (but for its rounding) and needs no test. Other conics, and parameters that are
-// not finite or so large that the terms could overflow, are not regular: the patches that meet one take the per-slot path, which tests.
+// which is not positive for a positive definite conic. Where its determinant is at least 2^-16 of a c, no rounding makes it so either: the
+// terms' magnitudes are then at most 2^18 times sigma and round by 2^-21 of themselves, and the weight needs no test. Other conics (axes
+// more than about 500 to 1 among them), and parameters that are not finite or so large that the terms could overflow, are not regular: the
+// patches that meet one take the per-slot path, which tests.
 struct RowGeometry {
     float x, y, a, b, c;
     bool regular;
@@ -207,9 +222,9 @@ __device__ __forceinline__ RowGeometry row_geometry(const float *xys, const floa
     constexpr float kLog2e = 1.4426950408889634f;
     const float x = __ldg(&xys[2 * (size_t)id]), y = __ldg(&xys[2 * (size_t)id + 1]);
     const float a = __ldg(&conics[3 * (size_t)id]), b = __ldg(&conics[3 * (size_t)id + 1]), c = __ldg(&conics[3 * (size_t)id + 2]);
-    const float ac = a * c, bb = b * b;
-    const float det = (ac - bb) + (fmaf(a, c, -ac) - fmaf(b, b, -bb));  // with the products' roundings
-    const bool regular = fabsf(x) < 1e9f && fabsf(y) < 1e9f && a > 0.f && a < 1e15f && c > 0.f && c < 1e15f && det > 0.f;
+    const float ac = a * c;
+    const bool regular = fabsf(x) < 1e9f && fabsf(y) < 1e9f && a > 0.f && a < 1e15f && c > 0.f && c < 1e15f &&
+                         ac - b * b > 0x1p-16f * ac;
     return {x, y, -0.5f * kLog2e * a, -kLog2e * b, -0.5f * kLog2e * c, regular};
 }
 
@@ -296,11 +311,10 @@ struct Rows {
 
 // Few Gaussians are finished by the last CTA of the patches' kernel instead of a kernel of its own. Both passes of the balance loss in a
 // graph: 15.4 against 16.4 us at 100 Gaussians (64x64), 16.0 against 16.8 at 256, but 19.9 against 18.1 at 500 and 22.8 against 17.4 at
-// 1000 (256x256); called one by one they gain the host's time for a launch each (48 against 53 us at all these sizes).
+// 1000 (256x256); called one by one they gain the host's time for a launch each (48 against 53 us then, at all these sizes).
 constexpr int kFinishInLast = 400;
 
 // Whether this CTA is the last to come here, of all CTAs of the grid; what the others wrote before is then visible. All threads together.
-// (No shared memory: the patches' kernels fill it to where a few bytes more would cost them a resident CTA or the L1 its share.)
 __device__ __forceinline__ bool last_cta(unsigned *ticket) {
     __threadfence();
     __syncthreads();

@@ -2,15 +2,21 @@
 // of the pixel. Both losses reach the gates n_k = w_k / D, D = eps + sum_j w_j, through a score that is linear in the row's values f_c and
 // the pixel's values v_c, s_k = sum_c f_c v_c (dropout: the colour and v_out; balance: one value, alpha, and v = 1). With
 //   v'_c = v_c / D,  m' = sum_j w_j s_j / D^2,  t = dL/dsigma = w (m' - sum_c f_c v'_c)
-// a Gaussian's sums are sum t dx, t dy, t dx^2, t dx dy, t dy^2 and (dropout) w v'_c, from which finish_kernel forms
+// a Gaussian's sums are sum t dx, t dy, t dx^2, t dx dy, t dy^2 and (dropout) w v'_c, from which the end forms
 //   v_xy = (a Sx + b Sy, b Sx + c Sy),  v_conic = (Sxx / 2, Sxy, Syy / 2),  v_f = S_c.
 //
-// A warp (an 8x8 patch, topk_lists.cuh) goes over its rows twice. First a lane is two pixels: weights into shared memory (32 rows of 64), D
-// and the scores' sum in registers. Then a lane is half a row: lane l sums row l % 16 over 32 pixels (four lines of 8), reading the weights
-// four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per line, so t and
-// t dx are summed along it first. One shuffle joins the halves, and the sums go to global memory with one 16-byte vector atomic per
-// four values. A patch of more than 32 rows goes over its groups once for D and the scores and once more for the sums. Where a value is not
-// finite, the patch takes the per-slot path instead: zero times it would reach Gaussians that the pixel does not name.
+// A warp (an 8x8 patch, topk_lists.cuh) goes over its rows twice. First a lane is two pixels: weights into shared memory (a row of 64 for
+// each Gaussian), D and the scores' sum in registers. Then a lane is a row or, up to 16 rows, half of one, summing over the pixels: the
+// weights are read four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per line of
+// the patch, so t and t dx are summed along it first. The sums go to global memory with one 16-byte vector atomic per four values, in a
+// buffer of their own that the last kernel (or CTA) turns into the gradients. A patch of more rows than a group goes over its groups once
+// for D and the scores and once more for the sums. Where a value is not finite, the patch takes the per-slot path instead: zero times it
+// would reach Gaussians that the pixel does not name.
+//
+// At 1920x1080 with 20,000 Gaussians the pass takes 60 us for the balance loss and 88 us for the dropout with three channels (the lists
+// alone, read at the memory's rate, 13 us); one thread per pixel and five or eight atomics per slot took 900 and 1090 us. What bounds it
+// stands in topk_lists.cuh. The sums are float and their atomics come in any order: the last bits of the gradients differ from run to run,
+// as the render's do.
 #pragma once
 
 #include "topk_lists.cuh"
@@ -296,7 +302,7 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Patch &patch, c
     }
 }
 
-// A patch of more than 32 rows: all groups for the pixels' sums, then all again for the rows'
+// A patch of more rows than a group: all groups for the pixels' sums, then all again for the rows'
 template <int C, bool kDropout>
 __device__ __noinline__ bool sum_groups(const SumArgs &a, typename SumSmem<C, kDropout>::Warp &sm) {
     const Patch patch(a.img_h, a.img_w);

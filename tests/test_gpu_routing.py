@@ -420,3 +420,73 @@ def test_values_that_are_not_finite_stay_where_they_belong(device):
     f2 = f.clone()
     f2[7] = float("inf")
     compare(ops.topk_dropout_backward(h, w, x, k, f2, v, one, 0.0, used), ops.topk_dropout_backward(h, w, x, k, f, v, one, 0.0, used), {7})
+
+
+@pytest.mark.parametrize("h,w,n,log_scale", [(120, 168, 900, 1.1), (90, 75, 2500, 0.2)])
+def test_rasterizer_lists(h, w, n, log_scale, device):
+    """The rasterizer's own lists, with more Gaussians than the last CTA finishes, sparse and dense enough that patches overflow their rows."""
+    _, inp = make_case(h, w, n, log_scale_mean=log_scale, seed=31)
+    d = to_dev(inp, device)
+    s = ours_stages(d, h, w)
+    xys, conics, lists = np_(s["xys"]), np_(s["conics"]), np_(s["pixel_topk"])
+    x, k, t = s["xys"], s["conics"], s["pixel_topk"]
+    got = ops.topk_balance_forward(h, w, x, k, t)
+    g, counts, totals = check_balance(got, h, w, xys, conics, lists)
+    grads = ops.topk_balance_backward(h, w, x, k, t, got[1], got[3], torch.tensor(1.0, device=device))
+    check_balance_grad(grads, g, counts, totals, 1.0, None)
+    rng = np.random.default_rng(7)
+    check_dropout(h, w, xys, conics, rng.standard_normal((n, 3)), lists, 0.15, (1, 2), rng.standard_normal((3, h, w)), device)
+
+
+def test_thin_gaussians(device):
+    """Axes from 1:1 to 3000:1 at all angles, and conics that are not positive definite: where rounding decides sigma's sign, the weight is 0
+    or the bound is as wide as sigma's rounding."""
+    h, w, n = 24, 40, 80
+    rng = np.random.default_rng(61)
+    xys, _, lists = lists_case(h, w, n, 62)
+    ratio, theta = np.geomspace(1, 3000, n), rng.uniform(0, np.pi, n)
+    i0, i1 = np.full(n, 1 / 6.0**2), (ratio / 6.0) ** 2 / np.maximum(1, ratio / 300) ** 2
+    cos, sin = np.cos(theta), np.sin(theta)
+    conics = np.float32(np.stack([cos**2 * i0 + sin**2 * i1, cos * sin * (i0 - i1), sin**2 * i0 + cos**2 * i1], 1))
+    conics[5], conics[9], conics[13] = (0.1, 0.2, 0.1), (-0.1, 0.0, 0.1), (0.0, 0.0, 0.0)
+    xys = np.float32(xys)
+    x, k, t = to_gpu(device, xys, conics, lists)
+    got = ops.topk_balance_forward(h, w, x, k, t)
+    _, counts, importance, totals, g = routing.balance(h, w, xys, conics, lists)
+    assert np.array_equal(np_(got[1]), counts) and tuple(got[3].tolist()) == totals
+    # sigma may be off by 8 u of its terms' magnitude, a weight by a factor exp of that (a weight whose sigma's sign that decides: by 1 at
+    # most): per slot, with the oracle's magnitudes
+    magnitude = 0.5 * (abs(g.a) * g.dx**2 + abs(g.c) * g.dy**2) + abs(g.b * g.dx * g.dy)
+    sigma = 0.5 * (g.a * g.dx**2 + g.c * g.dy**2) + g.b * g.dx * g.dy
+    off = 11 * U * magnitude + 8 * U
+    decided = sigma > off
+    wide = np.where(decided, np.expm1(np.minimum(off, 50.0)) * g.weight, 1.0) * g.filled
+    bound = wide.sum(1, keepdims=True) / (np.maximum(g.weight.sum(1, keepdims=True) - wide.sum(1, keepdims=True), 0) + 1e-4) * g.gate + \
+        wide / (np.maximum(g.weight.sum(1, keepdims=True) - wide.sum(1, keepdims=True), 0) + 1e-4) + 64 * U * g.gate
+    lists_flat = lists.reshape(h * w, 10)
+    sums = np.zeros(n)
+    np.add.at(sums, np.where(g.filled, lists_flat, 0)[g.filled], np.minimum(bound, 1.0)[g.filled])
+    check_sums(got[2], importance, np.ones(n), 0.0, "importance", floor=sums + 1e-6)
+    assert torch.isfinite(got[2]).all()
+    grads = ops.topk_balance_backward(h, w, x, k, t, got[1], got[3], torch.tensor(1.0, device=device))
+    assert all(torch.isfinite(v).all() for v in grads)
+
+
+def test_unaligned_parameters(device):
+    """xys, conics and colours that start on any 4-byte word."""
+    h, w, n = 21, 26, 60
+    xys, conics, lists = lists_case(h, w, n, 71)
+    x, k, t = to_gpu(device, xys, conics, lists)
+    f, v, rng = torch.randn(n, 5, device=device), torch.randn(5, h, w, device=device), torch.tensor([4, 4], device=device)
+
+    def shifted(a):
+        flat = torch.empty(a.numel() + 1, device=device)
+        flat[1:] = a.reshape(-1)
+        return flat[1:].view(a.shape)
+
+    want = ops.topk_balance_forward(h, w, x, k, t) + ops.topk_dropout_forward(h, w, x, k, f, t, 0.2, rng)
+    got = ops.topk_balance_forward(h, w, shifted(x), shifted(k), t) + ops.topk_dropout_forward(h, w, shifted(x), shifted(k), shifted(f), t, 0.2, rng)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    grads = ops.topk_dropout_backward(h, w, shifted(x), shifted(k), shifted(f), shifted(v), t, 0.2, rng)
+    for a, b in zip(grads, ops.topk_dropout_backward(h, w, x, k, f, v, t, 0.2, rng)):
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5 * float(b.abs().max()))
