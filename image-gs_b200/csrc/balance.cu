@@ -24,16 +24,15 @@ using igs::kWeightPitch;
 using Rows = igs::Rows<0>;
 
 struct BalanceWorkspace {
-    unsigned long long filled;                // A
     unsigned int ticket;
-    unsigned int pad;
+    unsigned int pad[3];
     unsigned long long routed[kRoutedSlots];  // T, over this many words, so that no one word takes every patch's atomic
-    // then uint64 fixed [n], double partials [blocks of the finish kernel]
+    // then uint64 fixed [n], double2 partials [blocks of the finish kernel]
 };
 
 int finish_blocks(int n) { return n > 0 ? igs::ceil_div(n, kThreads) : 1; }
 size_t forward_bytes(int n) {
-    return sizeof(BalanceWorkspace) + sizeof(unsigned long long) * (size_t)n + sizeof(double) * (size_t)finish_blocks(n);
+    return sizeof(BalanceWorkspace) + sizeof(unsigned long long) * (size_t)(n + 1) + sizeof(double2) * (size_t)finish_blocks(n);
 }
 size_t workspace_bytes_of(int n) { return std::max(forward_bytes(n), igs::sum_bytes<1, false>(n)); }
 
@@ -55,7 +54,7 @@ struct BalanceArgs {
     BalanceWorkspace *ws;
     double inv_scale;
     float *importance;
-    double *partials;  // a sum for each block of the finish kernel
+    double2 *partials;  // A and the loss's sum, of each block of the finish kernel
     float *loss;
     long long *totals;
 };
@@ -63,7 +62,7 @@ struct BalanceArgs {
 __global__ void __launch_bounds__(kThreads) balance_zero_kernel(const __grid_constant__ BalanceArgs a) {
     igs::wait_for_predecessor();
     const int id = blockIdx.x * kThreads + threadIdx.x;
-    if (id == 0) a.ws->filled = 0, a.ws->ticket = 0;
+    if (id == 0) a.ws->ticket = 0;
     if (id < kRoutedSlots) a.ws->routed[id] = 0;
     if (id < a.n) a.counts[id] = 0, a.fixed[id] = 0;
 }
@@ -203,33 +202,38 @@ __device__ __forceinline__ void count_patch(const BalanceArgs &a, BalanceSmem &s
     if (!regular) count_slots(a);
 }
 
-// The sum over the CTA, in one order, on all threads; s_sum: a word per warp
+// The sums over the CTA, in one order, on all threads; s_sum: a double2 per warp
 template <int kCta>
-__device__ __forceinline__ double cta_sum(double x, double *s_sum) {
+__device__ __forceinline__ double2 cta_sum(double2 v, double2 *s_sum) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    for (int o = 16; o > 0; o >>= 1) v.x += __shfl_xor_sync(0xffffffffu, v.x, o), v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = x;
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = v;
     __syncthreads();
-    double total = 0.0;
+    v = make_double2(0.0, 0.0);
 #pragma unroll
-    for (int w = 0; w < kCta / 32; ++w) total += s_sum[w];
-    return total;
+    for (int w = 0; w < kCta / 32; ++w) v.x += s_sum[w].x, v.y += s_sum[w].y;
+    return v;
 }
 
-// A Gaussian's importance, from its fixed-point sum; its counts and its term of the loss are added to filled and sum
-__device__ __forceinline__ void finish_gaussian(const BalanceArgs &a, const int g, double &filled, double &sum) {
+// A Gaussian's importance, from its fixed-point sum; its counts and its term of the loss are added to v
+__device__ __forceinline__ void finish_gaussian(const BalanceArgs &a, const int g, double2 &v) {
     const double importance = (double)(long long)__ldcg(&a.fixed[g]) * a.inv_scale;
     a.importance[g] = (float)importance;
     const int count = __ldcg(&a.counts[g]);
-    filled += count, sum += importance * count;
+    v.x += count, v.y += importance * count;
 }
 
-__device__ __forceinline__ void finish_loss(const BalanceArgs &a, const double filled, const double sum) {
-    unsigned long long routed = 0;
-    for (int q = 0; q < kRoutedSlots; ++q) routed += __ldcg(&a.ws->routed[q]);
-    *a.loss = filled > 0.0 ? (float)((double)a.n / (filled * (double)routed) * sum) : 0.f;
-    a.totals[0] = (long long)filled, a.totals[1] = (long long)routed;
+// By one warp
+__device__ __forceinline__ void finish_loss(const BalanceArgs &a, const double2 v) {
+    static_assert(kRoutedSlots == 32, "a word per lane");
+    const int lane = threadIdx.x & 31;
+    unsigned long long routed = __ldcg(&a.ws->routed[lane]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) routed += __shfl_xor_sync(0xffffffffu, routed, o);
+    if (lane != 0) return;
+    *a.loss = v.x > 0.0 ? (float)((double)a.n / (v.x * (double)routed) * v.y) : 0.f;
+    a.totals[0] = (long long)v.x, a.totals[1] = (long long)routed;
 }
 
 // kFinish: the last CTA finishes
@@ -240,28 +244,30 @@ __global__ void __launch_bounds__(igs::kPatchThreads, 6) balance_kernel(const __
     count_patch(a, smem[threadIdx.x >> 5]);
     if constexpr (kFinish) {
         if (!igs::last_cta(&a.ws->ticket)) return;
-        double filled = 0.0, sum = 0.0;
-        for (int g = threadIdx.x; g < a.n; g += igs::kPatchThreads) finish_gaussian(a, g, filled, sum);
-        double *const s_sum = reinterpret_cast<double *>(smem);
-        filled = cta_sum<igs::kPatchThreads>(filled, s_sum), sum = cta_sum<igs::kPatchThreads>(sum, s_sum);
-        if (threadIdx.x == 0) finish_loss(a, filled, sum);
+        double2 v = make_double2(0.0, 0.0);
+        for (int g = threadIdx.x; g < a.n; g += igs::kPatchThreads) finish_gaussian(a, g, v);
+        v = cta_sum<igs::kPatchThreads>(v, reinterpret_cast<double2 *>(smem));
+        if (threadIdx.x < 32) finish_loss(a, v);
     }
 }
 
 // Each block's sums, added in block order by the last block to finish
 __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const __grid_constant__ BalanceArgs a) {
     igs::wait_for_predecessor();
+    __shared__ double2 s_sum[kThreads / 32];
     const int g = blockIdx.x * kThreads + threadIdx.x;
-    double filled = 0.0, sum = 0.0;
-    if (g < a.n) finish_gaussian(a, g, filled, sum);
-    __shared__ double s_sum[kThreads / 32];
-    filled = cta_sum<kThreads>(filled, s_sum), sum = cta_sum<kThreads>(sum, s_sum);
-    if (threadIdx.x == 0) a.partials[blockIdx.x] = sum, atomicAdd(&a.ws->filled, (unsigned long long)filled);
+    double2 v = make_double2(0.0, 0.0);
+    if (g < a.n) finish_gaussian(a, g, v);
+    v = cta_sum<kThreads>(v, s_sum);
+    if (threadIdx.x == 0) a.partials[blockIdx.x] = v;
     if (!igs::last_cta(&a.ws->ticket)) return;
-    sum = 0.0;
-    for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) sum += __ldcg(&a.partials[b]);
-    sum = cta_sum<kThreads>(sum, s_sum);
-    if (threadIdx.x == 0) finish_loss(a, (double)__ldcg(&a.ws->filled), sum);
+    v = make_double2(0.0, 0.0);
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) {
+        const double2 q = __ldcg(&a.partials[b]);
+        v.x += q.x, v.y += q.y;
+    }
+    v = cta_sum<kThreads>(v, s_sum);
+    if (threadIdx.x < 32) finish_loss(a, v);
 }
 
 }  // namespace
@@ -285,7 +291,7 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
     char *base = static_cast<char *>(workspace);
     BalanceWorkspace *ws = reinterpret_cast<BalanceWorkspace *>(base);
     unsigned long long *fixed = reinterpret_cast<unsigned long long *>(base + sizeof(BalanceWorkspace));
-    double *partials = reinterpret_cast<double *>(fixed + num_points);
+    double2 *partials = reinterpret_cast<double2 *>(fixed + (num_points + 1) / 2 * 2);  // 16-byte aligned
     const int bits = fraction_bits(pixels);
     const int blocks = finish_blocks(num_points);
     const bool patches = pixels > 0 && num_points > 0, in_last = patches && num_points <= igs::kFinishInLast;

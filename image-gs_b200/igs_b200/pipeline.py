@@ -118,15 +118,17 @@ class RasterStep:
             self.pixel_topk = torch.empty(self.h, self.w, TOP_K, device=dev, dtype=i32)
             self.image_ws_bytes = self.lib.igs_l1_workspace(self.image.numel())
             self.image_ws = torch.zeros(self.image_ws_bytes, device=dev, dtype=torch.uint8)
+            # without dropout the backward pass from the lists is the dropout's with p = 0 (88 us at 1080p/20k, igs_raster_bwd_topk 153 us)
+            self.drop_p = 0.0
+            self.rng_used = torch.zeros(2, device=dev, dtype=torch.int64)
+            self.drop_ws_bytes = self.lib.igs_topk_dropout_workspace(n, nc)
+            self.drop_ws = torch.empty(self.drop_ws_bytes, device=dev, dtype=torch.uint8)
         if self.gate_dropout is not None:
             self.drop_p, self.rng_state = float(self.gate_dropout["p"]), self.gate_dropout["rng_state"]
             if not 0.0 <= self.drop_p <= 1.0:
                 raise ValueError(f"p must lie in [0, 1], got {self.drop_p}")
             if self.rng_state.dtype != torch.int64 or self.rng_state.numel() != 2 or self.rng_state.device != dev:
                 raise ValueError(f"rng_state must be two int64 values on {dev}")
-            self.rng_used = torch.empty(2, device=dev, dtype=torch.int64)
-            self.drop_ws_bytes = self.lib.igs_topk_dropout_workspace(n, nc)
-            self.drop_ws = torch.empty(self.drop_ws_bytes, device=dev, dtype=torch.uint8)
         if self.balance is not None:
             self.mask = self.balance.get("mask")
             if self.mask is not None:
@@ -231,16 +233,11 @@ class RasterStep:
         self._check(self.lib.igs_l1_loss(self.image.numel(), ptr(self.image), ptr(self.target), self.l1_ratio, ptr(self.loss),
                                          ptr(self.v_image), ptr(self.image_ws), self.image_ws_bytes, self._stream()), "image loss")
 
-    def _dropout_backward(self):
+    def _lists_backward(self):
         self._check(self.lib.igs_topk_dropout_bwd(self.h, self.w, self.c, self.n, ptr(self.xys), ptr(self.conics), ptr(self.features),
                                                   ptr(self.v_image), ptr(self.pixel_topk), self.drop_p, ptr(self.rng_used), ptr(self.v_xy),
                                                   ptr(self.v_conic), ptr(self.v_colors), ptr(self.drop_ws), self.drop_ws_bytes,
-                                                  self._stream()), "dropout backward")
-
-    def _lists_backward(self):
-        self._check(self.lib.igs_raster_bwd_topk(self.h, self.w, self.c, self.n, ptr(self.xys), ptr(self.conics), ptr(self.features),
-                                                 ptr(self.v_image), ptr(self.pixel_topk), ptr(self.v_xy), ptr(self.v_conic),
-                                                 ptr(self.v_colors), self._stream()), "backward from the lists")
+                                                  self._stream()), "backward from the lists")
 
     def _balance_term(self):
         """The balance loss, and factor times its gradient added to v_xy and v_conic."""
@@ -274,14 +271,14 @@ class RasterStep:
     # kernels each stage launches (memsets excluded)
     KERNELS = {"_quantize": 1, "_project": 1, "_cumsum": 2, "_bin": 4, "_raster": 2, "_forward": 2, "_backward": 1, "_project_backward": 1,
                "_rate_term": 2, "_feature_grads": 1, "_train_step": 8, "_lists_forward": 1, "_dropout_forward": 1, "_image_loss": 1,
-               "_dropout_backward": 3, "_lists_backward": 1, "_balance_term": 6, "_next_mask": 0}
+               "_lists_backward": 3, "_balance_term": 6, "_next_mask": 0}
 
     @property
     def BREAKDOWN_STAGES(self):
         """The step's stages as separate calls (the fused step's kernels, one stage at a time, for per-stage timing)."""
         if self.lists:
-            raster = (("_lists_forward", "_dropout_forward", "_image_loss", "_dropout_backward") if self.gate_dropout is not None
-                      else ("_lists_forward", "_image_loss", "_lists_backward"))
+            raster = ("_lists_forward",) + (("_dropout_forward",) if self.gate_dropout is not None else ())
+            raster += ("_image_loss", "_lists_backward")
             raster += ("_balance_term",) if self.balance is not None else ()
         else:
             raster = ("_raster",) if self.fused else ("_forward", "_backward")
