@@ -119,11 +119,15 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def raw_stream_of(index):
+    """The current stream's handle on the device of that index, an integer. torch.cuda.current_stream() builds a Stream object to say so,
+    which takes longer (4 us) than a launch."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def stream_of(device=None):
-    """The current stream of a device (default: the current device). torch.cuda.current_stream() builds a Stream object to say so, which
-    takes longer (4 us) than a launch; this is the handle alone."""
     index = device.index if isinstance(device, torch.device) else None
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index))
+    return ctypes.c_void_p(raw_stream_of(torch.cuda.current_device() if index is None else index))
 
 
 def constants():

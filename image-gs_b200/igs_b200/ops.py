@@ -4,12 +4,13 @@ pybind functions (gsplat/gsplat/cuda/csrc/ext.cpp:4-32, bindings.h). Outputs are
 device and every launch goes to the current CUDA stream, so the operators can be captured in CUDA graphs (the *_capacity paths never read
 device memory back to the host).
 """
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_of
+from ._lib import check, ptr, raw_stream_of, stream_of
 
 TILE = 16
 TOP_K = 10
@@ -296,17 +297,25 @@ def topk_feature_weights(img_height, img_width, xys, conics, pixel_topk, eps=EPS
 # ---- routing lists: balance and gate dropout ------------------------------------------------------------------------------------------
 
 def _run(dev, name, *args):
-    """One entry point on dev's current stream, the arguments (tensors as pointers) before the stream. These operators are used on small
+    """One entry point on dev's current stream, the arguments (pointers as integers) before the stream. These operators are used on small
     images too, where the host's time is the time: the device is only changed where it is not the current one."""
-    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
     call = getattr(_lib.load(), name)
     if torch.cuda.current_device() == dev.index:
-        status = call(*args, stream_of(dev))
+        status = call(*args, raw_stream_of(dev.index))
     else:
         with torch.cuda.device(dev):
-            status = call(*args, stream_of(dev))
+            status = call(*args, raw_stream_of(dev.index))
     if status:
         check(status, name)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name, *sizes):
+    return getattr(_lib.load(), name)(*sizes)
 
 
 def _check_lists(img_height, img_width, xys, conics, pixel_topk, *others):
@@ -353,9 +362,10 @@ def topk_balance_forward(img_height, img_width, xys, conics, pixel_topk, pixel_m
     counts = torch.empty(n, device=dev, dtype=torch.int32)
     importance = torch.empty(n, device=dev, dtype=torch.float32)
     totals = torch.empty(2, device=dev, dtype=torch.int64)
-    ws_bytes = _lib.load().igs_topk_balance_workspace(n)
+    ws_bytes = _workspace_bytes("igs_topk_balance_workspace", n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_balance_fwd", h, w, n, xys, conics, pixel_topk, pixel_mask, loss, counts, importance, totals, ws, ws_bytes)
+    _run(dev, "igs_topk_balance_fwd", h, w, n, xys.data_ptr(), conics.data_ptr(), pixel_topk.data_ptr(), _address(pixel_mask),
+         loss.data_ptr(), counts.data_ptr(), importance.data_ptr(), totals.data_ptr(), ws.data_ptr(), ws_bytes)
     return loss, counts, importance, totals
 
 
@@ -378,10 +388,11 @@ def topk_balance_backward(img_height, img_width, xys, conics, pixel_topk, counts
         if grad_importance.numel() != n:
             raise RuntimeError("grad_importance must be [N]")
     v_xy, v_conic = torch.empty_like(xys), torch.empty_like(conics)
-    ws_bytes = _lib.load().igs_topk_balance_workspace(n)
+    ws_bytes = _workspace_bytes("igs_topk_balance_workspace", n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_balance_bwd", h, w, n, xys, conics, pixel_topk, pixel_mask, counts, totals, grad_loss,
-         grad_importance, 0, v_xy, v_conic, ws, ws_bytes)
+    _run(dev, "igs_topk_balance_bwd", h, w, n, xys.data_ptr(), conics.data_ptr(), pixel_topk.data_ptr(), _address(pixel_mask),
+         counts.data_ptr(), totals.data_ptr(), _address(grad_loss), _address(grad_importance), 0, v_xy.data_ptr(), v_conic.data_ptr(),
+         ws.data_ptr(), ws_bytes)
     return v_xy, v_conic
 
 
@@ -410,7 +421,8 @@ def topk_dropout_forward(img_height, img_width, xys, conics, colors, pixel_topk,
     channels, p = _check_dropout(h, w, n, colors, p, rng_state)
     out_img = torch.empty(channels, h, w, device=dev, dtype=torch.float32)
     rng_used = torch.empty(2, device=dev, dtype=torch.int64)
-    _run(dev, "igs_topk_dropout_fwd", h, w, channels, n, xys, conics, colors, pixel_topk, p, rng_state, out_img, rng_used)
+    _run(dev, "igs_topk_dropout_fwd", h, w, channels, n, xys.data_ptr(), conics.data_ptr(), colors.data_ptr(), pixel_topk.data_ptr(), p,
+         rng_state.data_ptr(), out_img.data_ptr(), rng_used.data_ptr())
     return out_img, rng_used
 
 
@@ -422,10 +434,11 @@ def topk_dropout_backward(img_height, img_width, xys, conics, colors, v_output, 
     if v_output.numel() != channels * h * w:
         raise RuntimeError("v_output must be [C, H, W]")
     v_xy, v_conic, v_colors = torch.empty_like(xys), torch.empty_like(conics), torch.empty_like(colors)
-    ws_bytes = _lib.load().igs_topk_dropout_workspace(n, channels)
+    ws_bytes = _workspace_bytes("igs_topk_dropout_workspace", n, channels)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _run(dev, "igs_topk_dropout_bwd", h, w, channels, n, xys, conics, colors, v_output, pixel_topk, p, rng_used,
-         v_xy, v_conic, v_colors, ws, ws_bytes)
+    _run(dev, "igs_topk_dropout_bwd", h, w, channels, n, xys.data_ptr(), conics.data_ptr(), colors.data_ptr(), v_output.data_ptr(),
+         pixel_topk.data_ptr(), p, rng_used.data_ptr(), v_xy.data_ptr(), v_conic.data_ptr(), v_colors.data_ptr(), ws.data_ptr(),
+         ws_bytes)
     return v_xy, v_conic, v_colors
 
 
