@@ -8,20 +8,22 @@
 //
 // The importance is summed over a patch in float, in one order, and from there as 64-bit fixed point with as many fractional bits as the
 // image leaves room for (a Gaussian's importance is at most the pixel count), so no result depends on the order of the atomics.
+//
+// At 1920x1080 with 20,000 Gaussians the counts, importance and loss take 54 us and the gradient 59 us (the lists at the memory's rate 13 us
+// each); what bounds them stands in topk_lists.cuh.
 #include <algorithm>
 
 #include "topk_sums.cuh"
 
 namespace {
 
-using igs::kTile;
-
-constexpr int kThreads = 256;
-constexpr int kRoutedSlots = 32;
 using igs::kPatchPixels;
 using igs::kPix;
 using igs::kWeightPitch;
 using Rows = igs::Rows<0>;
+
+constexpr int kThreads = 256;
+constexpr int kRoutedSlots = 32;
 
 struct BalanceWorkspace {
     unsigned int ticket;
@@ -299,7 +301,9 @@ int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const fl
                            fixed, ws, 1.0 / (double)((int64_t)1 << bits), importance, partials, loss,
                            reinterpret_cast<long long *>(totals)};
     igs::launch(balance_zero_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
-    if (patches) igs::launch(in_last ? balance_kernel<true> : balance_kernel<false>, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads), 0, s, a);
+    if (patches)
+        igs::launch(in_last ? balance_kernel<true> : balance_kernel<false>, igs::tile_grid(img_height, img_width), dim3(igs::kPatchThreads),
+                    0, s, a);
     if (!in_last) igs::launch(balance_finish_kernel, dim3(blocks), dim3(kThreads), 0, s, a);
     return igs::check_launch("igs_topk_balance_fwd");
 }

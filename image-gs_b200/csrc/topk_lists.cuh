@@ -67,11 +67,12 @@ struct KeptSlots {
 // broadcasts, two rows per packed (f32x2) instruction, with no gather per slot, and sums per Gaussian become sums along a row. Patches need
 // no other warp, so nothing waits at a barrier.
 //
-// The kernels are bound by instruction issue and the shared-memory pipe (60 to 75 % of both, DRAM 15 to 20 %): of a patch's 1150
-// instructions (counts and importance), 210 load the lists, 120 sort, 410 walk to the rows, 330 weigh, 80 sum along the rows. Measured on
-// the way, counts and importance of 1920x1080 pixels and 20,000 Gaussians: one thread per pixel and an atomic per slot 330 us; the tile's
-// IDs collected by its warps in one hash table in shared memory 88 us (twice the instructions, and time at barriers); patches of 8x4 pixels
-// 63 us; 8x8 57 us.
+// The kernels are bound by instruction issue and the shared-memory pipe together (65 and 75 % busy; DRAM 20 %): of the 1120 instructions
+// of a patch's counts and importance some 140 load the lists, 120 sort, 400 walk to the rows, 330 weigh and 100 sum along the rows.
+// Measured on the way, counts and importance of 1920x1080 pixels and 20,000 Gaussians: one thread per pixel and an atomic per slot 330 us;
+// the tile's IDs collected by its warps in one hash table in shared memory 88 us (twice the instructions, and time at barriers); patches of
+// 8x4 pixels 63 us; 8x8 54 us. Copying a patch's lists through shared memory in whole lines (58 us where direct loads took 57) and
+// prefetching those of a later patch (115.6 us for both passes, 113.4 without) gained nothing.
 //
 // kRows is the shared memory of a patch's weights against the patches that do not fit it: 32 rows leave 5 CTAs on an SM, 28 leave 6 (125
 // and 118 us for both passes of the balance loss at 100 pixels per Gaussian, 142 and 137 at 40, 153 and 171 at 25), 24 leave 7 (116, 157
@@ -138,7 +139,7 @@ __device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const Patc
     bool counts[kPix];
 #pragma unroll
     for (int b = 0; b < kPix; ++b) {
-        const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)patch.p[b] * kTopK);  // (of some pixel, if it is outside)
+        const int2 *list = reinterpret_cast<const int2 *>(pixel_topk + (size_t)patch.p[b] * kTopK);  // (some pixel's, if it is outside)
 #pragma unroll
         for (int k = 0; k < kTopK; k += 2) {
             const int2 v = __ldg(&list[k / 2]);
@@ -240,7 +241,8 @@ __device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const flo
     float2 r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
         : "=l"(reinterpret_cast<uint64_t &>(r))
-        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)), "l"(reinterpret_cast<const uint64_t &>(c)));
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)),
+          "l"(reinterpret_cast<const uint64_t &>(c)));
     return r;
 }
 __device__ __forceinline__ float2 mul2(const float2 a, const float2 b) {
@@ -259,8 +261,9 @@ __device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
 }
 
 // The rows of a group with C values f each, in shared memory in pairs: (x x y y) (a' a' b' b') (c' c' f0 f0) (f1 f1 f2 f2) ... Each row is
-// read by a lane of its own from the parameters' arrays as they are. (Laid out beforehand as one block per Gaussian, the rows take fewer and
-// wider loads; the render is 2 % faster so at 3840x2160, no faster at 1920x1080, and a small one slower by the launch: 4.7 against 3.9 us.)
+// read by a lane of its own from the parameters' arrays as they are. (Laid out beforehand as one block per Gaussian, the rows take fewer
+// and wider loads; the render is 2 % faster so at 3840x2160, no faster at 1920x1080, and a small one slower by the launch: 4.7 against
+// 3.9 us.)
 template <int C>
 struct Rows {
     static constexpr int kPairQuads = (5 + C + 1) / 2;
@@ -268,7 +271,8 @@ struct Rows {
 
     // value(id, c) gives f_c. False, on all lanes, where a row is not regular or a value is not finite.
     template <typename Value>
-    static __device__ __forceinline__ bool gather(const PatchRows &rows, const float *xys, const float *conics, Value value, float4 *pairs) {
+    static __device__ __forceinline__ bool gather(const PatchRows &rows, const float *xys, const float *conics, Value value,
+                                                  float4 *pairs) {
         const int lane = threadIdx.x & 31;
         float q[5 + C];
 #pragma unroll
@@ -290,7 +294,7 @@ struct Rows {
         return __all_sync(0xffffffffu, good);
     }
 
-    // The weights of a pair's two rows at the lane's pixels, bits 0 and 1 of held saying which of them a pixel holds; minus_x is (-px, -px)
+    // The weights of a pair's two rows at the lane's pixels, bits 0 and 1 of held saying which a pixel holds; minus_x is (-px, -px)
     static __device__ __forceinline__ void weights(const float4 *pair, const unsigned (&held)[kPix], const float2 minus_x,
                                                    const float2 (&minus_y)[kPix], float2 (&w)[kPix]) {
         const float4 xy = pair[0], ab = pair[1];

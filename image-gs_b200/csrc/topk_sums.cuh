@@ -13,8 +13,9 @@
 // for D and the scores and once more for the sums. Where a value is not finite, the patch takes the per-slot path instead: zero times it
 // would reach Gaussians that the pixel does not name.
 //
-// At 1920x1080 with 20,000 Gaussians the pass takes 60 us for the balance loss and 88 us for the dropout with three channels (the lists
-// alone, read at the memory's rate, 13 us); one thread per pixel and five or eight atomics per slot took 900 and 1090 us. What bounds it
+// At 1920x1080 with 20,000 Gaussians the pass takes 59 us for the balance loss and 87 us for the dropout with three channels (the lists
+// alone, read at the memory's rate, 13 us); one thread per pixel and five or eight atomics per slot took 900 and 1090 us. With nine
+// channels (2048x2048, 50,000 Gaussians: 275 us) the shared-memory pipe is 79 % busy with the pixels' values. What bounds it
 // stands in topk_lists.cuh. The sums are float and their atomics come in any order: the last bits of the gradients differ from run to run,
 // as the render's do.
 #pragma once
