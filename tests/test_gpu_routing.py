@@ -490,3 +490,76 @@ def test_unaligned_parameters(device):
     grads = ops.topk_dropout_backward(h, w, shifted(x), shifted(k), shifted(f), shifted(v), t, 0.2, rng)
     for a, b in zip(grads, ops.topk_dropout_backward(h, w, x, k, f, v, t, 0.2, rng)):
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("c", [3, 12])
+def test_captured_autograd_step(c, device):
+    """Both operators through autograd, forward and backward, captured in one graph (after a warm-up on the capturing stream), with eager
+    steps of the same leaves before and after: the replayed gradients equal the eager ones at the same offset."""
+    h, w, n = 48, 64, 600
+    xys, conics, lists = lists_case(h, w, n, 17)
+    x, k, t = to_gpu(device, xys, conics, lists)
+    leaves = [a.requires_grad_(True) for a in (x, k, torch.randn(n, c, device=device))]
+    target, rng = torch.rand(h, w, c, device=device), torch.tensor([8, 40], device=device)
+
+    def step():
+        image = ag.rasterize_topk_dropout(*leaves, t, h, w, 0.2, rng)
+        loss = (image - target).square().mean() + 0.1 * ag.topk_balance(leaves[0], leaves[1], t, h, w)[0]
+        return loss, torch.autograd.grad(loss, leaves)
+
+    # The eager graph is gone before the capture: a live one ties the leaves to its stream, which ends the capture, whatever the operators
+    eager = float(step()[0])
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream(device).wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        loss, grads = step()
+        rng[1:].add_(1)
+    rng.copy_(torch.tensor([8, 40]))
+    for _ in range(2):
+        offset = rng.tolist()
+        graph.replay()
+        rng_after = rng.tolist()
+        rng.copy_(torch.tensor(offset))
+        want_loss, want = step()
+        rng.copy_(torch.tensor(rng_after))
+        assert float(loss) == float(want_loss) and rng_after[1] == offset[1] + 1
+        for a, b in zip(grads, want):
+            torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-5 * float(b.abs().max()))  # the order of the atomics alone
+    assert eager != float(loss)
+
+
+def test_two_streams_at_once(device):
+    """Calls of different sizes running at once on two streams share nothing."""
+    cases = []
+    for h, w, n, seed in ((300, 260, 350, 81), (200, 333, 1500, 82)):
+        rng = np.random.default_rng(seed)
+        xys = np.float32(rng.uniform(0, [w, h], (n, 2)))
+        conics = np.tile(np.float32([0.05, 0.01, 0.04]), (n, 1))
+        near = ((np.arange(h)[:, None] // 8) * (w // 8 + 1) + np.arange(w)[None] // 8) % n
+        lists = (near[..., None] + np.arange(10)) % n
+        cases.append((h, w) + to_gpu(device, xys, conics, lists) + (torch.randn(n, 3, device=device), torch.randn(3, h, w, device=device)))
+    state = torch.tensor([3, 3], device=device)
+
+    def run(h, w, x, k, t, f, v):
+        got = ops.topk_balance_forward(h, w, x, k, t)
+        image, used = ops.topk_dropout_forward(h, w, x, k, f, t, 0.3, state)
+        return got + (image,), ops.topk_dropout_backward(h, w, x, k, f, v, t, 0.3, used)
+
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device) for _ in cases]
+    results = [[], []]
+    for _ in range(20):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                results[i].append(run(*c))
+    torch.cuda.synchronize()
+    for (exact, sums), got in zip(want, results):
+        for e, g in got:
+            assert all(torch.equal(a, b) for a, b in zip(exact, e))
+            for a, b in zip(sums, g):
+                torch.testing.assert_close(b, a, rtol=1e-3, atol=1e-5 * float(a.abs().max()))
