@@ -279,7 +279,7 @@ int igs_feature_weights(int img_height, int img_width, int num_points, const flo
  * igs_topk_balance_bwd: the gradient of v_loss * loss + sum_g v_importance_g importance_g with the counts held constant (v_loss a device
  * scalar, v_importance [N]; either may be NULL, for 0), from the forward's counts and totals: v_xy [N,2], v_conic [N,3], written whole, or
  * added to when accumulate is not zero. workspace: igs_topk_balance_workspace(N) bytes, 16-byte aligned, whose content need not survive
- * between the two calls. At most 2^31 / 10 pixels, 2^24 a side, and 2^26 Gaussians. */
+ * between the two calls. At most 2^31 / 10 pixels, 65535 tiles a side and 2^26 Gaussians. */
 size_t igs_topk_balance_workspace(int num_points);
 int igs_topk_balance_fwd(int img_height, int img_width, int num_points, const float *xys, const float *conics, const int32_t *pixel_topk,
                          const uint8_t *pixel_mask, float *loss, int32_t *counts, float *importance, int64_t *totals, void *workspace,
