@@ -37,7 +37,7 @@ class RasterStep:
         separate forward and backward kernels, with the top-K lists and the image gradient (v_image) kept in HBM.
         balance: dict(factor, mask (optional, [H,W] bool or uint8)) adds the gradient of factor * the balance loss of the pixels over the
         Gaussians to the geometry's; the loss itself, the counts and the importance are in balance_loss, counts and importance.
-        gate_dropout: dict(p, rng_state (int64 [2] on the device: seed and offset)) renders with gates dropped; the step ends by moving the
+        gate_dropout: dict(p, rng_state (two int64 on the device side by side: seed and offset)) renders with gates dropped; the step ends by moving the
         offset on by one, so that every launch and every replay draws another mask. Both run from the [H, W, 10] lists, not fused."""
         self.balance, self.gate_dropout = balance, gate_dropout
         self.lists = balance is not None or gate_dropout is not None
@@ -129,6 +129,8 @@ class RasterStep:
                 raise ValueError(f"p must lie in [0, 1], got {self.drop_p}")
             if self.rng_state.dtype != torch.int64 or self.rng_state.numel() != 2 or self.rng_state.device != dev:
                 raise ValueError(f"rng_state must be two int64 values on {dev}")
+            if not self.rng_state.is_contiguous():  # a copy would not do: the step moves the caller's offset, and the caller may too
+                raise ValueError("rng_state must be contiguous: the kernels read seed and offset side by side")
         if self.balance is not None:
             self.mask = self.balance.get("mask")
             if self.mask is not None:
@@ -251,7 +253,7 @@ class RasterStep:
                                                   self._stream()), "balance backward")
 
     def _next_mask(self):
-        self.rng_state[1:].add_(1)
+        self.rng_state.view(2)[1:].add_(1)
 
     def _project_backward(self):
         self._check(self.lib.igs_project_bwd(self.n, ptr(self.scales), ptr(self.rotations), self.h, self.w, ptr(self.radii), ptr(self.conics),
