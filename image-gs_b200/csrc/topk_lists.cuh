@@ -260,6 +260,10 @@ __device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
     return r;
 }
 
+// Sums of magnitudes of a row's values, and of a pixel's, that the row path takes. It multiplies every row of a patch with every pixel and
+// leaves out by a weight of zero, so the products have to be finite where they do not count too: at most 2^120 in all.
+constexpr float kValueLimit = 0x1p60f;
+
 // The rows of a group with C values f each, in shared memory in pairs: (x x y y) (a' a' b' b') (c' c' f0 f0) (f1 f1 f2 f2) ... Each row is
 // read by a lane of its own from the parameters' arrays as they are. (Laid out beforehand as one block per Gaussian, the rows take fewer
 // and wider loads; the render is 2 % faster so at 3840x2160, no faster at 1920x1080, and a small one slower by the launch: 4.7 against
@@ -269,7 +273,7 @@ struct Rows {
     static constexpr int kPairQuads = (5 + C + 1) / 2;
     static constexpr int kGroupQuads = kRows / 2 * kPairQuads;
 
-    // value(id, c) gives f_c. False, on all lanes, where a row is not regular or a value is not finite.
+    // value(id, c) gives f_c. False, on all lanes, where a row is not regular or its values are not below kValueLimit.
     template <typename Value>
     static __device__ __forceinline__ bool gather(const PatchRows &rows, const float *xys, const float *conics, Value value,
                                                   float4 *pairs) {
@@ -284,7 +288,7 @@ struct Rows {
             float size = 0.f;
 #pragma unroll
             for (int c = 0; c < C; ++c) q[5 + c] = value(rows.id, c), size += fabsf(q[5 + c]);
-            good = g.regular && isfinite(size);
+            good = g.regular && size < kValueLimit;  // (not where it is NaN)
         }
         if (lane <= rows.n && lane < kRows) {  // one more, of zeros, to pad the last pair
             float *pair = reinterpret_cast<float *>(pairs + (lane >> 1) * kPairQuads) + (lane & 1);

@@ -10,8 +10,8 @@
 // weights are read four at a time and the pixels' v' and m' as broadcasts, two pixels per packed instruction; dy is one value per line of
 // the patch, so t and t dx are summed along it first. The sums go to global memory with one 16-byte vector atomic per four values, in a
 // buffer of their own that the last kernel (or CTA) turns into the gradients. A patch of more rows than a group goes over its groups once
-// for D and the scores and once more for the sums. Where a value is not finite, the patch takes the per-slot path instead: zero times it
-// would reach Gaussians that the pixel does not name.
+// for D and the scores and once more for the sums. Where a value is not finite, or so large that a product could overflow (kValueLimit), the
+// patch takes the per-slot path instead: zero times it would reach Gaussians that the pixel does not name.
 //
 // At 1920x1080 with 20,000 Gaussians the pass takes 59 us for the balance loss and 87 us for the dropout with three channels (the lists
 // alone, read at the memory's rate, 13 us); one thread per pixel and five or eight atomics per slot took 900 and 1090 us. With nine
@@ -214,9 +214,9 @@ struct PixelSums {
         }
     }
 
-    // v' and m' into shared memory; false, on all lanes, where one is not finite
+    // v' and m' into shared memory; false, on all lanes, where they are not below kValueLimit
     __device__ __forceinline__ bool finish(float (&pixel)[C + 1][kPatchPixels]) {
-        bool finite = true;
+        bool good = true;
 #pragma unroll
         for (int b = 0; b < kPix; ++b) {
             const float t = total[b].x + total[b].y;
@@ -230,9 +230,9 @@ struct PixelSums {
                 pixel[c][32 * b + (threadIdx.x & 31)] = vc;
             }
             pixel[C][32 * b + (threadIdx.x & 31)] = m;
-            finite = finite && isfinite(size);
+            good = good && size < kValueLimit;  // (not where it is NaN)
         }
-        return __all_sync(0xffffffffu, finite);
+        return __all_sync(0xffffffffu, good);
     }
 };
 
