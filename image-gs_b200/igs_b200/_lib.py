@@ -121,12 +121,19 @@ def ptr(t):
 
 def raw_stream_of(index):
     """The current stream's handle on the device of that index, an integer. torch.cuda.current_stream() builds a Stream object to say so,
-    which takes longer (4 us) than a launch."""
+    which takes longer (4 us) than a launch. (Not a public name of torch's; this is its only use, and the tests hold it to the public call.)"""
     return torch._C._cuda_getCurrentRawStream(index)
 
 
 def stream_of(device=None):
-    index = device.index if isinstance(device, torch.device) else None
+    """The current stream of a CUDA device: a torch.device, its name or its index; the current device's where no index is given."""
+    index = None
+    if device is not None:
+        if not isinstance(device, torch.device):
+            device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"stream_of takes a CUDA device, got {device}")
+        index = device.index
     return ctypes.c_void_p(raw_stream_of(torch.cuda.current_device() if index is None else index))
 
 

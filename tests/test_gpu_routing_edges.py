@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from igs_b200 import ops
+from igs_b200 import _lib, ops
 from oracle import routing
 from test_gpu_routing import check_balance_grad, check_dropout, to_gpu
 
@@ -39,3 +39,11 @@ def test_large_values_stay_where_they_belong(others, device):
     colors, v = rng.standard_normal((n, 3)), rng.standard_normal((3, h, w))
     colors[1], v[:, 0, 0], v[:, 7, 7] = 1e32, 1e4, 1e-20
     check_dropout(h, w, xys, conics, colors, lists, 0.0, (1, 1), v, device)
+
+
+def test_stream_handles_are_the_public_ones(device):
+    side = torch.cuda.Stream(device)
+    for stream in (torch.cuda.current_stream(device), side):
+        with torch.cuda.stream(stream):
+            for d in (device, device.index, "cuda:0", None):
+                assert (_lib.stream_of(d).value or 0) == torch.cuda.current_stream(d).cuda_stream == stream.cuda_stream
