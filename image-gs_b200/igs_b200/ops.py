@@ -334,6 +334,8 @@ def _check_lists(img_height, img_width, xys, conics, pixel_topk, *others):
         raise RuntimeError("conics must have dimensions (num_points, 3)")
     if pixel_topk.numel() != h * w * TOP_K:
         raise RuntimeError("pixel_topk must be [H, W, TOP_K]")
+    if max(h, w, n) > 2**31 - 1:  # the entry points refuse what is past their limits, but would see the low 32 bits of these
+        raise RuntimeError("at most 2^31 / 10 pixels, 65535 tiles a side and 2^26 Gaussians")
     dev = xys.device
     for t in (conics, pixel_topk) + others:
         if t is not None and t.device != dev:

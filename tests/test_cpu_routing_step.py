@@ -1,12 +1,12 @@
 """
-The training step's routing options without a GPU: what RasterStep refuses when it is built (with a capacity given, building launches
-nothing).
+The routing options of the training step without a GPU: what RasterStep refuses when it is built (with a capacity given, building launches
+nothing), and sizes that the operators refuse.
 """
 import pytest
 import torch
 
 from common import make_case
-from igs_b200 import pipeline
+from igs_b200 import ops, pipeline
 
 
 def build(**options):
@@ -32,3 +32,14 @@ def test_step_moves_the_offset_whatever_the_shape(shape):
     for _ in range(2):
         step._next_mask()
     assert states.tolist() == [[0, 1], [2, 5], [4, 5]]
+
+
+@pytest.mark.parametrize("h,w,n", [(4, 6, (1 << 32) + 3), (0, (1 << 32) + 5, 7), ((1 << 32) + 4, 0, 7), (4, 6, 1 << 31)])
+def test_sizes_past_the_entry_points_integers_are_refused(h, w, n, monkeypatch):
+    """An entry point takes 32-bit sizes and would see the low 32 bits of these: 3 Gaussians, 5 columns. (Tensors without storage.)"""
+    monkeypatch.setattr(ops, "_check_input", lambda t, name, dtype=None: None)  # which wants CUDA tensors
+    xys, conics = torch.empty(n, 2, device="meta"), torch.empty(n, 3, device="meta")
+    topk = torch.empty(h, w, 10, dtype=torch.int32, device="meta")
+    with pytest.raises(RuntimeError, match="2\\^26 Gaussians"):
+        ops._check_lists(h, w, xys, conics, topk)
+    assert ops._check_lists(4, 6, xys[:7], conics[:7], torch.empty(4, 6, 10, device="meta"))[:3] == (4, 6, 7)
