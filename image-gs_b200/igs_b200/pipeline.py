@@ -35,8 +35,9 @@ class RasterStep:
         the canonical, non-negative ones); loss_transform [C,C]: render feat T^T (YUV loss space, needs quant); rate: dict(model (the
         fields of compress.rate.RateModel), inv_rot_step, factor) adds the rate term on the raw features and rotations. fused=False:
         separate forward and backward kernels, with the top-K lists and the image gradient (v_image) kept in HBM.
-        balance: dict(factor, mask (optional, [H,W] bool or uint8)) adds the gradient of factor * the balance loss of the pixels over the
-        Gaussians to the geometry's; the loss itself, the counts and the importance are in balance_loss, counts and importance.
+        balance: dict(factor, mask (optional, [H,W] bool or uint8 of any strides, read anew by every step)) adds the gradient of factor *
+        the balance loss of the pixels over the Gaussians to the geometry's; the loss itself, the counts and the importance are in
+        balance_loss, counts and importance.
         gate_dropout: dict(p, rng_state (two int64 on the device side by side: seed and offset)) renders with gates dropped; the step ends by moving the
         offset on by one, so that every launch and every replay draws another mask. Both run from the [H, W, 10] lists, not fused."""
         self.balance, self.gate_dropout = balance, gate_dropout
@@ -136,7 +137,10 @@ class RasterStep:
             if self.mask is not None:
                 if self.mask.dtype not in (torch.bool, torch.uint8) or tuple(self.mask.shape) != (self.h, self.w) or self.mask.device != dev:
                     raise ValueError(f"the balance mask must be [{self.h}, {self.w}] bool or uint8 on {dev}")
-                self.mask = self.mask.contiguous()
+            # the caller may change the mask between steps: one that is not contiguous is copied by every step
+            self.mask_source = self.mask
+            if self.mask is not None and not self.mask.is_contiguous():
+                self.mask = torch.empty(self.h, self.w, device=dev, dtype=self.mask.dtype)
             self.balance_factor = torch.full((), float(self.balance["factor"]), device=dev, dtype=f32)
             self.balance_loss = torch.empty((), device=dev, dtype=f32)
             self.counts = torch.empty(n, device=dev, dtype=i32)
@@ -243,6 +247,8 @@ class RasterStep:
 
     def _balance_term(self):
         """The balance loss, and factor times its gradient added to v_xy and v_conic."""
+        if self.mask is not self.mask_source:
+            self.mask.copy_(self.mask_source)
         self._check(self.lib.igs_topk_balance_fwd(self.h, self.w, self.n, ptr(self.xys), ptr(self.conics), ptr(self.pixel_topk),
                                                   ptr(self.mask), ptr(self.balance_loss), ptr(self.counts), ptr(self.importance),
                                                   ptr(self.totals), ptr(self.balance_ws), self.balance_ws_bytes, self._stream()),
