@@ -320,7 +320,7 @@ struct Rows {
 // Few Gaussians are finished by the last CTA of the patches' kernel instead of a kernel of its own. Both passes of the balance loss in a
 // graph: 15.4 against 16.4 us at 100 Gaussians (64x64), 16.0 against 16.8 at 256, but 19.9 against 18.1 at 500 and 22.8 against 17.4 at
 // 1000 (256x256); called one by one they gain the host's time for a launch each (48 against 53 us then, at all these sizes).
-constexpr int kFinishInLast = 400;
+constexpr int kFinishInLast = 400;  // (igs_b200/pipeline.py counts its kernels by it)
 
 // Whether this CTA is the last to come here, of all CTAs of the grid; what the others wrote before is then visible. All threads together.
 __device__ __forceinline__ bool last_cta(unsigned *ticket) {

@@ -276,10 +276,12 @@ class RasterStep:
                                                ptr(self.v_scale), ptr(self.v_rot), ptr(self.step_ws), self.step_ws_bytes, self._stream()),
                     "train step")
 
-    # kernels each stage launches (memsets excluded)
+    # kernels each stage launches (memsets excluded; kernels_of() has the exceptions)
     KERNELS = {"_quantize": 1, "_project": 1, "_cumsum": 2, "_bin": 4, "_raster": 2, "_forward": 2, "_backward": 1, "_project_backward": 1,
                "_rate_term": 2, "_feature_grads": 1, "_train_step": 8, "_lists_forward": 1, "_dropout_forward": 1, "_image_loss": 1,
-               "_lists_backward": 3, "_balance_term": 6, "_next_mask": 0}
+               "_lists_backward": 3, "_balance_term": 6, "_next_mask": 1}
+    # up to this many Gaussians the last CTA of a pass from the lists finishes it, without a kernel for that (kFinishInLast in topk_lists.cuh)
+    FINISH_IN_LAST = 400
 
     @property
     def BREAKDOWN_STAGES(self):
@@ -311,9 +313,18 @@ class RasterStep:
         for s in self.STAGES:
             getattr(self, s)()
 
+    def kernels_of(self, stage):
+        """Kernels that a stage of this step launches."""
+        count = self.KERNELS[stage]
+        if stage in ("_lists_backward", "_balance_term") and self.n <= self.FINISH_IN_LAST:
+            count -= 1 if stage == "_lists_backward" else 2
+        if stage == "_balance_term" and self.mask is not self.mask_source:
+            count += 1
+        return count
+
     @property
     def kernels_per_step(self):
-        return sum(self.KERNELS[s] for s in self.STAGES)
+        return sum(self.kernels_of(s) for s in self.STAGES)
 
     PACK_ALIGN = 64  # floats: each parameter array of the packed buffer starts on a 256-byte boundary
 

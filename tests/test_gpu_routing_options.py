@@ -37,3 +37,48 @@ def test_mask_is_read_anew_by_every_step(layout, dtype, replayed, device):
             assert torch.equal(a, b)
         seen.append(int(step.totals[0]))
     assert seen[0] > seen[1] > seen[2]
+
+
+def kernel_nodes(issue):
+    """How many kernels issue() launches: the kernel nodes of a graph captured from it."""
+    from cuda.bindings import driver
+
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        issue()
+    raw = driver.CUgraph(graph.raw_cuda_graph())
+    error, _, count = driver.cuGraphGetNodes(raw)
+    assert error == driver.CUresult.CUDA_SUCCESS
+    error, nodes, count = driver.cuGraphGetNodes(raw, count)
+    assert error == driver.CUresult.CUDA_SUCCESS and len(nodes) == count
+    kinds = [driver.cuGraphNodeGetType(node) for node in nodes]
+    assert all(error == driver.CUresult.CUDA_SUCCESS for error, _ in kinds)
+    return sum(kind == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL for _, kind in kinds)
+
+
+@pytest.mark.parametrize("n", [1, 400, 401, 900])
+@pytest.mark.parametrize("options", ["balance", "balance, strided mask", "dropout", "both"])
+def test_kernels_per_step_are_those_that_a_step_launches(options, n, device):
+    """On both sides of the Gaussians that the last CTA finishes."""
+    h, w = 48, 64
+    kw = {}
+    if options != "dropout":
+        mask = torch.ones(w, h, dtype=torch.bool, device=device).t() if "strided" in options else None
+        kw["balance"] = dict(factor=0.05, mask=mask)
+    if options in ("dropout", "both"):
+        kw["gate_dropout"] = dict(p=0.1, rng_state=torch.zeros(2, dtype=torch.int64, device=device))
+    step = build(device, h, w, n, **kw)
+    step.launch()  # outside a capture first
+    torch.cuda.synchronize()
+    routing = [s for s in step.STAGES if s in ("_lists_forward", "_dropout_forward", "_image_loss", "_lists_backward", "_balance_term",
+                                               "_next_mask")]
+    assert {s: step.kernels_of(s) for s in routing} == {s: kernel_nodes(getattr(step, s)) for s in routing}
+    assert step.kernels_per_step == sum(step.kernels_of(s) for s in step.STAGES) == kernel_nodes(step.launch)
+
+
+def test_kernels_per_step_without_the_options(device):
+    for fused in (True, False):
+        step = build(device, 48, 64, 200, fused=fused)
+        step.launch()
+        torch.cuda.synchronize()
+        assert step.kernels_per_step == kernel_nodes(step.launch)
