@@ -8,7 +8,7 @@ import torch
 
 from igs_b200 import _lib, ops
 from oracle import routing
-from test_gpu_routing import check_balance_grad, check_dropout, to_gpu
+from test_gpu_routing import U, check_balance, check_balance_grad, check_dropout, gate_tolerance, to_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,89 @@ def test_stream_handles_are_the_public_ones(device):
         with torch.cuda.stream(stream):
             for d in (device, device.index, "cuda:0", None):
                 assert (_lib.stream_of(d).value or 0) == torch.cuda.current_stream(d).cuda_stream == stream.cuda_stream
+
+
+def neighbour_lists(cells_y, cells_x, cell):
+    """Gaussians one per cell of `cell` pixels a side; every pixel names its own cell's and the eight around it."""
+    y, x = np.mgrid[:cells_y * cell, :cells_x * cell] // cell
+    lists = np.full((cells_y * cell, cells_x * cell, 10), -1, np.int32)
+    for k, (dy, dx) in enumerate((a, b) for a in (-1, 0, 1) for b in (-1, 0, 1)):
+        inside = (0 <= y + dy) & (y + dy < cells_y) & (0 <= x + dx) & (x + dx < cells_x)
+        lists[..., k] = np.where(inside, (y + dy) * cells_x + x + dx, -1)
+    return lists
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_a_value_that_is_not_finite_reaches_those_that_share_a_pixel_alone(value, device):
+    """Lists of nine Gaussians: one that is not finite leaves the gradients of all that share no pixel with it, of its own patches too."""
+    cell, cells_y, cells_x, bad = 4, 4, 12, 13  # cell (1, 1): named by rows and columns 0 to 11, half of the patches beside the first
+    lists = neighbour_lists(cells_y, cells_x, cell)
+    h, w, n = lists.shape[0], lists.shape[1], cells_y * cells_x
+    rng = np.random.default_rng(17)
+    at = np.arange(n)
+    xys = np.float32(np.stack([at % cells_x, at // cells_x], 1) * cell + rng.uniform(0, cell, (n, 2)))
+    conics = np.tile(np.float32([0.11, 0.02, 0.09]), (n, 1))
+    holds = (lists == bad).any(-1)
+    together = set(lists[holds].ravel()) - {-1}
+    apart = np.setdiff1d(at, list(together))
+    patch = lambda m: m.reshape(h // 8, 8, w // 8, 8).any((1, 3))  # noqa: E731
+    same_patch = [i for i in apart if (patch((lists == i).any(-1)) & patch(holds)).any()]
+    assert len(apart) > 20 and len(same_patch) > 3
+
+    def compare(got, want, sizes, rel):
+        for a, b, size in zip(got, want, sizes):
+            a = a.cpu().numpy().astype(np.float64)
+            assert not np.isfinite(a[bad]).all()
+            assert np.all(abs(a[apart] - b[apart]) <= rel * size[apart] + 1e-30)
+
+    x, k, t = to_gpu(device, xys, conics, lists)
+    _, counts, _, totals = ops.topk_balance_forward(h, w, x, k, t)
+    alpha = np.float32(rng.standard_normal(n))
+    _, o_counts, _, o_totals, g = routing.balance(h, w, xys, conics, lists)
+    v_xy, v_conic, *sizes = routing.balance_grad(g, o_counts, o_totals, 0.0, alpha)
+    alpha[bad] = value
+    got = ops.topk_balance_backward(h, w, x, k, t, counts, totals, None, torch.from_numpy(alpha).to(device))
+    rel = 2 * gate_tolerance(g) + (64 + o_counts.max()) * U
+    compare(got, (v_xy, v_conic), sizes, rel)
+
+    colors, v = np.float32(rng.standard_normal((n, 3))), np.float32(rng.standard_normal((3, h, w)))
+    v_xy, v_conic, v_colors, *sizes = routing.dropout_grad(g, colors, v)
+    colors[bad, 1] = value
+    state = torch.tensor([2, 2], device=device)
+    f, v_out = torch.from_numpy(colors).to(device), torch.from_numpy(v).to(device)
+    image = ops.topk_dropout_forward(h, w, x, k, f, t, 0.0, state)[0]
+    assert torch.isfinite(image[0]).all() and torch.equal(~torch.isfinite(image[1]).cpu(), torch.from_numpy(holds))
+    got = ops.topk_dropout_backward(h, w, x, k, f, v_out, t, 0.0, state)
+    compare(got[:2], (v_xy, v_conic), sizes[:2], rel)
+    a = got[2].cpu().numpy().astype(np.float64)  # the colours' gradients hold no colour
+    assert np.all(abs(a - v_colors) <= rel * sizes[2] + 1e-30)
+
+
+ROWS = 28  # of a group
+
+
+@pytest.mark.parametrize("ids,repeats", [(15, 0), (16, 0), (17, 0), (ROWS - 1, 0), (ROWS, 0), (ROWS + 1, 0), (2 * ROWS, 0), (2 * ROWS + 1, 0),
+                                         (ROWS - 1, 1), (ROWS, 1), (ROWS + 1, 1), (ROWS, 9), (2 * ROWS, 1)])
+def test_rows_at_the_border_of_a_group(ids, repeats, device):
+    """One patch whose lists name just as many Gaussians as half a warp or a group of rows takes, one fewer and one more; and with the last of
+    a group's IDs in 1 + repeats slots of one pixel, each a row of its own, so that the same ID lies on both sides of the border."""
+    h = w = 8
+    rng = np.random.default_rng(1000 * ids + repeats)
+    lists = np.full((h * w, 10), -1, np.int32)
+    for p in range(h * w):
+        lists[p, :7] = (p * 5 + np.arange(7)) % ids  # every ID in some pixels
+    if repeats:
+        lists[11] = -1
+        lists[11, rng.permutation(10)[:1 + repeats]] = min(ROWS, ids) - 1
+    lists = rng.permuted(lists, axis=1).reshape(h, w, 10)
+    assert len(np.unique(lists[lists >= 0])) == ids
+    n = ids + 3  # some that nothing names
+    xys, conics = np.float32(rng.uniform(0, 8, (n, 2))), np.tile(np.float32([0.2, 0.05, 0.3]), (n, 1))
+    x, k, t = to_gpu(device, xys, conics, lists)
+    got = ops.topk_balance_forward(h, w, x, k, t)
+    g, counts, totals = check_balance(got, h, w, xys, conics, lists)
+    v_imp = np.float32(rng.standard_normal(n))
+    grads = ops.topk_balance_backward(h, w, x, k, t, got[1], got[3], torch.tensor(1.0, device=device), torch.from_numpy(v_imp).to(device))
+    check_balance_grad(grads, g, counts, totals, 1.0, v_imp)
+    for p, c in ((0.0, 3), (0.2, 1), (0.2, 9)):
+        check_dropout(h, w, xys, conics, rng.standard_normal((n, c)), lists, p, (ids, repeats), rng.standard_normal((c, h, w)), device)
