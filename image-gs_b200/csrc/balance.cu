@@ -7,7 +7,10 @@
 //   v_xy += dL/dsigma (a dx + b dy, b dx + c dy),  v_conic += dL/dsigma (dx^2 / 2, dx dy, dy^2 / 2)      (topk_sums.cuh).
 //
 // The importance is summed over a patch in float, in one order, and from there as 64-bit fixed point with as many fractional bits as the
-// image leaves room for (a Gaussian's importance is at most the pixel count), so no result depends on the order of the atomics.
+// image leaves room for (a Gaussian's importance is at most the pixel count), so no result depends on the order of the atomics. The float sums
+// of at most 64 gates round by 2^-24 of themselves (the results are within 1e-7 of the definition's in 64 bits, where sums in 64 bits
+// throughout are within 0.5e-7); the fixed point rounds a patch's share to 2^-(62 - ceil(log2 pixels)), 2^-39 at 3840x2160, and half of that
+// to 0.
 //
 // At 1920x1080 with 20,000 Gaussians the counts, importance and loss take 54 us and the gradient 59 us (the lists at the memory's rate 13 us
 // each); what bounds them stands in topk_lists.cuh.

@@ -106,7 +106,8 @@ struct Patch {
     }
 };
 
-// A sorting network for ten keys (29 comparators, depth 8)
+// A sorting network for ten keys: A. Waksman's of 29 comparators (1969; D. Knuth, The Art of Computer Programming, volume 3, section 5.3.4),
+// nine steps deep
 __device__ __forceinline__ void sort_slots(int (&key)[kTopK]) {
     constexpr int kPairs[29][2] = {{4, 9}, {3, 8}, {2, 7}, {1, 6}, {0, 5}, {1, 4}, {6, 9}, {0, 3}, {5, 8}, {0, 2}, {3, 6}, {7, 9},
                                    {0, 1}, {2, 4}, {5, 7}, {8, 9}, {1, 2}, {4, 6}, {7, 8}, {3, 5}, {2, 5}, {6, 8}, {1, 3}, {4, 7},
@@ -200,7 +201,7 @@ __device__ __forceinline__ PatchRows find_rows(const int *pixel_topk, const Patc
     return rows;
 }
 
-// exp2(x) (ex2.approx: 2 ulp; results below 2^-126 are 0, far below what eps leaves of a gate)
+// exp2(x) (ex2.approx: 2 ulp, 2^-22 of the weight; results below 2^-126 are 0, far below what eps leaves of a gate)
 __device__ __forceinline__ float exp2_approx(const float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -210,10 +211,11 @@ __device__ __forceinline__ float exp2_approx(const float x) {
 // A Gaussian's geometry as the kernels use it: centre, and the conic times -log2(e) (its outer terms halved too), so that the weight is
 // exp2 of
 //   (a' dx) dx + (c' dy + b' dx) dy
-// which is not positive for a positive definite conic. Where its determinant is at least 2^-16 of a c, no rounding makes it so either: the
-// terms' magnitudes are then at most 2^18 times sigma and round by 2^-21 of themselves, and the weight needs no test. Other conics (axes
-// more than about 500 to 1 among them), and parameters that are not finite or so large that the terms could overflow, are not regular: the
-// patches that meet one take the per-slot path, which tests.
+// which is not positive for a positive definite conic. Folding the factor in costs two of the at most 8 roundings of 2^-24 of the terms'
+// magnitudes that the exponent has. Where the conic's determinant is at least 2^-16 of a c, none of them makes it positive either: the terms'
+// magnitudes are then at most 2^18 times sigma and round by 2^-21 of themselves, and the weight needs no test. Other conics (axes more than
+// about 500 to 1 among them), and parameters that are not finite or so large that the terms could overflow, are not regular: the patches that
+// meet one take the per-slot path, which tests.
 struct RowGeometry {
     float x, y, a, b, c;
     bool regular;

@@ -275,7 +275,8 @@ int igs_feature_weights(int img_height, int img_width, int num_points, const flo
  * the filled slots of pixel_topk [H,W,10] (IDs in [0, N), of pixels whose pixel_mask [H,W] byte is not zero; pixel_mask may be NULL):
  * counts [N] = slots that hold the Gaussian, importance [N] = sum of their gates w_k / (sum_j w_j + 1e-4), w = exp(-sigma) (0 where sigma
  * is negative, NaN or infinite), totals [2] (int64) = A, the filled slots, and T, the pixels with one, and
- * loss = N / (A T) sum_g counts_g importance_g (0 when A is 0). All are written whole; none depends on the order of the atomics.
+ * loss = N / (A T) sum_g counts_g importance_g (0 when A is 0). All are written whole; none depends on the order of the atomics. importance is
+ * summed in multiples of 2^-(62 - ceil(log2(H W))), 2^-39 at 3840x2160, to which a Gaussian's share of an 8x8 patch is rounded.
  * igs_topk_balance_bwd: the gradient of v_loss * loss + sum_g v_importance_g importance_g with the counts held constant (v_loss a device
  * scalar, v_importance [N]; either may be NULL, for 0), from the forward's counts and totals: v_xy [N,2], v_conic [N,3], written whole, or
  * added to when accumulate is not zero. workspace: igs_topk_balance_workspace(N) bytes, 16-byte aligned, whose content need not survive
@@ -297,7 +298,8 @@ int igs_topk_balance_bwd(int img_height, int img_width, int num_points, const fl
  * 0, 1, 2 and 3, 4, 5 (the first most significant). rng_used [2] gets the values that the pass saw; the backward pass takes them, so the
  * caller may move rng_state on in between, in a captured graph too. igs_topk_dropout_bwd writes v_xy [N,2], v_conic [N,3] and v_colors
  * [N,C] whole, from v_output [C,H,W]; its workspace: igs_topk_dropout_workspace(N, C) bytes, 16-byte aligned. 1 to 12 channels, sizes as
- * above. */
+ * above. A colour or a value of v_output that is not finite reaches the outputs of the pixels and Gaussians that share a pixel's kept
+ * slots with it. */
 size_t igs_topk_dropout_workspace(int num_points, int channels);
 int igs_topk_dropout_fwd(int img_height, int img_width, int channels, int num_points, const float *xys, const float *conics,
                          const float *colors, const int32_t *pixel_topk, double p, const int64_t *rng_state, float *out_img,
