@@ -8,7 +8,7 @@ import torch
 
 from igs_b200 import _lib, ops
 from oracle import routing
-from test_gpu_routing import U, check_balance, check_balance_grad, check_dropout, gate_tolerance, to_gpu
+from test_gpu_routing import U, check_balance, check_balance_grad, check_dropout, check_sums, gate_tolerance, to_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,72 @@ def test_rows_at_the_border_of_a_group(ids, repeats, device):
     check_balance_grad(grads, g, counts, totals, 1.0, v_imp)
     for p, c in ((0.0, 3), (0.2, 1), (0.2, 9)):
         check_dropout(h, w, xys, conics, rng.standard_normal((n, c)), lists, p, (ids, repeats), rng.standard_normal((c, h, w)), device)
+
+
+@pytest.mark.slow
+def test_largest_image(device):
+    """The tallest image of the operators' limits, 214 million pixels, with slots in its first and last rows alone: lists of 8.6 GB, and twelve
+    channels, whose planes pass 2^31 values."""
+    h, w, c, half = 65535 * 16, 204, 12, 20
+    top, bottom = 2, 5
+    rng = np.random.default_rng(77)
+    n = 2 * half
+    xys = rng.uniform(0, [w, 5], (n, 2))
+    xys[half:, 1] += h - bottom
+    xys, conics = np.float32(xys), np.tile(np.float32([0.02, 0.003, 0.1]), (n, 1))
+    lists = torch.full((h, w, 10), -1, dtype=torch.int32, device=device)
+    ends = [rng.permuted(np.broadcast_to(np.arange(half), (rows, w, half)), axis=2)[..., :10] for rows in (top, bottom)]
+    ends[1] = ends[1] + half
+    lists[:top], lists[-bottom:] = torch.from_numpy(ends[0]).to(device), torch.from_numpy(ends[1]).to(device)
+    x, k = torch.from_numpy(xys).to(device), torch.from_numpy(conics).to(device)
+
+    def at_the_ends(what):  # what(rows, xys of these rows, lists, first pixel) at both ends; the halves of the Gaussians are apart
+        shifted = xys.astype(np.float64)
+        shifted[:, 1] -= h - bottom
+        return what(top, xys, ends[0], 0), what(bottom, shifted, ends[1], (h - bottom) * w)
+
+    loss, counts, importance, totals = ops.topk_balance_forward(h, w, x, k, lists)
+    both = at_the_ends(lambda rows, at, ids, _: routing.balance(rows, w, at, conics, ids))
+    o_counts, o_importance = (sum(b[i] for b in both) for i in (1, 2))
+    o_totals = tuple(sum(b[3][i] for b in both) for i in (0, 1))
+    assert np.array_equal(counts.cpu().numpy(), o_counts) and tuple(totals.tolist()) == o_totals == ((top + bottom) * w * 10, (top + bottom) * w)
+    gate = max(gate_tolerance(b[4]) for b in both)
+    check_sums(importance, o_importance, o_importance, gate + 64 * U, "importance", floor=1e-8)  # 2^-34 in each of some 52 patches
+    factor = n / (o_totals[0] * o_totals[1])
+    o_loss = factor * float((o_counts * o_importance).sum())
+    assert abs(float(loss) - o_loss) <= (gate + 64 * U) * o_loss + factor * float(o_counts.sum()) * 1e-8
+    grads = ops.topk_balance_backward(h, w, x, k, lists, counts, totals, torch.tensor(1.0, device=device))
+    alpha = factor * o_counts  # as an importance gradient, the counts and totals of one end being its own
+    parts = [routing.balance_grad(b[4], b[1], b[3], 0.0, alpha) for b in both]
+    v_xy, v_conic, m_xy, m_conic = (sum(p[i] for p in parts) for i in range(4))
+    rel = 2 * gate + (64 + o_counts.max()) * U
+    check_sums(grads[0], v_xy, m_xy, rel, "v_xy", floor=1e-30)
+    check_sums(grads[1], v_conic, m_conic, rel, "v_conic", floor=1e-30)
+
+    p, seed, offset = 0.3, 5, 6
+    colors = np.float32(rng.standard_normal((n, c)))
+    f = torch.from_numpy(colors).to(device)
+    image, used = ops.topk_dropout_forward(h, w, x, k, f, lists, p, torch.tensor([seed, offset], device=device))
+    assert not image[:, top:-bottom].any()
+    v = [np.float32(rng.standard_normal((c, rows, w))) for rows in (top, bottom)]
+    image_ends = image[:, :top].clone(), image[:, -bottom:].clone()
+    v_output = image.fill_(1.0)  # (10 GB: in place)
+    v_output[:, :top], v_output[:, -bottom:] = torch.from_numpy(v[0]).to(device), torch.from_numpy(v[1]).to(device)
+    grads = ops.topk_dropout_backward(h, w, x, k, f, v_output, lists, p, used)
+
+    def render(rows, at, ids, first):
+        words = [[routing.philox4x32((i, j, offset, 0), (seed, 0)) for j in (0, 1)] for i in range(first, first + rows * w)]
+        words = np.array(words, np.int64).reshape(-1, 8)
+        low = words & 255
+        tail = np.stack([low[:, i] << 16 | low[:, i + 1] << 8 | low[:, i + 2] for i in (0, 3)], 1)
+        kept = np.concatenate([words >> 8, tail], 1) >= int(np.rint(p * 2.0**24))
+        return routing.dropout(rows, w, at, conics, colors, ids, kept)
+
+    both = at_the_ends(render)
+    gate = max(gate_tolerance(g) for *_, g in both)
+    for got, (want, size, _) in zip(image_ends, both):
+        check_sums(got, want, size, gate + 32 * U, "image", floor=1e-30)
+    parts = [routing.dropout_grad(g, colors, v_end) for (*_, g), v_end in zip(both, v)]
+    sums = [sum(part[i] for part in parts) for i in range(6)]
+    for got, want, size, what in zip(grads, sums[:3], sums[3:], ("v_xy", "v_conic", "v_colors")):
+        check_sums(got, want, size, 2 * gate + (64 + o_counts.max()) * U, what, floor=1e-30)
