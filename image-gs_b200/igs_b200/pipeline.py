@@ -38,8 +38,9 @@ class RasterStep:
         balance: dict(factor, mask (optional, [H,W] bool or uint8 of any strides, read anew by every step)) adds the gradient of factor *
         the balance loss of the pixels over the Gaussians to the geometry's; the loss itself, the counts and the importance are in
         balance_loss, counts and importance.
-        gate_dropout: dict(p, rng_state (two int64 on the device side by side: seed and offset)) renders with gates dropped; the step ends by moving the
-        offset on by one, so that every launch and every replay draws another mask. Both run from the [H, W, 10] lists, not fused."""
+        gate_dropout: dict(p, rng_state (two int64 on the device side by side: seed and offset)) renders with gates dropped; the step ends
+        by moving the offset on by one, so that every launch and every replay draws another mask. Both run from the [H, W, 10] lists, not
+        fused."""
         self.balance, self.gate_dropout = balance, gate_dropout
         self.lists = balance is not None or gate_dropout is not None
         fused = fused and not self.lists
